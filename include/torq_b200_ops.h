@@ -90,6 +90,23 @@ enum tb200_op_kind {
                                * tests/testdata/torch_ops/matmul_dql_q8_0.mlir, ExpandWeightsPattern.cpp:350-376);
                                * weights int8 [K, N], bias slot = scales bf16 [K/i0, N], multiplier slot = zero
                                * points int8 [K/i0, N] or -1 */
+  /* A chunk of new tokens over a paged key/value cache (no counterpart in the reference, whose decoder passes one dense cache through).
+   * Ragged batch: rows row_start[s] .. row_start[s+1] - 1 (in1, i32 [S+1], ascending; a sequence may have none) are the new tokens of
+   * sequence s, at positions context[s], context[s] + 1, ... (in2, i32 [S]); rows in no sequence are padding, and what an op would write for
+   * them is left as it was. Position p of a sequence lies in page table[s][p / page_size] (multiplier slot, i32 [S, max_pages], bound or
+   * state); a page id outside [0, pages), or a position behind max_pages * page_size, holds nothing: writes to it are dropped, its keys are
+   * not seen, reads of it give zeros. Caches: shift slot = keys, table slot = values, [layers, pages, page_size, kv * D], bf16, or
+   * int8 with fp32 scales [layers, pages, page_size, 2 * kv] (bias slot; of the keys, then of the values): bound or state tensors that the
+   * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. */
+  TB200_OP_ROPE_KV_PAGED = 43,/* in0 = qkv [rows, (i0 + 2 kv) * D] -> out0 = rotated queries [rows, i0 * D]; keys and values go to their pages.
+                               * weights = bf16 norms [2, D] of queries and keys (x * rsqrt(mean(x^2) + f1) * (1 + w)) or -1; f0 = RoPE base >= 1.
+                               * fp32 inside, rounded once. int8: scale = amax / 127 of a token's head, nearest integer; a head with
+                               * a value that is not finite gets scale NaN. */
+  TB200_OP_KV_READ_PAGED = 44,/* out0 / out1 = keys / values [rows, kv * D] bf16 of the tokens at those positions (in0 = row_start, in1 = context) */
+  TB200_OP_ATTN_PAGED = 45,   /* in0 = queries [rows, i0 * D] -> out0 of the same shape: softmax(f0 * q k^T) v over the keys j <= p, and with
+                               * i3 = window > 0 only j > p - window or j < pad_b (first tokens that stay visible). Keys of masked
+                               * places count for nothing whatever they hold; a row that sees no key gets zeros. pad_l > 0: a promise
+                               * that no sequence has more new rows (those behind are left as they were). */
   /* tensor ops outside the layer set: what the reference's fixtures exercise around the layers
    * (tests/testdata/tosa_ops: cast-*, Elementwise_*, rescale-*, transpose-*, pad_*, identity-stride-offset-*,
    * reduce-*, argmax-*). Dense row-major tensors of rank <= 4, element types i8 / i16 / i32 / f32 / bf16;

@@ -9,6 +9,7 @@
 
 #include "chunk_divide.h"
 #include "common.cuh"
+#include "paged.h"
 
 namespace tb200 {
 
@@ -349,6 +350,41 @@ bool rmsnorm_row_applies(int H);
 // rmsnorm; with w2 a second norm without residual of its result goes to out2
 void launch_rmsnorm_row(const uint16_t* x, const uint16_t* res, const uint16_t* w, uint16_t* out, const uint16_t* w2, uint16_t* out2, int rows,
                         int H, float eps, float eps2, cudaStream_t stream);
+
+// ---- a chunk of tokens over a paged cache (paged_cache.cu, paged_attn.cu); caches and scales of one layer ----
+struct RopePagedArgs {
+  PagedView v;
+  const uint16_t* qkv;              // [rows][(n_q + 2 n_kv) * D]
+  const uint16_t* norms;            // [2][D], of the queries and of the keys, or null
+  const unsigned long long* turns;  // [D / 2], theta^(-2i / D) / 2 pi as a fraction of 2^64
+  uint16_t* q_out;                  // [rows][n_q * D]
+  void* k;
+  void* vv;
+  float* scales;                    // int8 caches, else null
+  int n_q, per;                     // per: heads a group of lanes takes (filled by the launcher)
+  float eps;
+};
+cudaError_t launch_rope_kv_paged(RopePagedArgs a, cudaStream_t stream);
+struct ReadPagedArgs {
+  PagedView v;
+  const void* k;
+  const void* vv;
+  const float* scales;
+  uint16_t* k_out;  // [rows][n_kv * D]
+  uint16_t* v_out;
+};
+cudaError_t launch_kv_read_paged(const ReadPagedArgs& a, cudaStream_t stream);
+struct AttnPagedArgs {
+  PagedView v;
+  const uint16_t* q;  // [rows][n_q * D]
+  const void* k;
+  const void* vv;
+  const float* scales;
+  uint16_t* out;      // [rows][n_q * D]
+  int n_q, window, sinks, max_new;  // max_new: most rows of a sequence, 0 = any number
+  float scale;
+};
+cudaError_t launch_attn_paged(const AttnPagedArgs& a, cudaStream_t stream);
 
 // ---- whole decode step as one persistent kernel (decode_step.cu) ----
 // Byte offsets: weights and norm vectors into the constant image, caches into the arena.

@@ -381,6 +381,71 @@ bool decode_per_op() {
   return e && *e && *e != '0';
 }
 
+// What the ops on a paged cache share: multiplier = page table [S, max_pages], shift / table = key / value pages [layers, pages, page_size,
+// kv * D], bias = scales [layers, pages, page_size, 2 * kv] of int8 pages; i1 = kv heads, i2 = head size, pad_t = layer. The pages and the scales are tensors the caller binds, or state: ops write them in place.
+struct PagedPlan {
+  PagedView v{};  // pointers are filled at dispatch
+  bool i8 = false;
+  size_t layer_bytes = 0, layer_scales = 0;  // byte offset of the layer in the pages, element offset in the scales
+};
+bool paged_plan(Builder& b, const tb200_op_t& op, int row_start, int context, int i, const char* name, PagedPlan& c) {
+  const auto& T = b.tensors;
+  auto held = [&](int id) { return b.valid_id(id) && (T[id].kind == TB200_TENSOR_INPUT || T[id].kind == TB200_TENSOR_STATE); };
+  if (!b.is_t(row_start, TB200_I32, 1) || !b.is_t(context, TB200_I32, 1) || !b.is_t(op.multiplier, TB200_I32, 2) || !held(op.multiplier) ||
+      T[row_start].shape[0] != T[context].shape[0] + 1 || T[op.multiplier].shape[0] != T[context].shape[0]) {
+    b.fail(TB200_INVALID_ARGUMENT, "op %d: %s wants i32 row starts [S+1], contexts [S] and a bound page table [S,max_pages]", i, name);
+    return false;
+  }
+  c.i8 = b.valid_id(op.shift) && T[op.shift].dtype == TB200_I8;
+  const uint32_t dtype = c.i8 ? TB200_I8 : TB200_BF16;
+  if (!b.is_t(op.shift, dtype, 4) || !b.is_t(op.table, dtype, 4) || !b.same_shape(op.shift, op.table) || !held(op.shift) || !held(op.table) ||
+      op.shift == op.table) {
+    b.fail(TB200_INVALID_ARGUMENT, "op %d: %s wants two bound bf16 or int8 caches [layers,pages,page_size,kv*D]", i, name);
+    return false;
+  }
+  const auto& p = T[op.shift];
+  const int n_kv = op.i1, D = op.i2, layer = op.pad_t;
+  if (n_kv < 1 || D < 1 || (long long)p.shape[3] != (long long)n_kv * D || layer < 0 || layer >= p.shape[0]) {
+    b.fail(TB200_INVALID_ARGUMENT, "op %d: %s: head counts or the layer do not match the caches", i, name);
+    return false;
+  }
+  if (D % 16 || D > 256 || T[context].shape[0] > 4096 || (long long)T[op.multiplier].shape[1] * p.shape[2] > (1ll << 30)) {
+    b.fail(TB200_UNIMPLEMENTED, "op %d: %s supports head sizes of a multiple of 16 up to 256, 4096 sequences, 2^30 positions", i, name);
+    return false;
+  }
+  if (c.i8 != (op.bias >= 0) || (c.i8 && (!b.is_t(op.bias, TB200_F32, 4) || !held(op.bias) || T[op.bias].shape[0] != p.shape[0] ||
+                                          T[op.bias].shape[1] != p.shape[1] || T[op.bias].shape[2] != p.shape[2] || T[op.bias].shape[3] != 2 * n_kv))) {
+    b.fail(TB200_INVALID_ARGUMENT, "op %d: %s: int8 caches (and no others) come with bound f32 scales [layers,pages,page_size,2*kv]", i, name);
+    return false;
+  }
+  c.v.S = T[context].shape[0];
+  c.v.max_pages = T[op.multiplier].shape[1];
+  c.v.pages = p.shape[1];
+  c.v.page_size = p.shape[2];
+  c.v.n_kv = n_kv;
+  c.v.D = D;
+  c.v.capacity = c.v.max_pages * c.v.page_size;
+  c.v.div = page_divisor(c.v.page_size);
+  const size_t slots = (size_t)layer * p.shape[1] * p.shape[2];
+  c.layer_bytes = slots * p.shape[3] * (c.i8 ? 1 : 2);
+  c.layer_scales = slots * 2 * n_kv;
+  return true;
+}
+struct PagedLoc {
+  Loc row_start, context, pages_of, k, v, scales;
+  PagedView view(const PagedPlan& c, const ExecContext& x) const {
+    PagedView w = c.v;
+    w.row_start = (const int32_t*)row_start.resolve(x);
+    w.context = (const int32_t*)context.resolve(x);
+    w.table = (const int32_t*)pages_of.resolve(x);
+    return w;
+  }
+};
+template <typename F>
+PagedLoc paged_loc(const tb200_op_t& op, int row_start, int context, F& loc) {
+  return PagedLoc{loc(row_start), loc(context), loc(op.multiplier), loc(op.shift), loc(op.table), loc(op.bias)};
+}
+
 // Recognises the whole-graph shape of one decode step (embed; per layer rmsnorm, gemv,
 // rope_kv, attn_decode, gemv, rmsnorm+residual, rmsnorm, gemv, geglu, gemv, rmsnorm+residual;
 // final rmsnorm, gemv to fp32 logits, argmax) and replaces its per-op launches by the one
@@ -2091,10 +2156,25 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         if (op.i1 < 0 || op.i1 + K > tensors[op.in0].shape[1] || tensors[op.out0].shape[0] != B || tensors[op.out0].shape[1] != N)
           return b.fail(TB200_INVALID_ARGUMENT, "op %d: gemv_w8 shape mismatch", i);
         if (op.i1 != 0 || K != tensors[op.in0].shape[1]) needs_fusion = true;
-        if (K % 16 != 0 || B > 32) return b.fail(TB200_UNIMPLEMENTED, "op %d: gemv_w8 needs K %% 16 == 0 and batch <= 32", i);
+        if (K % 16 != 0) return b.fail(TB200_UNIMPLEMENTED, "op %d: gemv_w8 needs K %% 16 == 0", i);
         size_t w_off, s_off;
         if (!b.add_raw_const(op.weights, (size_t)N * K, "weights", i, w_off)) return b.status;
         if (!b.add_raw_const(op.bias, (size_t)N * 2, "scales", i, s_off)) return b.status;
+        if (B > 32) {  // the rows of a chunk, 32 at a time
+          const int splits = op.i0 > 0 ? op.i0 : gemv_w8_splits(32, N, K);
+          if (!gemv_w8_splits_fit(32, N, K, splits))
+            return b.fail(TB200_OUT_OF_RANGE, "op %d: %d K slices leave a slice longer than the tensor-core gemv_w8 can stage", i, splits);
+          scratch_need = std::max(scratch_need, gemv_w8_scratch_bytes(32, N, splits));
+          Loc lx = loc(op.in0), lo = loc(op.out0);
+          step.kernel_name = "gemv_w8_rows";
+          step.launches = (B + 31) / 32 * (splits > 1 ? 2 : 1);
+          step.launch = [=](const ExecContext& c) {
+            for (int r = 0; r < B; r += 32)
+              launch_gemv_w8((const uint16_t*)lx.resolve(c) + (size_t)r * K, (const int8_t*)(c.consts + w_off), (const uint16_t*)(c.consts + s_off),
+                             (char*)lo.resolve(c) + (size_t)r * N * (y_f32 ? 4 : 2), y_f32, (float*)c.scratch, std::min(32, B - r), N, K, splits, c.stream);
+          };
+          break;
+        }
         if (op.i0 <= 0 && op.i1 == 0 && K == tensors[op.in0].shape[1] && linear_w8_applies(B, N, K, y_f32 != 0)) {
           // the product after the next one: its weights have that long to come from memory
           size_t next_off = 0, next_bytes = 0;
@@ -2203,6 +2283,97 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         step.launch = [=](const ExecContext& c) {
           launch_attn_decode((const uint16_t*)lq.resolve(c), (const int32_t*)lp.resolve(c), (const uint16_t*)lk.resolve(c),
                              (const uint16_t*)lv.resolve(c), (uint16_t*)lo.resolve(c), B, n_q, T, window, scale, early, c.stream);
+        };
+        break;
+      }
+      case TB200_OP_ROPE_KV_PAGED: {
+        PagedPlan c;
+        if (!paged_plan(b, op, op.in1, op.in2, i, "rope_kv_paged", c)) return b.status;
+        const int n_q = op.i0;
+        if (!b.is_t(op.in0, TB200_BF16, 2) || !b.is_t(op.out0, TB200_BF16, 2) || n_q < 1 ||
+            (long long)tensors[op.in0].shape[1] != (n_q + 2ll * c.v.n_kv) * c.v.D || tensors[op.out0].shape[1] != n_q * c.v.D ||
+            tensors[op.out0].shape[0] != tensors[op.in0].shape[0])
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: rope_kv_paged wants bf16 qkv [rows,(q+2kv)*D] -> bf16 [rows,q*D]", i);
+        if (!(op.f0 >= 1.0f) || !(op.f1 >= 0.0f))
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: rope_kv_paged wants theta >= 1 and eps >= 0", i);
+        c.v.rows = tensors[op.in0].shape[0];
+        const bool norms = op.weights >= 0;
+        size_t n_off = 0;
+        if (norms && (!b.is_t(op.weights, TB200_BF16, 2) || b.numel(op.weights) != (size_t)2 * c.v.D))
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: rope_kv_paged wants bf16 norm weights [2,D]", i);
+        if (norms && !b.add_raw_const(op.weights, (size_t)4 * c.v.D, "norm weights", i, n_off)) return b.status;
+        std::vector<unsigned long long> turns(c.v.D / 2);
+        for (int j = 0; j < c.v.D / 2; j++)
+          turns[j] = (unsigned long long)llrintl(ldexpl(powl((long double)op.f0, -2.0L * j / c.v.D) / (2.0L * acosl(-1.0L)), 64));
+        const size_t t_off = b.add_const(turns.data(), turns.size() * sizeof(turns[0]));
+        Loc lx = loc(op.in0), lq = loc(op.out0);
+        const PagedLoc at = paged_loc(op, op.in1, op.in2, loc);
+        const float eps = op.f1;
+        step.kernel_name = c.i8 ? "rope_kv_paged_i8" : "rope_kv_paged";
+        step.launch = [=](const ExecContext& x) {
+          RopePagedArgs k{};
+          k.v = at.view(c, x);
+          k.qkv = (const uint16_t*)lx.resolve(x);
+          k.norms = norms ? (const uint16_t*)(x.consts + n_off) : nullptr;
+          k.turns = (const unsigned long long*)(x.consts + t_off);
+          k.q_out = (uint16_t*)lq.resolve(x);
+          k.k = (char*)at.k.resolve(x) + c.layer_bytes;
+          k.vv = (char*)at.v.resolve(x) + c.layer_bytes;
+          k.scales = c.i8 ? (float*)at.scales.resolve(x) + c.layer_scales : nullptr;
+          k.n_q = n_q;
+          k.eps = eps;
+          report(launch_rope_kv_paged(k, x.stream), x);
+        };
+        break;
+      }
+      case TB200_OP_KV_READ_PAGED: {
+        PagedPlan c;
+        if (!paged_plan(b, op, op.in0, op.in1, i, "kv_read_paged", c)) return b.status;
+        if (!b.is_t(op.out0, TB200_BF16, 2) || !b.is_t(op.out1, TB200_BF16, 2) || !b.same_shape(op.out0, op.out1) ||
+            tensors[op.out0].shape[1] != c.v.n_kv * c.v.D)
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: kv_read_paged wants two bf16 results [rows,kv*D]", i);
+        c.v.rows = tensors[op.out0].shape[0];
+        Loc lk = loc(op.out0), lv = loc(op.out1);
+        const PagedLoc at = paged_loc(op, op.in0, op.in1, loc);
+        step.kernel_name = c.i8 ? "kv_read_paged_i8" : "kv_read_paged";
+        step.launch = [=](const ExecContext& x) {
+          ReadPagedArgs k{};
+          k.v = at.view(c, x);
+          k.k = (const char*)at.k.resolve(x) + c.layer_bytes;
+          k.vv = (const char*)at.v.resolve(x) + c.layer_bytes;
+          k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
+          k.k_out = (uint16_t*)lk.resolve(x);
+          k.v_out = (uint16_t*)lv.resolve(x);
+          report(launch_kv_read_paged(k, x.stream), x);
+        };
+        break;
+      }
+      case TB200_OP_ATTN_PAGED: {
+        PagedPlan c;
+        if (!paged_plan(b, op, op.in1, op.in2, i, "attn_paged", c)) return b.status;
+        const int n_q = op.i0;
+        if (!b.is_t(op.in0, TB200_BF16, 2) || !b.is_t(op.out0, TB200_BF16, 2) || !b.same_shape(op.in0, op.out0) || n_q < 1 ||
+            (long long)tensors[op.in0].shape[1] != (long long)n_q * c.v.D)
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: attn_paged wants bf16 q [rows,q*D] -> bf16 of the same shape", i);
+        if (n_q % c.v.n_kv || n_q / c.v.n_kv > 64)
+          return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged wants a whole number of query heads, at most 64, to a key/value head", i);
+        if (op.i3 < 0 || op.pad_b < 0 || op.pad_l < 0 || !(op.f0 > 0.0f) || !std::isfinite(op.f0))
+          return b.fail(TB200_INVALID_ARGUMENT, "op %d: attn_paged wants window, sinks and max_new >= 0 and a positive scale", i);
+        c.v.rows = tensors[op.in0].shape[0];
+        AttnPagedArgs a{};
+        a.n_q = n_q; a.window = op.i3; a.sinks = op.pad_b; a.max_new = op.pad_l; a.scale = op.f0;
+        Loc lq = loc(op.in0), lo = loc(op.out0);
+        const PagedLoc at = paged_loc(op, op.in1, op.in2, loc);
+        step.kernel_name = "attn_paged";
+        step.launch = [=](const ExecContext& x) {
+          AttnPagedArgs k = a;
+          k.v = at.view(c, x);
+          k.q = (const uint16_t*)lq.resolve(x);
+          k.k = (const char*)at.k.resolve(x) + c.layer_bytes;
+          k.vv = (const char*)at.v.resolve(x) + c.layer_bytes;
+          k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
+          k.out = (uint16_t*)lo.resolve(x);
+          report(launch_attn_paged(k, x.stream), x);
         };
         break;
       }

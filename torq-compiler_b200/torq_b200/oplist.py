@@ -29,6 +29,7 @@ OP_KINDS = {
     "rescale": 9, "resize_nn2x": 10, "concat": 11, "sub": 12, "matmul_i32": 13, "reshape": 14,
     "embed": 32, "rmsnorm": 33, "gemv_w8": 34, "rope_kv": 35, "attn_decode": 36, "geglu": 37,
     "add_bf16": 38, "argmax": 39, "allreduce": 40, "act_bf16": 41, "gemv_q8b": 42,
+    "rope_kv_paged": 43, "kv_read_paged": 44, "attn_paged": 45,
     "ew": 48, "transpose": 49, "slice": 50, "pad": 51, "concat_axis": 52, "reduce": 53, "table16": 54, "softmax": 55, "conv2d_i16": 56, "permute": 57, "gather": 58, "scatter": 59, "matmul_f": 60, "depthwise_f": 61,
 }
 
@@ -461,6 +462,67 @@ class Graph:
         self.ops.append(Op("attn_decode", [q, pos, k_cache], [out], {"weights": v_cache},
                            dict(i0=n_q, i1=n_kv, i2=head_dim, i3=window, f0=float(scale))))
         return out
+
+    # ---- a chunk of new tokens over a paged cache ------------------------------
+    # Rows row_start[s] .. row_start[s + 1] - 1 are the new tokens of sequence s (row_start i32 [S + 1], ascending), at positions
+    # context[s], context[s] + 1, ... (i32 [S]); rows in no sequence are padding and keep what their results held. Position p lies in page
+    # page_table[s, p // page_size] (i32 [S, max_pages]); an id outside the cache (-1, say) holds nothing: writes are dropped,
+    # keys are not seen. k_pages / v_pages are [layers, pages, page_size, n_kv * head_dim], bf16, or i8 with
+    # scales f32 [layers, pages, page_size, 2 * n_kv]: inputs or state tensors, read and written in place (bind them with
+    # Executable.dispatch; a host call would write into its own copies).
+    def _paged(self, row_start, context, page_table, k_pages, v_pages, scales, n_kv, head_dim, layer):
+        S = context.shape[0]
+        if len(row_start.shape) != 1 or len(context.shape) != 1 or len(page_table.shape) != 2 or row_start.shape[0] != S + 1 or \
+                page_table.shape[0] != S or any(t.dtype != "i32" for t in (row_start, context, page_table)):
+            raise ValueError("a paged op wants i32 row_start [S + 1], context [S] and page_table [S, max_pages]")
+        if len(k_pages.shape) != 4 or v_pages.shape != k_pages.shape or k_pages.dtype not in ("bf16", "i8") or v_pages.dtype != k_pages.dtype or \
+                k_pages.shape[3] != n_kv * head_dim:
+            raise ValueError("a paged op wants bf16 or i8 k_pages and v_pages [layers, pages, page_size, n_kv * head_dim]")
+        if k_pages.id == v_pages.id or any(t is not None and t.kind not in (INPUT, STATE) for t in (page_table, k_pages, v_pages, scales)):
+            raise ValueError("page table, caches and scales are inputs or state tensors of their own")
+        if (scales is not None) != (k_pages.dtype == "i8") or \
+                (scales is not None and (scales.dtype != "f32" or tuple(scales.shape) != tuple(k_pages.shape[:3]) + (2 * n_kv,))):
+            raise ValueError("i8 caches come with f32 scales [layers, pages, page_size, 2 * n_kv], bf16 ones without")
+        if not 0 <= layer < k_pages.shape[0]:
+            raise ValueError("layer outside the cache")
+        consts = {"multiplier": page_table, "shift": k_pages, "table": v_pages}
+        if scales is not None:
+            consts["bias"] = scales
+        return consts, dict(i1=int(n_kv), i2=int(head_dim), pad_t=int(layer))
+
+    def rope_kv_paged(self, qkv, row_start, context, page_table, k_pages, v_pages, q_norm_w=None, k_norm_w=None, *, n_q, n_kv, head_dim,
+                      theta, eps=1e-6, layer=0, scales=None):
+        """Per-head RMSNorm (where norm weights are given) and rotary on the chunk's q and k [rows, (n_q + 2 n_kv) * head_dim]; k and v go to
+        their pages (i8: rounded to the nearest multiple of amax / 127 of each token's head). Returns the rotated queries
+        [rows, n_q * head_dim]."""
+        consts, attrs = self._paged(row_start, context, page_table, k_pages, v_pages, scales, n_kv, head_dim, layer)
+        if (q_norm_w is None) != (k_norm_w is None):
+            raise ValueError("rope_kv_paged wants norm weights for queries and keys, or for neither")
+        if len(qkv.shape) != 2 or qkv.dtype != "bf16" or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+            raise ValueError("rope_kv_paged wants bf16 qkv [rows, (n_q + 2 n_kv) * head_dim]")
+        if q_norm_w is not None:
+            consts["weights"] = self.const(np.stack([np.asarray(w, np.uint16) for w in (q_norm_w, k_norm_w)]), "bf16")
+        return self._emit("rope_kv_paged", [qkv, row_start, context], (qkv.shape[0], n_q * head_dim), "bf16", consts=consts, i0=int(n_q),
+                          f0=float(theta), f1=float(eps), **attrs)
+
+    def kv_read_paged(self, row_start, first, page_table, k_pages, v_pages, *, rows, n_kv, head_dim, layer=0, scales=None):
+        """The keys and values of the tokens at positions first[s], first[s] + 1, ... as two bf16 tensors [rows, n_kv * head_dim]: rows
+        row_start[s] .. row_start[s + 1] - 1 are those of sequence s. Positions that hold nothing read as zeros."""
+        consts, attrs = self._paged(row_start, first, page_table, k_pages, v_pages, scales, n_kv, head_dim, layer)
+        k, v = (self._tensor((rows, n_kv * head_dim), "bf16", ACTIVATION) for _ in range(2))
+        self.ops.append(Op("kv_read_paged", [row_start, first], [k, v], consts, attrs))
+        return k, v
+
+    def attn_paged(self, q, row_start, context, page_table, k_pages, v_pages, *, n_q, n_kv, head_dim, scale, window=0, sinks=0, max_new=0,
+                   layer=0, scales=None):
+        """Causal attention of the chunk's queries [rows, n_q * head_dim] over the cached keys, the chunk's own included (write them first). A
+        token at position p sees the keys j <= p; with a window only j > p - window and the first `sinks` tokens. max_new: no sequence has
+        more new rows than this (1 for a decode step; 0 = any number). A row that sees no key gets zeros."""
+        consts, attrs = self._paged(row_start, context, page_table, k_pages, v_pages, scales, n_kv, head_dim, layer)
+        if len(q.shape) != 2 or q.dtype != "bf16" or q.shape[1] != n_q * head_dim or n_q % n_kv:
+            raise ValueError("attn_paged wants bf16 q [rows, n_q * head_dim], n_q a multiple of n_kv")
+        return self._emit("attn_paged", [q, row_start, context], q.shape, "bf16", consts=consts, i0=int(n_q), i3=int(window), pad_b=int(sinks),
+                          pad_l=int(max_new), f0=float(scale), **attrs)
 
     def geglu(self, gate_up):
         """y = bf16(bf16(gelu_tanh(gate)) * up), gate = first half of the columns."""
