@@ -383,8 +383,22 @@ struct AttnPagedArgs {
   uint16_t* out;      // [rows][n_q * D]
   int n_q, window, sinks, max_new;  // max_new: most rows of a sequence, 0 = any number
   float scale;
+  float* partial;      // attn_paged_partial_bytes: sums of tiles that several blocks share
+  uint32_t* counters;  // attn_paged_counter_bytes, zero before the first launch and left so
+  int* status;
+  // filled by attn_paged_shape
+  int tokens_per_tile, max_tiles, grid;
+  PageDivisor group_div;
+  // filled by the launchers
+  int few_rows;        // sequences with at most so many rows (tokens x query heads of a key/value head) are the other kernel's
+  unsigned long long wait_ns;
 };
-cudaError_t launch_attn_paged(const AttnPagedArgs& a, cudaStream_t stream);
+constexpr int kTileMinBlocks = 2;  // least key blocks a block of the grid is started for
+void attn_paged_shape(AttnPagedArgs& a, int sms);
+size_t attn_paged_counter_bytes(const AttnPagedArgs& a);
+size_t attn_paged_partial_bytes(const AttnPagedArgs& a);
+cudaError_t launch_attn_paged(AttnPagedArgs a, cudaStream_t stream);
+cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream);
 
 // ---- whole decode step as one persistent kernel (decode_step.cu) ----
 // Byte offsets: weights and norm vectors into the constant image, caches into the arena.

@@ -39,4 +39,42 @@ struct PagedView {
   PageDivisor div;
 };
 
+// ---- how attention cuts a chunk into tiles, and shares the tiles' work out ----
+// A tile is up to tokens_per_tile new tokens of a sequence with the query heads of one key/value head; its work is the blocks of kKeyBlock
+// keys that one of its tokens may see: those of the first tokens that stay visible, then those from the window's start on.
+constexpr int kKeyBlock = 128;
+struct TileSpan {
+  int sink_blocks;  // key blocks 0 .. sink_blocks - 1 come first
+  int near_block;   // then near_block, near_block + 1, ...
+  int blocks;       // in all; at least one, so that a tile that sees nothing is visited as well
+  int near_key;     // keys in front of it are seen as first tokens only
+  int end_key;      // one past the last key a token of the tile sees
+};
+TB200_BOTH long long span_min(long long a, long long b) { return a < b ? a : b; }
+TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int window, int sinks, int capacity) {
+  const long long first = (long long)ctx + (long long)tile * tokens_per_tile;
+  const long long end = span_min((long long)ctx + span_min((long long)(tile + 1) * tokens_per_tile, n), capacity);
+  long long near = window > 0 && first - window + 1 > 0 ? first - window + 1 : 0;
+  near = span_min(near, end);
+  TileSpan s;
+  s.near_key = (int)near;
+  s.end_key = (int)end;
+  s.near_block = (int)(near / kKeyBlock);
+  const int sink_blocks = (int)span_min((sinks + (long long)kKeyBlock - 1) / kKeyBlock, s.near_block);
+  s.sink_blocks = sink_blocks;
+  const int last = (int)((end + kKeyBlock - 1) / kKeyBlock);
+  s.blocks = sink_blocks + (last > s.near_block ? last - s.near_block : 0);
+  if (s.blocks < 1) s.blocks = 1;
+  return s;
+}
+TB200_BOTH int tile_block(const TileSpan& s, int i) { return i < s.sink_blocks ? i : s.near_block + (i - s.sink_blocks); }
+// `total` pieces of work in one row, shared out to `parts`: part i begins here
+TB200_BOTH long long work_begin(long long total, int i, int parts) { return total * i / parts; }
+TB200_BOTH int work_owner(long long w, long long total, int parts) {
+  int c = (int)(w * parts / total);
+  while (c + 1 < parts && work_begin(total, c + 1, parts) <= w) c++;
+  while (c > 0 && work_begin(total, c, parts) > w) c--;
+  return c;
+}
+
 }  // namespace tb200

@@ -1,0 +1,718 @@
+// Attention of many rows over a paged cache on the tensor cores (paged.cuh, paged.h: tiles and the sharing-out of their work).
+//
+// A tile is 128 rows: up to 128 / group tokens with the query heads of one key/value head. Per block of 128 keys: S = Q K^T into TMEM
+// (fp32), softmax in registers against a running maximum, P as bf16 back into TMEM, O += P V with P as the TMEM operand. S is double
+// buffered, so the product of the next block runs while this block's softmax does; O (up to 256 columns) and both S fill TMEM.
+//   p = 2^((s - m) scale log2 e), sums in fp32; m is the row's maximum, but follows it only when it has grown by more than 2^8 in
+//   p (O and the sum are scaled then): a bound serves as well as the maximum itself, and most blocks leave O alone.
+// Warps: eight for softmax (two to a row quarter, half a row's keys each), four that copy, one that issues the matrix instructions.
+// Copies gather: each key row's place comes from the page table, so any page size and any sequence end fits; a unit is 128 keys
+// x 64 dims in the 128-byte swizzle, zeros where a key is seen by no row of the tile. Keys are the K-major operand, values the same
+// bytes read as MN-major.  int8 caches are widened to bf16 (exact) on the way; the keys' scales meet the scores, the values' scales P.
+// Work is shared out evenly: all tiles' key blocks in one row, every block of the grid takes an equal piece. A tile that falls to
+// several leaves partial sums in memory, which the last one to arrive adds up in their order (results do not depend on who that is).
+#include <algorithm>
+
+#include "dependent_launch.cuh"
+#include "kernels.h"
+#include "paged.cuh"
+#include "paged_row.cuh"
+#include "tcgen05_ptx.cuh"
+
+namespace tb200 {
+
+namespace {
+
+constexpr int kSoftmaxWarps = 8, kCopyWarps = 4, kThreads = (kSoftmaxWarps + kCopyWarps + 1) * 32;
+constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
+constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
+constexpr int kMetaBlocks = 8;
+static_assert(kSoftmaxThreads == kRowThreads, "the plain row is computed by the softmax warps");
+
+struct Meta {
+  float k_scale[kKeyBlock], v_scale[kKeyBlock];
+  uint32_t holds[4];  // a bit for each key of the block: its page holds something
+};
+struct Control {
+  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty;
+  uint32_t tmem, bad_rows[4], arrived;
+  int abort;
+  float top[2][2][128];  // row maxima of the two halves, by parity of the block
+  long long totals[32], start_rem;
+  int start_seq, start_tile, start_index, start_off;
+};
+
+// what a sequence brings
+struct Span {
+  int row0, n, ctx;
+};
+__device__ __forceinline__ Span span_of(const AttnPagedArgs& a, int s) {
+  Span r;
+  r.row0 = max(a.v.row_start[s], 0);
+  r.n = max(0, min(a.v.row_start[s + 1], a.v.rows) - r.row0);
+  if (a.max_new) r.n = min(r.n, a.max_new);
+  r.ctx = max(a.v.context[s], 0);
+  return r;
+}
+__device__ __forceinline__ int tiles_of(const AttnPagedArgs& a, const Span& s) {
+  return s.n * (a.n_q / a.v.n_kv) > a.few_rows ? (s.n + a.tokens_per_tile - 1) / a.tokens_per_tile : 0;
+}
+
+// A block's items, one after another: (head, tile, a range of the tile's key blocks). Every role walks them by itself.
+struct Walker {
+  long long cur, end;
+  int head, seq, tile, index, tiles, n_tiles, off;
+  Span span;
+  TileSpan ts;
+  int b0, b1;
+
+  __device__ __forceinline__ void load_tile(const AttnPagedArgs& a) {
+    ts = tile_span(span.ctx, span.n, tile, a.tokens_per_tile, a.window, a.sinks, a.v.capacity);
+    b0 = off;
+    b1 = (int)min((long long)ts.blocks, off + (end - cur));
+  }
+  __device__ __forceinline__ bool split() const { return b0 > 0 || b1 < ts.blocks; }
+  __device__ __forceinline__ void start(const AttnPagedArgs& a, const Control& c, long long begin, long long end_, long long per_head, int n_tiles_) {
+    cur = begin; end = end_; n_tiles = n_tiles_;
+    head = (int)(begin / per_head);
+    seq = c.start_seq; tile = c.start_tile; index = c.start_index; off = c.start_off;
+    span = span_of(a, seq);
+    tiles = tiles_of(a, span);
+    load_tile(a);
+  }
+  __device__ __forceinline__ bool next(const AttnPagedArgs& a) {
+    cur += b1 - b0;
+    if (cur >= end) return false;
+    off = 0;
+    tile++;
+    if (++index >= n_tiles) {  // the next head begins
+      index = 0;
+      head++;
+      seq = -1;
+      tile = tiles;
+    }
+    if (tile >= tiles) {
+      tile = 0;
+      do {
+        if (++seq >= a.v.S) seq = 0;  // there is a tile, so a sequence with one
+        span = span_of(a, seq);
+        tiles = tiles_of(a, span);
+      } while (!tiles);
+    }
+    load_tile(a);
+    return true;
+  }
+};
+
+// Sum over the block's threads (or the running sum up to and including this thread), through c.totals.
+__device__ long long block_total(Control& c, long long x, bool running) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  long long v = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) c.totals[warp] = v;
+  __syncthreads();
+  long long all = 0, before = 0;
+  for (int w = 0; w < kThreads / 32; w++) {
+    if (w < warp) before += c.totals[w];
+    all += c.totals[w];
+  }
+  return running ? before + v : all;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// four int8 -> four bf16, exact: 0x4300 | low seven bits of the biased byte is 128 + those bits, and 128 or 256 comes off again
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u, low = u & 0x7f7f7f7fu, off = ~u & 0x80808080u;
+  const uint32_t a0 = __byte_perm(low, 0x43434343u, 0x4140), a1 = __byte_perm(low, 0x43434343u, 0x4342);
+  const uint32_t c0 = __byte_perm(off, 0x43434343u, 0x4140), c1 = __byte_perm(off, 0x43434343u, 0x4342);
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a0), "r"(c0));
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(a1), "r"(c1));
+}
+__device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {  // zeros when not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+
+// DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
+template <int DC, int UNITS, bool I8>
+__global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const AttnPagedArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  // [Q units][ring units] on 1024-byte boundaries, then the rest
+  unsigned char* const base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t q_smem = smem_u32(base), ring = q_smem + DC * kUnit;
+  Meta* const meta = reinterpret_cast<Meta*>(base + (DC + UNITS) * kUnit);
+  RowScratch& plain = *reinterpret_cast<RowScratch*>(meta + kMetaBlocks);
+  Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(RowScratch));
+  int* const first_tile = reinterpret_cast<int*>(base);  // while the work is shared out: tiles in front of each sequence
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const PagedView& v = a.v;
+  const int group = a.n_q / v.n_kv, D = v.D, tpt = a.tokens_per_tile;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    for (int i = 0; i < UNITS; i++) {
+      mbar_init(smem_u32(&c.full[i]), kCopyThreads);
+      mbar_init(smem_u32(&c.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; i++) {  // a softmax warp may be one block ahead of another: a barrier for each buffer
+      mbar_init(smem_u32(&c.s_full[i]), 1);
+      mbar_init(smem_u32(&c.p_ready[i]), kSoftmaxThreads);
+    }
+    mbar_init(smem_u32(&c.pv_done), 1);
+    mbar_init(smem_u32(&c.o_done), 1);
+    mbar_init(smem_u32(&c.q_full), kCopyThreads);
+    mbar_init(smem_u32(&c.q_empty), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    c.abort = 0;
+    c.bad_rows[0] = c.bad_rows[1] = c.bad_rows[2] = c.bad_rows[3] = 0;
+  }
+  grid_dependency_wait();
+  grid_dependency_release();
+
+  // ---- the work: tiles of the sequences, key blocks of the tiles ----
+  int run = 0;
+  for (int s0 = 0; s0 < v.S; s0 += kThreads) {
+    const int s = s0 + tid;
+    const int mine = s < v.S ? tiles_of(a, span_of(a, s)) : 0;
+    const int upto = run + (int)block_total(c, mine, true);
+    if (s < v.S) first_tile[s + 1] = upto;
+    run += (int)block_total(c, mine, false);
+  }
+  if (tid == 0) first_tile[0] = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = c.tmem;
+  const int n_tiles = min(run, a.max_tiles);
+  auto locate = [&](int i, int& seq) {
+    int lo = 0, hi = v.S - 1;  // the last sequence with first_tile[seq] <= i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_tile[mid] <= i) lo = mid;
+      else hi = mid - 1;
+    }
+    seq = lo;
+    return i - first_tile[lo];
+  };
+  auto blocks_of = [&](int i) {
+    int seq;
+    const int t = locate(i, seq);
+    const Span sp = span_of(a, seq);
+    return tile_span(sp.ctx, sp.n, t, tpt, a.window, a.sinks, v.capacity).blocks;
+  };
+  long long mine = 0;
+  for (int i = tid; i < n_tiles; i += kThreads) mine += blocks_of(i);
+  const long long per_head = block_total(c, mine, false), total = per_head * v.n_kv;
+  const int parts = (int)max(1ll, min((long long)gridDim.x, total / kTileMinBlocks));
+  const bool works = total > 0 && (int)blockIdx.x < parts;
+  const long long begin = works ? work_begin(total, blockIdx.x, parts) : 0, end = works ? work_begin(total, blockIdx.x + 1, parts) : 0;
+  if (works) {
+    const long long rem = begin % per_head;
+    long long before = 0;
+    for (int i0 = 0; i0 < n_tiles && before <= rem; i0 += kThreads) {
+      const int i = i0 + tid, n = i < n_tiles ? blocks_of(i) : 0;
+      const long long upto = before + block_total(c, n, true);
+      if (n && upto > rem && upto - n <= rem) {
+        int seq;
+        c.start_tile = locate(i, seq);
+        c.start_seq = seq;
+        c.start_index = i;
+        c.start_off = (int)(rem - (upto - n));
+      }
+      before += block_total(c, n, false);
+    }
+  }
+  __syncthreads();  // the start is known, and first_tile's room is free
+
+  bool gave_up = false;
+  auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
+    // one wait that ran out ends all others at once: every role then runs through without waiting, and the results are not used
+    if (gave_up) return;
+    const uint32_t at = smem_u32(&bar);
+    if (mbar_poll(at, parity, 256)) return;
+    const unsigned long long t0 = globaltimer_ns();
+    for (;;) {
+      if (mbar_poll(at, parity, 256)) return;
+      if (*(volatile int*)&c.abort) break;
+      if (globaltimer_ns() - t0 > a.wait_ns) {
+        report_expired_wait(a.status, code);
+        *(volatile int*)&c.abort = 1;
+        break;
+      }
+    }
+    gave_up = true;
+  };
+
+  const uint32_t o_tmem = tmem + 256;
+  if (works && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
+    // ------------------------------------------------ copies
+    const int t = tid - kSoftmaxThreads;
+    uint32_t unit = 0;       // units asked for so far
+    uint32_t signalled = 0;  // units handed over
+    uint32_t items = 0, blocks = 0;
+    auto hand_over = [&](uint32_t upto) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      for (; signalled < upto; signalled++) mbar_arrive(smem_u32(&c.full[signalled % UNITS]));
+    };
+    auto drain = [&]() {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      hand_over(unit);
+    };
+    auto slot_free = [&]() {  // room for unit `unit`
+      if (unit < UNITS) return;
+      const uint32_t bar = smem_u32(&c.empty[unit % UNITS]), parity = (unit / UNITS - 1) & 1;
+      if (mbar_try_wait(bar, parity)) return;
+      drain();  // nothing that has arrived is held back while this waits
+      wait(c.empty[unit % UNITS], parity, 301);
+    };
+    const char* const kp = (const char*)a.k;
+    const char* const vp = (const char*)a.vv;
+    constexpr int kRows = I8 ? 4 : 8;           // rows of a unit that a thread copies a piece of
+    constexpr int kPieces = I8 ? 4 : 8;         // pieces of 16 bytes in a unit's row
+    const int piece = t % kPieces, row0 = t / kPieces;
+    constexpr int kRowStep = kCopyThreads / kPieces;
+    const long long row_bytes = (long long)v.n_kv * D * (I8 ? 1 : 2);
+    Walker w;
+    w.start(a, c, begin, end, per_head, n_tiles);
+    do {
+      const long long head_bytes = (long long)w.head * D * (I8 ? 1 : 2);
+      // queries
+      if (items && !mbar_try_wait(smem_u32(&c.q_empty), (items - 1) & 1)) {
+        drain();  // the scores that free the queries need the units still held back
+        wait(c.q_empty, (items - 1) & 1, 302);
+      }
+      {
+        const int qp = t & 7, used = min(tpt, w.span.n - w.tile * tpt) * group;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int r = (t >> 3) + 16 * i, tok = page_of(r, a.group_div), h = r - tok * group;
+          const bool ok = r < used;
+          const uint16_t* src = a.q + ((long long)(w.span.row0 + w.tile * tpt + (ok ? tok : 0)) * a.n_q + w.head * group + (ok ? h : 0)) * D;
+#pragma unroll
+          for (int u = 0; u < DC; u++) {
+            const int d = u * 64 + qp * 8;
+            copy16(q_smem + u * kUnit + r * 128 + ((qp ^ (r & 7)) << 4), src + (d < D ? d : 0), ok && d < D);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        drain();
+        mbar_arrive(smem_u32(&c.q_full));
+      }
+      items++;
+      const int n = w.b1 - w.b0;
+      // the slots of this thread's rows of a block; -1 where no token of the tile sees the key
+      auto slots_of = [&](int b, long long (&slot)[kRows]) {
+        const int key0 = tile_block(w.ts, w.b0 + b) * kKeyBlock;
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+          const int key = key0 + row0 + kRowStep * i;
+          const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
+          slot[i] = wanted ? slot_of(v, w.seq, key) : -1;
+        }
+      };
+      auto copy_units = [&](const char* pages, const long long (&slot)[kRows]) {
+#pragma unroll
+        for (int u = 0; u < DC; u++) {
+          slot_free();
+          const uint32_t dst = ring + (unit % UNITS) * kUnit;
+          const int d = u * 64 + piece * (I8 ? 16 : 8);
+#pragma unroll
+          for (int i = 0; i < kRows; i++) {
+            const int r = row0 + kRowStep * i;
+            const bool ok = slot[i] >= 0 && d < D;
+            const char* src = pages + (slot[i] >= 0 ? slot[i] : 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
+            if (!I8) {
+              copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src, ok);
+            } else {
+              uint4 x = ok ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+              uint4 lo, hi;
+              widen4(x.x, lo.x, lo.y); widen4(x.y, lo.z, lo.w);
+              widen4(x.z, hi.x, hi.y); widen4(x.w, hi.z, hi.w);
+              sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
+              sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
+            }
+          }
+          if (!I8) asm volatile("cp.async.commit_group;" ::: "memory");
+          unit++;
+          if (I8) {
+            hand_over(unit);
+          } else {  // three units stay in flight
+            asm volatile("cp.async.wait_group 3;" ::: "memory");
+            if (unit > 3 + signalled) hand_over(unit - 3);
+          }
+        }
+      };
+      for (int b = 0; b <= n; b++) {
+        if (b < n) {
+          long long slot[kRows];
+          slots_of(b, slot);
+          Meta& m = meta[blocks % kMetaBlocks];
+          blocks++;
+          const int key0 = tile_block(w.ts, w.b0 + b) * kKeyBlock;
+          {  // what this block's keys are, by one thread a key
+            const int key = key0 + t;
+            const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
+            const long long s = wanted ? slot_of(v, w.seq, key) : -1;
+            const uint32_t bits = __ballot_sync(0xffffffffu, s >= 0);
+            if (lane == 0) m.holds[t >> 5] = bits;
+            if (I8) {
+              const float* sc = a.scales + (s >= 0 ? s : 0) * 2 * v.n_kv + w.head;
+              m.k_scale[t] = s >= 0 ? __ldg(sc) : 0.f;
+              m.v_scale[t] = s >= 0 ? __ldg(sc + v.n_kv) : 0.f;
+            }
+          }
+          copy_units(kp, slot);
+        }
+        if (b > 0) {
+          long long slot[kRows];
+          slots_of(b - 1, slot);
+          copy_units(vp, slot);
+        }
+      }
+    } while (w.next(a));
+    drain();
+  } else if (works && warp == kSoftmaxWarps + kCopyWarps) {
+    // ------------------------------------------------ matrix instructions
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1024 bytes apart, sm_100 descriptor, 128-byte swizzle
+    const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kKeyBlock >> 3) << 17) | (8u << 24);
+    uint32_t unit = 0, blocks = 0, items = 0;
+    auto lo_of = [](uint32_t at) { return ((at & 0x3FFFF) >> 4) | (64u << 16); };
+    Walker w;
+    w.start(a, c, begin, end, per_head, n_tiles);
+    do {
+      wait(c.q_full, items & 1, 303);
+      items++;
+      const int n = w.b1 - w.b0;
+      for (int b = 0; b <= n; b++) {
+        if (b < n) {  // scores of block b
+          const uint32_t s_tmem = tmem + ((blocks + b) & 1) * 128;
+#pragma unroll
+          for (int u = 0; u < DC; u++) {
+            wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
+            tc_fence_after();
+            const uint32_t qa = lo_of(q_smem + u * kUnit), kb = lo_of(ring + (unit % UNITS) * kUnit);
+            const int steps = min(4, (D - u * 64) >> 4);
+            for (int k = 0; k < steps; k++) mma_f16_elect(s_tmem, qa + 2 * k, hi, kb + 2 * k, hi, idesc_s, (u | k) ? 1u : 0u);
+            mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
+            unit++;
+          }
+          mma_commit_elect(smem_u32(&c.s_full[(blocks + b) & 1]));
+          if (b == n - 1) mma_commit_elect(smem_u32(&c.q_empty));
+        }
+        if (b > 0) {  // sums of block b - 1
+          const uint32_t g = blocks + b - 1, p_tmem = tmem + (g & 1) * 128;
+          wait(c.p_ready[g & 1], (g >> 1) & 1, 305);
+          tc_fence_after();
+#pragma unroll
+          for (int u = 0; u < DC; u++) {
+            wait(c.full[unit % UNITS], (unit / UNITS) & 1, 306);
+            tc_fence_after();
+            const int width = min(64, D - u * 64);
+            const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(width >> 3) << 17) | (8u << 24);
+            const uint32_t vb = lo_of(ring + (unit % UNITS) * kUnit);
+#pragma unroll
+            for (int k = 0; k < 8; k++)  // keys 0..63 of P lie in columns 0..31, keys 64..127 in columns 64..95
+              mma_f16_ts_elect(o_tmem + u * 64, p_tmem + (k < 4 ? k * 8 : 64 + (k - 4) * 8), vb + k * (2048 >> 4), hi, idesc_o, (b > 1 || k > 0) ? 1u : 0u);
+            mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
+            unit++;
+          }
+          mma_commit_elect(smem_u32(&c.pv_done));
+          if (b == n) mma_commit_elect(smem_u32(&c.o_done));
+        }
+      }
+      blocks += n;
+    } while (w.next(a));
+  } else if (works) {
+    // ------------------------------------------------ softmax: thread = (row, half of the block's keys)
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int tok = page_of(row, a.group_div), pieces = D >> 4;
+    const float cexp = a.scale * 1.4426950408889634f;
+    uint32_t blocks = 0, items = 0;
+    Walker w;
+    w.start(a, c, begin, end, per_head, n_tiles);
+    do {
+      const int tokens = min(tpt, w.span.n - w.tile * tpt), used = tokens * group, n = w.b1 - w.b0;
+      const bool warp_used = (warp & 3) * 32 < used;
+      const long long p64 = (long long)w.span.ctx + w.tile * tpt + min(tok, tokens - 1);
+      const int pos = (int)min(p64, 0x7fffffffll);
+      const int first_pos = (int)min((long long)w.span.ctx + w.tile * tpt, 0x7fffffffll);
+      const int last_pos = (int)min((long long)w.span.ctx + w.tile * tpt + tokens - 1, 0x7fffffffll);
+      const int near = a.window ? max(0, pos - a.window + 1) : 0;  // this row sees keys [near, pos] and those in front of sinks
+      float m = -INFINITY, sum = 0.f;
+      for (int b = 0; b < n; b++, blocks++) {
+        const uint32_t s_tmem = tmem + lanes + (blocks & 1) * 128 + half * 64;
+        if (!warp_used) {  // rows of nobody: P keeps what it holds, and so does O
+          wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
+          mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
+          continue;
+        }
+        wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
+        tc_fence_after();
+        uint32_t s0[32], s1[32];
+        tmem_ld32_issue(s_tmem, s0);
+        tmem_ld32_issue(s_tmem + 32, s1);
+        const Meta& mt = meta[blocks % kMetaBlocks];
+        const int block = tile_block(w.ts, w.b0 + b), key0 = block * kKeyBlock + half * 64;
+        const uint32_t holds0 = mt.holds[half * 2], holds1 = mt.holds[half * 2 + 1];
+        const bool partial = (holds0 & holds1) != 0xffffffffu || key0 + 63 > first_pos ||
+                             (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
+        tmem_ld_wait32(s0);
+        tmem_ld_wait32(s1);
+        if (I8) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&mt.k_scale[half * 64 + i]), y = *reinterpret_cast<const float4*>(&mt.k_scale[half * 64 + 32 + i]);
+            s0[i] = __float_as_uint(__uint_as_float(s0[i]) * x.x); s0[i + 1] = __float_as_uint(__uint_as_float(s0[i + 1]) * x.y);
+            s0[i + 2] = __float_as_uint(__uint_as_float(s0[i + 2]) * x.z); s0[i + 3] = __float_as_uint(__uint_as_float(s0[i + 3]) * x.w);
+            s1[i] = __float_as_uint(__uint_as_float(s1[i]) * y.x); s1[i + 1] = __float_as_uint(__uint_as_float(s1[i + 1]) * y.y);
+            s1[i + 2] = __float_as_uint(__uint_as_float(s1[i + 2]) * y.z); s1[i + 3] = __float_as_uint(__uint_as_float(s1[i + 3]) * y.w);
+          }
+        }
+        if (partial) {
+          const uint32_t none = __float_as_uint(-INFINITY);
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            const int k0 = key0 + i, k1 = k0 + 32;
+            const bool see0 = k0 <= pos && (k0 >= near || k0 < a.sinks) && (holds0 >> i & 1);
+            const bool see1 = k1 <= pos && (k1 >= near || k1 < a.sinks) && (holds1 >> i & 1);
+            s0[i] = see0 ? s0[i] : none;
+            s1[i] = see1 ? s1[i] : none;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i++) top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+        c.top[blocks & 1][half][row] = top;
+        named_sync(1 + (warp & 3), 64);
+        top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
+        // follow the maximum when p could grow beyond 2^8, or when there was none yet
+        const bool grows = top > m && !((top - m) * cexp <= 8.f);
+        if (b == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, grows)) {
+          const float keep = grows ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * cexp)) : 1.f;
+          if (grows) m = top;
+          sum *= keep;
+          // these scores were issued behind the sums of the block before the last: its phase is over, the last one's is waited for
+          wait(c.pv_done, (blocks - 1) & 1, 308);
+          tc_fence_after();
+          for (int i = half; i < pieces; i += 2) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + lanes + i * 16, o);
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+            tmem_st16(o_tmem + lanes + i * 16, o);
+          }
+          tmem_st_wait();
+        }
+        const float from = m == -INFINITY ? 0.f : m;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        auto weights = [&](uint32_t (&s)[32], const float* v_scale, uint32_t holds, uint32_t to) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x = exp2_fast((__uint_as_float(s[i]) - from) * cexp), y = exp2_fast((__uint_as_float(s[i + 1]) - from) * cexp);
+            part[i & 2] += x;
+            part[(i & 2) + 1] += y;
+            if (I8) {
+              const float2 vs = *reinterpret_cast<const float2*>(v_scale + i);
+              x *= vs.x;
+              y *= vs.y;
+            }
+            p[i >> 1] = pack_bf16(x, y);
+          }
+          tmem_st16(to, p);
+        };
+        weights(s0, mt.v_scale + half * 64, holds0, s_tmem);
+        weights(s1, mt.v_scale + half * 64 + 32, holds1, s_tmem + 16);
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
+      }
+      // ---- the item's rows: finished, or left for whoever finishes the tile
+      wait(c.o_done, items & 1, 309);
+      items++;
+      tc_fence_after();
+      c.top[0][half][row] = sum;
+      named_sync(5, kSoftmaxThreads);
+      const float l = c.top[0][0][row] + c.top[0][1][row];
+      named_sync(5, kSoftmaxThreads);
+      const bool mine = row < used;
+      const int my_row = w.span.row0 + w.tile * tpt + tok, my_head = w.head * group + row - tok * group;
+      uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
+      bool finite = true;
+      auto store = [&](int piece, const float (&o)[16], float inv) {
+        uint32_t p[8];
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+          const float x = o[j] * inv, y = o[j + 1] * inv;
+          finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
+          p[j >> 1] = pack_bf16(x, y);
+        }
+        uint4* to = reinterpret_cast<uint4*>(dst + piece * 16);
+        to[0] = make_uint4(p[0], p[1], p[2], p[3]);
+        to[1] = make_uint4(p[4], p[5], p[6], p[7]);
+      };
+      bool done = true;
+      if (!w.split()) {
+        if (warp_used) {
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          for (int i = half; i < pieces; i += 2) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + lanes + i * 16, o);
+            float f[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) f[j] = l == 0.f ? 0.f : __uint_as_float(o[j]);
+            if (mine) store(i, f, inv);
+          }
+        }
+      } else {
+        // partial sums: [piece][row][16] and (m, l) of every row, in one of this block's two places
+        const long long w0 = w.cur - w.b0;
+        const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.ts.blocks - 1, total, parts);
+        auto place = [&](int part) { return part * 2 + (part == first && work_begin(total, part, parts) < w0 ? 1 : 0); };
+        const long long floats = (long long)(D + 2) * 128;
+        {
+          float* const to = a.partial + place(blockIdx.x) * floats;
+          if (warp_used) {
+            for (int i = half; i < pieces; i += 2) {
+              uint32_t o[16];
+              tmem_ld16(o_tmem + lanes + i * 16, o);
+              if (mine) {
+                uint4* at = reinterpret_cast<uint4*>(to + ((long long)i * 128 + row) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) at[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              }
+            }
+            if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m, l);
+          }
+        }
+        __threadfence();
+        named_sync(5, kSoftmaxThreads);
+        uint32_t* const counter = a.counters + (long long)w.head * a.max_tiles + w.index;
+        if (tid == 0) {
+          c.arrived = atomicAdd(counter, 1u);
+          if (c.arrived == (uint32_t)(last - first)) *counter = 0;  // as it was found
+        }
+        named_sync(5, kSoftmaxThreads);
+        done = c.arrived == (uint32_t)(last - first);
+        if (done) {
+          __threadfence();
+          if (mine) {
+            float top = -INFINITY;
+            for (int f = first; f <= last; f++) top = fmaxf(top, __ldcg(a.partial + place(f) * floats + D * 128 + row * 2));
+            const float from = top == -INFINITY ? 0.f : top;
+            auto factor = [&](int f, float& part) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial + place(f) * floats + D * 128 + row * 2));
+              part = ml.y;
+              return ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - from) * cexp);
+            };
+            float all = 0.f;
+            for (int f = first; f <= last; f++) {
+              float part;
+              const float x = factor(f, part);
+              all += x == 0.f ? 0.f : x * part;
+            }
+            const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);
+            for (int i = half; i < pieces; i += 2) {
+              float o[16] = {};
+              for (int f = first; f <= last; f++) {
+                float part;
+                const float x = factor(f, part);
+                if (x == 0.f) continue;
+                const float4* at = reinterpret_cast<const float4*>(a.partial + place(f) * floats + ((long long)i * 128 + row) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                  const float4 y = __ldcg(at + j);
+                  o[4 * j] += x * y.x; o[4 * j + 1] += x * y.y; o[4 * j + 2] += x * y.z; o[4 * j + 3] += x * y.w;
+                }
+              }
+              store(i, o, inv);
+            }
+          }
+        }
+      }
+      if (done) {
+        if (mine && !finite) atomicOr(&c.bad_rows[row >> 5], 1u << (row & 31));
+        named_sync(5, kSoftmaxThreads);
+        const uint32_t bad[4] = {c.bad_rows[0], c.bad_rows[1], c.bad_rows[2], c.bad_rows[3]};
+        if (bad[0] | bad[1] | bad[2] | bad[3]) {  // rare: an infinity or a NaN among the values
+          auto sync = [] { named_sync(5, kSoftmaxThreads); };
+          for (int r = 0; r < used; r++) {
+            if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
+            const int tk = page_of(r, a.group_div);
+            const long long p = (long long)w.span.ctx + w.tile * tpt + tk;
+            attend_row(a, plain, tid, w.span.row0 + w.tile * tpt + tk, w.head * group + r - tk * group, w.seq, (int)min(p, 0x7fffffffll), sync);
+          }
+          if (tid < 4) c.bad_rows[tid] = 0;
+        }
+      }
+      tc_fence_before();
+      named_sync(5, kSoftmaxThreads);  // everybody has read O, the exchange and the flags
+    } while (w.next(a));
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    __syncwarp();
+    if (*(volatile int*)&c.abort) __nanosleep(1000000);  // let what is in flight land after a failed wait
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+template <int DC, int UNITS, bool I8>
+cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
+  constexpr int smem = 1024 + (DC + UNITS) * kUnit + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(RowScratch) + (int)sizeof(Control);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
+  auto kernel = attn_paged_tile_kernel<DC, UNITS, I8>;
+  static std::atomic<unsigned long long> attr_done;
+  if (first_use_on_device(attr_done)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    mark_used_on_device(attr_done);
+  }
+  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a);
+}
+
+}  // namespace
+
+void attn_paged_shape(AttnPagedArgs& a, int sms) {
+  const int group = a.n_q / a.v.n_kv;
+  a.tokens_per_tile = 128 / group;
+  a.group_div = page_divisor(group);
+  a.max_tiles = a.v.rows / a.tokens_per_tile + std::min(a.v.S, a.v.rows);
+  a.grid = sms;
+}
+size_t attn_paged_counter_bytes(const AttnPagedArgs& a) { return (size_t)a.v.n_kv * a.max_tiles * 4; }
+size_t attn_paged_partial_bytes(const AttnPagedArgs& a) { return (size_t)a.grid * 2 * (a.v.D + 2) * 128 * 4; }
+
+cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream) {
+  a.wait_ns = wait_limit_ns();
+  const int units = (a.v.D + 63) / 64;
+  if (a.scales)
+    return units == 1 ? run_tile<1, 8, true>(a, stream) : units == 2 ? run_tile<2, 8, true>(a, stream)
+         : units == 3 ? run_tile<3, 9, true>(a, stream) : run_tile<4, 9, true>(a, stream);
+  return units == 1 ? run_tile<1, 8, false>(a, stream) : units == 2 ? run_tile<2, 8, false>(a, stream)
+       : units == 3 ? run_tile<3, 9, false>(a, stream) : run_tile<4, 9, false>(a, stream);
+}
+
+}  // namespace tb200
