@@ -23,7 +23,11 @@ namespace tb200 {
 
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kCopyWarps = 4, kThreads = (kSoftmaxWarps + kCopyWarps + 1) * 32;
+// four warpgroups: two for softmax, one that copies, one whose first warp issues matrix instructions; the registers go where they are needed
+// (256 x 176 + 128 x 104 + 128 x 56 of the 512 x 128 that a block starts with)
+constexpr int kSoftmaxWarps = 8, kCopyWarps = 4, kThreads = 512;
+constexpr int kSoftmaxRegs = 176, kCopyRegs = 104, kIssueRegs = 56;
+static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + kCopyWarps * 32 * kCopyRegs + 128 * kIssueRegs <= kThreads * 128, "register split");
 constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
 constexpr int kMetaBlocks = 8;
@@ -34,11 +38,11 @@ struct Meta {
   uint32_t holds[4];  // a bit for each key of the block: its page holds something
 };
 struct Control {
-  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty;
+  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_empty;
   uint32_t tmem, bad_rows[4], arrived;
   int abort;
   float top[2][2][128];  // row maxima of the two halves, by parity of the block
-  long long totals[32], start_rem;
+  long long totals[kThreads / 32];
   int start_seq, start_tile, start_index, start_off;
 };
 
@@ -104,8 +108,8 @@ struct Walker {
   }
 };
 
-// Sum over the block's threads (or the running sum up to and including this thread), through c.totals.
-__device__ long long block_total(Control& c, long long x, bool running) {
+// Running sum over the block's threads up to and including this one, and the sum of all, through c.totals.
+__device__ long long block_scan(Control& c, long long x, long long& all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long v = x;
 #pragma unroll
@@ -116,12 +120,15 @@ __device__ long long block_total(Control& c, long long x, bool running) {
   __syncthreads();
   if (lane == 31) c.totals[warp] = v;
   __syncthreads();
-  long long all = 0, before = 0;
+  long long before = 0;
+  all = 0;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; w++) {
-    if (w < warp) before += c.totals[w];
-    all += c.totals[w];
+    const long long y = c.totals[w];
+    before += w < warp ? y : 0;
+    all += y;
   }
-  return running ? before + v : all;
+  return before + v;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -175,7 +182,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     }
     mbar_init(smem_u32(&c.pv_done), 1);
     mbar_init(smem_u32(&c.o_done), 1);
-    mbar_init(smem_u32(&c.q_full), kCopyThreads);
     mbar_init(smem_u32(&c.q_empty), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     c.abort = 0;
@@ -185,13 +191,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   grid_dependency_release();
 
   // ---- the work: tiles of the sequences, key blocks of the tiles ----
+  long long all = 0;
   int run = 0;
   for (int s0 = 0; s0 < v.S; s0 += kThreads) {
     const int s = s0 + tid;
-    const int mine = s < v.S ? tiles_of(a, span_of(a, s)) : 0;
-    const int upto = run + (int)block_total(c, mine, true);
+    const int upto = run + (int)block_scan(c, s < v.S ? tiles_of(a, span_of(a, s)) : 0, all);
     if (s < v.S) first_tile[s + 1] = upto;
-    run += (int)block_total(c, mine, false);
+    run += (int)all;
   }
   if (tid == 0) first_tile[0] = 0;
   tc_fence_before();
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   tc_fence_after();
   const uint32_t tmem = c.tmem;
   const int n_tiles = min(run, a.max_tiles);
-  auto locate = [&](int i, int& seq) {
+  auto blocks_of = [&](int i, int& seq, int& tile) {
     int lo = 0, hi = v.S - 1;  // the last sequence with first_tile[seq] <= i
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -207,17 +213,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       else hi = mid - 1;
     }
     seq = lo;
-    return i - first_tile[lo];
-  };
-  auto blocks_of = [&](int i) {
-    int seq;
-    const int t = locate(i, seq);
+    tile = i - first_tile[lo];
     const Span sp = span_of(a, seq);
-    return tile_span(sp.ctx, sp.n, t, tpt, a.window, a.sinks, v.capacity).blocks;
+    return tile_span(sp.ctx, sp.n, tile, tpt, a.window, a.sinks, v.capacity).blocks;
   };
-  long long mine = 0;
-  for (int i = tid; i < n_tiles; i += kThreads) mine += blocks_of(i);
-  const long long per_head = block_total(c, mine, false), total = per_head * v.n_kv;
+  int seq0 = 0, tile0 = 0, n0 = tid < n_tiles ? blocks_of(tid, seq0, tile0) : 0;
+  long long upto0 = block_scan(c, n0, all), per_head = all;
+  if (n_tiles > kThreads) {
+    long long mine = 0;
+    for (int i = tid + kThreads; i < n_tiles; i += kThreads) mine += blocks_of(i, seq0, tile0);
+    block_scan(c, mine, all);
+    per_head += all;
+  }
+  const long long total = per_head * v.n_kv;
   const int parts = (int)max(1ll, min((long long)gridDim.x, total / kTileMinBlocks));
   const bool works = total > 0 && (int)blockIdx.x < parts;
   const long long begin = works ? work_begin(total, blockIdx.x, parts) : 0, end = works ? work_begin(total, blockIdx.x + 1, parts) : 0;
@@ -225,16 +233,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     const long long rem = begin % per_head;
     long long before = 0;
     for (int i0 = 0; i0 < n_tiles && before <= rem; i0 += kThreads) {
-      const int i = i0 + tid, n = i < n_tiles ? blocks_of(i) : 0;
-      const long long upto = before + block_total(c, n, true);
-      if (n && upto > rem && upto - n <= rem) {
-        int seq;
-        c.start_tile = locate(i, seq);
-        c.start_seq = seq;
-        c.start_index = i;
-        c.start_off = (int)(rem - (upto - n));
+      const int i = i0 + tid;
+      if (n_tiles > kThreads) {
+        n0 = i < n_tiles ? blocks_of(i, seq0, tile0) : 0;
+        upto0 = block_scan(c, n0, all);
       }
-      before += block_total(c, n, false);
+      const long long upto = before + upto0;
+      if (n0 && upto > rem && upto - n0 <= rem) {
+        c.start_tile = tile0;
+        c.start_seq = seq0;
+        c.start_index = i;
+        c.start_off = (int)(rem - (upto - n0));
+      }
+      before += n_tiles > kThreads ? all : per_head;
     }
   }
   __syncthreads();  // the start is known, and first_tile's room is free
@@ -259,8 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   };
 
   const uint32_t o_tmem = tmem + 256;
-  if (works && warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
+  if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ copies
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegs));
+    if (works) {
     const int t = tid - kSoftmaxThreads;
     uint32_t unit = 0;       // units asked for so far
     uint32_t signalled = 0;  // units handed over
@@ -280,8 +293,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       drain();  // nothing that has arrived is held back while this waits
       wait(c.empty[unit % UNITS], parity, 301);
     };
-    const char* const kp = (const char*)a.k;
-    const char* const vp = (const char*)a.vv;
     constexpr int kRows = I8 ? 4 : 8;           // rows of a unit that a thread copies a piece of
     constexpr int kPieces = I8 ? 4 : 8;         // pieces of 16 bytes in a unit's row
     const int piece = t % kPieces, row0 = t / kPieces;
@@ -291,11 +302,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     w.start(a, c, begin, end, per_head, n_tiles);
     do {
       const long long head_bytes = (long long)w.head * D * (I8 ? 1 : 2);
-      // queries
+      // queries: they are there when the first unit of keys behind them is
       if (items && !mbar_try_wait(smem_u32(&c.q_empty), (items - 1) & 1)) {
         drain();  // the scores that free the queries need the units still held back
         wait(c.q_empty, (items - 1) & 1, 302);
       }
+      items++;
+      // slots (32 bits: the planner refuses more) of this thread's rows of a block, -1 where no token of the tile sees the key or
+      // nothing is held; asked for a block ahead of their use
+      auto slot_at = [&](int key) {
+        const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
+        return wanted ? (int)slot_of(v, w.seq, key) : -1;
+      };
+      auto slots_of = [&](int b, int (&slot)[kRows]) {
+        const int key0 = tile_block(w.ts, b) * kKeyBlock + row0;
+#pragma unroll
+        for (int i = 0; i < kRows; i++) slot[i] = slot_at(key0 + kRowStep * i);
+      };
+      int key_slot[kRows], val_slot[kRows], next_slot[kRows], own_slot, next_own;
+      slots_of(w.b0, key_slot);
+      own_slot = slot_at(tile_block(w.ts, w.b0) * kKeyBlock + t);
       {
         const int qp = t & 7, used = min(tpt, w.span.n - w.tile * tpt) * group;
 #pragma unroll
@@ -310,93 +336,83 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        drain();
-        mbar_arrive(smem_u32(&c.q_full));
       }
-      items++;
-      const int n = w.b1 - w.b0;
-      // the slots of this thread's rows of a block; -1 where no token of the tile sees the key
-      auto slots_of = [&](int b, long long (&slot)[kRows]) {
-        const int key0 = tile_block(w.ts, w.b0 + b) * kKeyBlock;
-#pragma unroll
-        for (int i = 0; i < kRows; i++) {
-          const int key = key0 + row0 + kRowStep * i;
-          const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
-          slot[i] = wanted ? slot_of(v, w.seq, key) : -1;
-        }
-      };
-      auto copy_units = [&](const char* pages, const long long (&slot)[kRows]) {
+      auto copy_units = [&](const char* pages, const int (&slot)[kRows], bool behind_queries) {
 #pragma unroll
         for (int u = 0; u < DC; u++) {
           slot_free();
           const uint32_t dst = ring + (unit % UNITS) * kUnit;
           const int d = u * 64 + piece * (I8 ? 16 : 8);
+          uint4 x[I8 ? kRows : 1];
 #pragma unroll
           for (int i = 0; i < kRows; i++) {
             const int r = row0 + kRowStep * i;
             const bool ok = slot[i] >= 0 && d < D;
-            const char* src = pages + (slot[i] >= 0 ? slot[i] : 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
-            if (!I8) {
-              copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src, ok);
-            } else {
-              uint4 x = ok ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+            const char* src = pages + max(slot[i], 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
+            if (I8) x[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+            else copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src, ok);
+          }
+          if (I8) {
+#pragma unroll
+            for (int i = 0; i < kRows; i++) {
+              const int r = row0 + kRowStep * i;
               uint4 lo, hi;
-              widen4(x.x, lo.x, lo.y); widen4(x.y, lo.z, lo.w);
-              widen4(x.z, hi.x, hi.y); widen4(x.w, hi.z, hi.w);
+              widen4(x[i].x, lo.x, lo.y); widen4(x[i].y, lo.z, lo.w);
+              widen4(x[i].z, hi.x, hi.y); widen4(x[i].w, hi.z, hi.w);
               sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
               sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
             }
-          }
-          if (!I8) asm volatile("cp.async.commit_group;" ::: "memory");
-          unit++;
-          if (I8) {
+            unit++;
+            if (behind_queries && u == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
             hand_over(unit);
           } else {  // three units stay in flight
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            unit++;
             asm volatile("cp.async.wait_group 3;" ::: "memory");
             if (unit > 3 + signalled) hand_over(unit - 3);
           }
         }
       };
-      for (int b = 0; b <= n; b++) {
-        if (b < n) {
-          long long slot[kRows];
-          slots_of(b, slot);
+      for (int b = w.b0; b <= w.b1; b++) {
+        if (b < w.b1) {
+          if (b + 1 < w.b1) {
+            slots_of(b + 1, next_slot);
+            next_own = slot_at(tile_block(w.ts, b + 1) * kKeyBlock + t);
+          }
           Meta& m = meta[blocks % kMetaBlocks];
           blocks++;
-          const int key0 = tile_block(w.ts, w.b0 + b) * kKeyBlock;
-          {  // what this block's keys are, by one thread a key
-            const int key = key0 + t;
-            const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
-            const long long s = wanted ? slot_of(v, w.seq, key) : -1;
-            const uint32_t bits = __ballot_sync(0xffffffffu, s >= 0);
-            if (lane == 0) m.holds[t >> 5] = bits;
-            if (I8) {
-              const float* sc = a.scales + (s >= 0 ? s : 0) * 2 * v.n_kv + w.head;
-              m.k_scale[t] = s >= 0 ? __ldg(sc) : 0.f;
-              m.v_scale[t] = s >= 0 ? __ldg(sc + v.n_kv) : 0.f;
-            }
+          // what this block's keys are, by one thread a key
+          const uint32_t bits = __ballot_sync(0xffffffffu, own_slot >= 0);
+          if (lane == 0) m.holds[t >> 5] = bits;
+          if (I8) {
+            const float* sc = a.scales + (long long)max(own_slot, 0) * 2 * v.n_kv + w.head;
+            m.k_scale[t] = own_slot >= 0 ? __ldg(sc) : 0.f;
+            m.v_scale[t] = own_slot >= 0 ? __ldg(sc + v.n_kv) : 0.f;
           }
-          copy_units(kp, slot);
+          copy_units((const char*)a.k, key_slot, b == w.b0);
         }
-        if (b > 0) {
-          long long slot[kRows];
-          slots_of(b - 1, slot);
-          copy_units(vp, slot);
+        if (b > w.b0) copy_units((const char*)a.vv, val_slot, false);
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+          val_slot[i] = key_slot[i];
+          key_slot[i] = next_slot[i];
         }
+        own_slot = next_own;
       }
     } while (w.next(a));
     drain();
-  } else if (works && warp == kSoftmaxWarps + kCopyWarps) {
+    }
+  } else if (warp >= kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ matrix instructions
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+    if (works && warp == kSoftmaxWarps + kCopyWarps) {
     const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1024 bytes apart, sm_100 descriptor, 128-byte swizzle
     const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kKeyBlock >> 3) << 17) | (8u << 24);
-    uint32_t unit = 0, blocks = 0, items = 0;
+    uint32_t unit = 0, blocks = 0;
     auto lo_of = [](uint32_t at) { return ((at & 0x3FFFF) >> 4) | (64u << 16); };
     Walker w;
     w.start(a, c, begin, end, per_head, n_tiles);
     do {
-      wait(c.q_full, items & 1, 303);
-      items++;
       const int n = w.b1 - w.b0;
       for (int b = 0; b <= n; b++) {
         if (b < n) {  // scores of block b
@@ -437,7 +453,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       }
       blocks += n;
     } while (w.next(a));
-  } else if (works) {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    if (works) {
     // ------------------------------------------------ softmax: thread = (row, half of the block's keys)
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -615,36 +634,74 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         done = c.arrived == (uint32_t)(last - first);
         if (done) {
           __threadfence();
-          if (mine) {
-            float top = -INFINITY;
-            for (int f = first; f <= last; f++) top = fmaxf(top, __ldcg(a.partial + place(f) * floats + D * 128 + row * 2));
-            const float from = top == -INFINITY ? 0.f : top;
-            auto factor = [&](int f, float& part) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial + place(f) * floats + D * 128 + row * 2));
-              part = ml.y;
-              return ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - from) * cexp);
-            };
-            float all = 0.f;
-            for (int f = first; f <= last; f++) {
-              float part;
-              const float x = factor(f, part);
-              all += x == 0.f ? 0.f : x * part;
+          // rows' maxima and sums first, `share` threads to a row; then every thread four values at a time, four of them from four parts in flight
+          const int count = last - first + 1;
+          int share = 2;
+          while (share < 32 && used * share * 2 <= kSoftmaxThreads) share *= 2;
+          const int sub = tid & (share - 1), r0 = tid / share;
+          auto at_ml = [&](int f, int r) { return reinterpret_cast<const float2*>(a.partial + place(first + f) * floats + D * 128 + r * 2); };
+          float top = -INFINITY, sums = 0.f;
+          if (r0 < used) {
+#pragma unroll 4
+            for (int f = sub; f < count; f += share) top = fmaxf(top, __ldcg(at_ml(f, r0)).x);
+          }
+          for (int o = 1; o < share; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float from = top == -INFINITY ? 0.f : top;
+          if (r0 < used) {
+#pragma unroll 4
+            for (int f = sub; f < count; f += share) {
+              const float2 ml = __ldcg(at_ml(f, r0));
+              sums += ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - from) * cexp) * ml.y;
             }
-            const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);
-            for (int i = half; i < pieces; i += 2) {
-              float o[16] = {};
-              for (int f = first; f <= last; f++) {
-                float part;
-                const float x = factor(f, part);
-                if (x == 0.f) continue;
-                const float4* at = reinterpret_cast<const float4*>(a.partial + place(f) * floats + ((long long)i * 128 + row) * 16);
+          }
+          for (int o = 1; o < share; o <<= 1) sums += __shfl_xor_sync(0xffffffffu, sums, o);
+          if (r0 < used && sub == 0) {
+            c.top[0][0][r0] = from;
+            c.top[0][1][r0] = sums > 0.f ? 1.f / sums : (sums == 0.f ? 0.f : sums);
+          }
+          named_sync(5, kSoftmaxThreads);
+          const int quads = used * (D >> 2);  // (16 columns, row, four of the 16)
+          for (int i0 = 0; i0 < quads; i0 += 4 * kSoftmaxThreads) {
+            float4 o[4];
+            int r[4], q[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                  const float4 y = __ldcg(at + j);
-                  o[4 * j] += x * y.x; o[4 * j + 1] += x * y.y; o[4 * j + 2] += x * y.z; o[4 * j + 3] += x * y.w;
+            for (int k = 0; k < 4; k++) {
+              const int i = min(i0 + k * kSoftmaxThreads + tid, quads - 1), y = i >> 2, p = y / used;
+              r[k] = y - p * used;
+              q[k] = p * 4 + (i & 3);
+              o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            for (int f0 = 0; f0 < count; f0 += 4) {
+              float4 x[4][4];
+              float m4[4][4];
+#pragma unroll
+              for (int f = 0; f < 4; f++) {
+                const float* part = a.partial + place(first + min(f0 + f, count - 1)) * floats;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  m4[f][k] = f0 + f < count ? __ldcg(part + D * 128 + r[k] * 2) : -INFINITY;
+                  x[f][k] = __ldcg(reinterpret_cast<const float4*>(part + ((long long)(q[k] >> 2) * 128 + r[k]) * 16 + (q[k] & 3) * 4));
                 }
               }
-              store(i, o, inv);
+#pragma unroll
+              for (int f = 0; f < 4; f++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  if (m4[f][k] == -INFINITY) continue;  // that part saw no key of this row
+                  const float y = exp2_fast((m4[f][k] - c.top[0][0][r[k]]) * cexp);
+                  o[k].x += y * x[f][k].x; o[k].y += y * x[f][k].y; o[k].z += y * x[f][k].z; o[k].w += y * x[f][k].w;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              if (i0 + k * kSoftmaxThreads + tid >= quads) continue;
+              const float inv = c.top[0][1][r[k]];
+              const float x0 = o[k].x * inv, x1 = o[k].y * inv, x2 = o[k].z * inv, x3 = o[k].w * inv;
+              const int tk = page_of(r[k], a.group_div);
+              uint16_t* to = a.out + ((long long)(w.span.row0 + w.tile * tpt + tk) * a.n_q + w.head * group + r[k] - tk * group) * D + q[k] * 4;
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
+              if (!(fabsf(x0) <= 3.0e38f && fabsf(x1) <= 3.0e38f && fabsf(x2) <= 3.0e38f && fabsf(x3) <= 3.0e38f))
+                atomicOr(&c.bad_rows[r[k] >> 5], 1u << (r[k] & 31));
             }
           }
         }
@@ -667,6 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       tc_fence_before();
       named_sync(5, kSoftmaxThreads);  // everybody has read O, the exchange and the flags
     } while (w.next(a));
+    }
   }
   tc_fence_before();
   __syncthreads();

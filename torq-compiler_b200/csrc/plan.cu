@@ -409,8 +409,9 @@ bool paged_plan(Builder& b, const tb200_op_t& op, int row_start, int context, in
     b.fail(TB200_INVALID_ARGUMENT, "op %d: %s: head counts or the layer do not match the caches", i, name);
     return false;
   }
-  if (D % 16 || D > 256 || T[context].shape[0] > 4096 || (long long)T[op.multiplier].shape[1] * p.shape[2] > (1ll << 30)) {
-    b.fail(TB200_UNIMPLEMENTED, "op %d: %s supports head sizes of a multiple of 16 up to 256, 4096 sequences, 2^30 positions", i, name);
+  if (D % 16 || D > 256 || T[context].shape[0] > 4096 || (long long)T[op.multiplier].shape[1] * p.shape[2] > (1ll << 30) ||
+      (long long)p.shape[1] * p.shape[2] > 0x7fffffffll) {
+    b.fail(TB200_UNIMPLEMENTED, "op %d: %s supports head sizes of a multiple of 16 up to 256, 4096 sequences, 2^30 positions, 2^31 - 1 slots", i, name);
     return false;
   }
   if (c.i8 != (op.bias >= 0) || (c.i8 && (!b.is_t(op.bias, TB200_F32, 4) || !held(op.bias) || T[op.bias].shape[0] != p.shape[0] ||
