@@ -136,6 +136,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two fp32 operations in one instruction
+__device__ __forceinline__ unsigned long long pack_f32(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul_f32x2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // four int8 -> four bf16, exact: 0x4300 | low seven bits of the biased byte is 128 + those bits, and 128 or 256 comes off again
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   const uint32_t u = w ^ 0x80808080u, low = u & 0x7f7f7f7fu, off = ~u & 0x80808080u;
@@ -173,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   }
   if (tid == 32) {
     for (int i = 0; i < UNITS; i++) {
-      mbar_init(smem_u32(&c.full[i]), kCopyThreads);
+      mbar_init(smem_u32(&c.full[i]), I8 ? kCopyThreads : 2 * kCopyThreads);
       mbar_init(smem_u32(&c.empty[i]), 1);
     }
     for (int i = 0; i < 2; i++) {  // a softmax warp may be one block ahead of another: a barrier for each buffer
@@ -276,22 +293,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     if (works) {
     const int t = tid - kSoftmaxThreads;
     uint32_t unit = 0;       // units asked for so far
-    uint32_t signalled = 0;  // units handed over
     uint32_t items = 0, blocks = 0;
-    auto hand_over = [&](uint32_t upto) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      for (; signalled < upto; signalled++) mbar_arrive(smem_u32(&c.full[signalled % UNITS]));
-    };
-    auto drain = [&]() {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      hand_over(unit);
-    };
     auto slot_free = [&]() {  // room for unit `unit`
-      if (unit < UNITS) return;
-      const uint32_t bar = smem_u32(&c.empty[unit % UNITS]), parity = (unit / UNITS - 1) & 1;
-      if (mbar_try_wait(bar, parity)) return;
-      drain();  // nothing that has arrived is held back while this waits
-      wait(c.empty[unit % UNITS], parity, 301);
+      if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
+    };
+    // This thread's part of unit `unit`: what it has stored itself is handed over with a fence towards the matrix instructions, what its
+    // asynchronous copies bring when they arrive (the issuing warp fences). The plain arrival covers the block's Meta either way.
+    auto hand_over = [&]() {
+      const uint32_t bar = smem_u32(&c.full[unit % UNITS]);
+      if (I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      else asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+      mbar_arrive(bar);
+      unit++;
     };
     constexpr int kRows = I8 ? 4 : 8;           // rows of a unit that a thread copies a piece of
     constexpr int kPieces = I8 ? 4 : 8;         // pieces of 16 bytes in a unit's row
@@ -303,10 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     do {
       const long long head_bytes = (long long)w.head * D * (I8 ? 1 : 2);
       // queries: they are there when the first unit of keys behind them is
-      if (items && !mbar_try_wait(smem_u32(&c.q_empty), (items - 1) & 1)) {
-        drain();  // the scores that free the queries need the units still held back
-        wait(c.q_empty, (items - 1) & 1, 302);
-      }
+      if (items) wait(c.q_empty, (items - 1) & 1, 302);
       items++;
       // slots (32 bits: the planner refuses more) of this thread's rows of a block, -1 where no token of the tile sees the key or
       // nothing is held; asked for a block ahead of their use
@@ -335,53 +345,71 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             copy16(q_smem + u * kUnit + r * 128 + ((qp ^ (r & 7)) << 4), src + (d < D ? d : 0), ok && d < D);
           }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      auto copy_units = [&](const char* pages, const int (&slot)[kRows], bool behind_queries) {
+      auto source = [&](const char* pages, int slot, int d) {
+        return pages + max(slot, 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
+      };
+      auto copy_units = [&](const char* pages, const int (&slot)[kRows]) {  // bf16
 #pragma unroll
         for (int u = 0; u < DC; u++) {
           slot_free();
           const uint32_t dst = ring + (unit % UNITS) * kUnit;
-          const int d = u * 64 + piece * (I8 ? 16 : 8);
-          uint4 x[I8 ? kRows : 1];
+          const int d = u * 64 + piece * 8;
 #pragma unroll
           for (int i = 0; i < kRows; i++) {
             const int r = row0 + kRowStep * i;
-            const bool ok = slot[i] >= 0 && d < D;
-            const char* src = pages + max(slot[i], 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
-            if (I8) x[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-            else copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), src, ok);
+            copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), source(pages, slot[i], d), slot[i] >= 0 && d < D);
           }
-          if (I8) {
-#pragma unroll
-            for (int i = 0; i < kRows; i++) {
-              const int r = row0 + kRowStep * i;
-              uint4 lo, hi;
-              widen4(x[i].x, lo.x, lo.y); widen4(x[i].y, lo.z, lo.w);
-              widen4(x[i].z, hi.x, hi.y); widen4(x[i].w, hi.z, hi.w);
-              sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
-              sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
-            }
-            unit++;
-            if (behind_queries && u == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-            hand_over(unit);
-          } else {  // three units stay in flight
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            unit++;
-            asm volatile("cp.async.wait_group 3;" ::: "memory");
-            if (unit > 3 + signalled) hand_over(unit - 3);
-          }
+          hand_over();
         }
       };
-      for (int b = w.b0; b <= w.b1; b++) {
-        if (b < w.b1) {
-          if (b + 1 < w.b1) {
-            slots_of(b + 1, next_slot);
-            next_own = slot_at(tile_block(w.ts, b + 1) * kKeyBlock + t);
+      // int8: groups of up to two units go through registers, the next group asked for before one is widened
+      constexpr int G = DC > 1 ? 2 : 1;
+      uint4 x[I8 ? G : 1][kRows], y[I8 ? G : 1][kRows];
+      auto load = [&](uint4 (&to)[I8 ? G : 1][kRows], const char* pages, const int (&slot)[kRows], int u0) {
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          if (u0 + g >= DC) continue;
+          const int d = (u0 + g) * 64 + piece * 16;
+#pragma unroll
+          for (int i = 0; i < kRows; i++)
+            to[I8 ? g : 0][i] = slot[i] >= 0 && d < D ? __ldg(reinterpret_cast<const uint4*>(source(pages, slot[i], d))) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      auto store = [&](const uint4 (&from)[I8 ? G : 1][kRows], int u0) {
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          if (u0 + g >= DC) continue;
+          slot_free();
+          const uint32_t dst = ring + (unit % UNITS) * kUnit;
+#pragma unroll
+          for (int i = 0; i < kRows; i++) {
+            const int r = row0 + kRowStep * i;
+            const uint4 q = from[I8 ? g : 0][i];
+            uint4 lo, hi;
+            widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
+            widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
+            sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
+            sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
           }
+          hand_over();
+        }
+      };
+      const char* const kp = (const char*)a.k;
+      const char* const vp = (const char*)a.vv;
+      if (I8) {
+        load(x, kp, key_slot, 0);
+        asm volatile("cp.async.wait_all;" ::: "memory");  // the queries
+      }
+      for (int b = w.b0; b <= w.b1; b++) {
+        const bool keys = b < w.b1, values = b > w.b0, more = b + 1 < w.b1;
+        if (more) {
+          slots_of(b + 1, next_slot);
+          next_own = slot_at(tile_block(w.ts, b + 1) * kKeyBlock + t);
+        }
+        if (keys) {  // what this block's keys are, by one thread a key
           Meta& m = meta[blocks % kMetaBlocks];
           blocks++;
-          // what this block's keys are, by one thread a key
           const uint32_t bits = __ballot_sync(0xffffffffu, own_slot >= 0);
           if (lane == 0) m.holds[t >> 5] = bits;
           if (I8) {
@@ -389,9 +417,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             m.k_scale[t] = own_slot >= 0 ? __ldg(sc) : 0.f;
             m.v_scale[t] = own_slot >= 0 ? __ldg(sc + v.n_kv) : 0.f;
           }
-          copy_units((const char*)a.k, key_slot, b == w.b0);
         }
-        if (b > w.b0) copy_units((const char*)a.vv, val_slot, false);
+        if (!I8) {
+          if (keys) copy_units(kp, key_slot);
+          if (values) copy_units(vp, val_slot);
+        } else if (DC <= 2) {
+          if (values) load(y, vp, val_slot, 0);
+          if (keys) store(x, 0);
+          if (more) load(x, kp, next_slot, 0);
+          if (values) store(y, 0);
+        } else {
+          if (keys) {
+            load(y, kp, key_slot, 2);
+            store(x, 0);
+          }
+          if (values) load(x, vp, val_slot, 0);
+          if (keys) store(y, 2);
+          if (values) {
+            load(y, vp, val_slot, 2);
+            store(x, 0);
+          }
+          if (more) load(x, kp, next_slot, 0);
+          if (values) store(y, 2);
+        }
 #pragma unroll
         for (int i = 0; i < kRows; i++) {
           val_slot[i] = key_slot[i];
@@ -400,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         own_slot = next_own;
       }
     } while (w.next(a));
-    drain();
+    asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else if (warp >= kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ matrix instructions
@@ -420,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
+            if (!I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_after();
             const uint32_t qa = lo_of(q_smem + u * kUnit), kb = lo_of(ring + (unit % UNITS) * kUnit);
             const int steps = min(4, (D - u * 64) >> 4);
@@ -437,6 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 306);
+            if (!I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_after();
             const int width = min(64, D - u * 64);
             const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(width >> 3) << 17) | (8u << 24);
@@ -514,9 +564,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             s1[i] = see1 ? s1[i] : none;
           }
         }
-        float top = -INFINITY;
+        float tops[4];
 #pragma unroll
-        for (int i = 0; i < 32; i++) top = fmaxf(top, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+        for (int i = 0; i < 4; i++) tops[i] = fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i]));
+#pragma unroll
+        for (int i = 4; i < 32; i++) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         c.top[blocks & 1][half][row] = top;
         named_sync(1 + (warp & 3), 64);
         top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
@@ -541,26 +594,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           tmem_st_wait();
         }
         const float from = m == -INFINITY ? 0.f : m;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-        auto weights = [&](uint32_t (&s)[32], const float* v_scale, uint32_t holds, uint32_t to) {
+        const unsigned long long minus = pack_f32(-from, -from), scale2 = pack_f32(cexp, cexp);
+        unsigned long long parts2[2] = {0ull, 0ull};  // two pairs of running sums
+        auto weights = [&](const uint32_t (&s)[32], const float* v_scale, uint32_t to) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            float x = exp2_fast((__uint_as_float(s[i]) - from) * cexp), y = exp2_fast((__uint_as_float(s[i + 1]) - from) * cexp);
-            part[i & 2] += x;
-            part[(i & 2) + 1] += y;
+            float x, y;
+            unpack_f32(mul_f32x2(add_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), minus), scale2), x, y);
+            x = exp2_fast(x);
+            y = exp2_fast(y);
+            parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(x, y));
             if (I8) {
               const float2 vs = *reinterpret_cast<const float2*>(v_scale + i);
-              x *= vs.x;
-              y *= vs.y;
+              unpack_f32(mul_f32x2(pack_f32(x, y), pack_f32(vs.x, vs.y)), x, y);
             }
             p[i >> 1] = pack_bf16(x, y);
           }
           tmem_st16(to, p);
         };
-        weights(s0, mt.v_scale + half * 64, holds0, s_tmem);
-        weights(s1, mt.v_scale + half * 64 + 32, holds1, s_tmem + 16);
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        weights(s0, mt.v_scale + half * 64, s_tmem);
+        weights(s1, mt.v_scale + half * 64 + 32, s_tmem + 16);
+        {
+          float x, y;
+          unpack_f32(add_f32x2(parts2[0], parts2[1]), x, y);
+          sum += x + y;
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
@@ -577,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const int my_row = w.span.row0 + w.tile * tpt + tok, my_head = w.head * group + row - tok * group;
       uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
       bool finite = true;
-      auto store = [&](int piece, const float (&o)[16], float inv) {
+      auto store = [&](uint16_t* at, const float (&o)[16], float inv) {
         uint32_t p[8];
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
@@ -585,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
           p[j >> 1] = pack_bf16(x, y);
         }
-        uint4* to = reinterpret_cast<uint4*>(dst + piece * 16);
+        uint4* to = reinterpret_cast<uint4*>(at);
         to[0] = make_uint4(p[0], p[1], p[2], p[3]);
         to[1] = make_uint4(p[4], p[5], p[6], p[7]);
       };
@@ -599,11 +658,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             float f[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) f[j] = l == 0.f ? 0.f : __uint_as_float(o[j]);
-            if (mine) store(i, f, inv);
+            if (mine) store(dst + i * 16, f, inv);
           }
         }
       } else {
-        // partial sums: [piece][row][16] and (m, l) of every row, in one of this block's two places
+        // partial sums: [four columns][row][4] and (m, l) of every row, in one of this block's two places
         const long long w0 = w.cur - w.b0;
         const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.ts.blocks - 1, total, parts);
         auto place = [&](int part) { return part * 2 + (part == first && work_begin(total, part, parts) < w0 ? 1 : 0); };
@@ -615,9 +674,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
               uint32_t o[16];
               tmem_ld16(o_tmem + lanes + i * 16, o);
               if (mine) {
-                uint4* at = reinterpret_cast<uint4*>(to + ((long long)i * 128 + row) * 16);
+                uint4* at = reinterpret_cast<uint4*>(to) + i * 4 * 128 + row;
 #pragma unroll
-                for (int j = 0; j < 4; j++) at[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                for (int j = 0; j < 4; j++) at[j * 128] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
               }
             }
             if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m, l);
@@ -660,49 +719,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             c.top[0][1][r0] = sums > 0.f ? 1.f / sums : (sums == 0.f ? 0.f : sums);
           }
           named_sync(5, kSoftmaxThreads);
-          const int quads = used * (D >> 2);  // (16 columns, row, four of the 16)
-          for (int i0 = 0; i0 < quads; i0 += 4 * kSoftmaxThreads) {
-            float4 o[4];
-            int r[4], q[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const int i = min(i0 + k * kSoftmaxThreads + tid, quads - 1), y = i >> 2, p = y / used;
-              r[k] = y - p * used;
-              q[k] = p * 4 + (i & 3);
-              o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+          for (int i = tid; i < used * pieces; i += kSoftmaxThreads) {  // 16 columns of a row
+            const int pc = i / used, r = i - pc * used;
+            const float top_r = c.top[0][0][r], inv = c.top[0][1][r];
+            float o[16] = {};
             for (int f0 = 0; f0 < count; f0 += 4) {
               float4 x[4][4];
-              float m4[4][4];
+              float mf[4];
 #pragma unroll
               for (int f = 0; f < 4; f++) {
                 const float* part = a.partial + place(first + min(f0 + f, count - 1)) * floats;
+                mf[f] = f0 + f < count ? __ldcg(part + D * 128 + r * 2) : -INFINITY;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                  m4[f][k] = f0 + f < count ? __ldcg(part + D * 128 + r[k] * 2) : -INFINITY;
-                  x[f][k] = __ldcg(reinterpret_cast<const float4*>(part + ((long long)(q[k] >> 2) * 128 + r[k]) * 16 + (q[k] & 3) * 4));
-                }
+                for (int j = 0; j < 4; j++) x[f][j] = __ldcg(reinterpret_cast<const float4*>(part) + (pc * 4 + j) * 128 + r);
               }
 #pragma unroll
-              for (int f = 0; f < 4; f++)
+              for (int f = 0; f < 4; f++) {
+                if (mf[f] == -INFINITY) continue;  // that part saw no key of this row
+                const float y = exp2_fast((mf[f] - top_r) * cexp);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                  if (m4[f][k] == -INFINITY) continue;  // that part saw no key of this row
-                  const float y = exp2_fast((m4[f][k] - c.top[0][0][r[k]]) * cexp);
-                  o[k].x += y * x[f][k].x; o[k].y += y * x[f][k].y; o[k].z += y * x[f][k].z; o[k].w += y * x[f][k].w;
+                for (int j = 0; j < 4; j++) {
+                  o[4 * j] += y * x[f][j].x; o[4 * j + 1] += y * x[f][j].y; o[4 * j + 2] += y * x[f][j].z; o[4 * j + 3] += y * x[f][j].w;
                 }
+              }
             }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              if (i0 + k * kSoftmaxThreads + tid >= quads) continue;
-              const float inv = c.top[0][1][r[k]];
-              const float x0 = o[k].x * inv, x1 = o[k].y * inv, x2 = o[k].z * inv, x3 = o[k].w * inv;
-              const int tk = page_of(r[k], a.group_div);
-              uint16_t* to = a.out + ((long long)(w.span.row0 + w.tile * tpt + tk) * a.n_q + w.head * group + r[k] - tk * group) * D + q[k] * 4;
-              *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x0, x1), pack_bf16(x2, x3));
-              if (!(fabsf(x0) <= 3.0e38f && fabsf(x1) <= 3.0e38f && fabsf(x2) <= 3.0e38f && fabsf(x3) <= 3.0e38f))
-                atomicOr(&c.bad_rows[r[k] >> 5], 1u << (r[k] & 31));
-            }
+            const int tk = page_of(r, a.group_div);
+            finite = true;
+            store(a.out + ((long long)(w.span.row0 + w.tile * tpt + tk) * a.n_q + w.head * group + r - tk * group) * D + pc * 16, o, inv);
+            if (!finite) atomicOr(&c.bad_rows[r >> 5], 1u << (r & 31));
+            finite = true;
           }
         }
       }
