@@ -30,17 +30,29 @@ constexpr int kSoftmaxRegs = 176, kCopyRegs = 104, kIssueRegs = 56;
 static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + kCopyWarps * 32 * kCopyRegs + 128 * kIssueRegs <= kThreads * 128, "register split");
 constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
-constexpr int kMetaBlocks = 8;
+constexpr int kMetaBlocks = 8, kItems = 4;
 static_assert(kSoftmaxThreads == kRowThreads, "the plain row is computed by the softmax warps");
 
-struct Meta {
+struct alignas(16) Meta {
   float k_scale[kKeyBlock], v_scale[kKeyBlock];
-  uint32_t holds[4];  // a bit for each key of the block: its page holds something
+  uint32_t holds[4];  // a bit for each key of the block: it is seen by a row of the tile, and its page holds something
+  int key0;
+};
+static_assert(sizeof(Meta) % 16 == 0 && sizeof(RowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
+// A piece of work of a block of the grid: key blocks b0 .. b1 - 1 of a tile of one key/value head.
+struct Item {
+  int seq, head, index;     // index: of the tile among all tiles
+  int row0, tokens;         // the tile's rows of the chunk; tokens 0: there is no more work
+  int first_pos;            // position of the first token
+  int near_key, end_key, sink_blocks, near_block, blocks;  // tile_span
+  int b0, b1;
+  long long w0;             // where the tile's work begins
 };
 struct Control {
-  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_empty;
+  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_empty, item_full[kItems], item_empty[kItems];
+  Item items[kItems];
   uint32_t tmem, bad_rows[4], arrived;
-  int abort;
+  int abort, stop;
   float top[2][2][128];  // row maxima of the two halves, by parity of the block
   long long totals[kThreads / 32];
   int start_seq, start_tile, start_index, start_off;
@@ -61,52 +73,6 @@ __device__ __forceinline__ Span span_of(const AttnPagedArgs& a, int s) {
 __device__ __forceinline__ int tiles_of(const AttnPagedArgs& a, const Span& s) {
   return s.n * (a.n_q / a.v.n_kv) > a.few_rows ? (s.n + a.tokens_per_tile - 1) / a.tokens_per_tile : 0;
 }
-
-// A block's items, one after another: (head, tile, a range of the tile's key blocks). Every role walks them by itself.
-struct Walker {
-  long long cur, end;
-  int head, seq, tile, index, tiles, n_tiles, off;
-  Span span;
-  TileSpan ts;
-  int b0, b1;
-
-  __device__ __forceinline__ void load_tile(const AttnPagedArgs& a) {
-    ts = tile_span(span.ctx, span.n, tile, a.tokens_per_tile, a.window, a.sinks, a.v.capacity);
-    b0 = off;
-    b1 = (int)min((long long)ts.blocks, off + (end - cur));
-  }
-  __device__ __forceinline__ bool split() const { return b0 > 0 || b1 < ts.blocks; }
-  __device__ __forceinline__ void start(const AttnPagedArgs& a, const Control& c, long long begin, long long end_, long long per_head, int n_tiles_) {
-    cur = begin; end = end_; n_tiles = n_tiles_;
-    head = (int)(begin / per_head);
-    seq = c.start_seq; tile = c.start_tile; index = c.start_index; off = c.start_off;
-    span = span_of(a, seq);
-    tiles = tiles_of(a, span);
-    load_tile(a);
-  }
-  __device__ __forceinline__ bool next(const AttnPagedArgs& a) {
-    cur += b1 - b0;
-    if (cur >= end) return false;
-    off = 0;
-    tile++;
-    if (++index >= n_tiles) {  // the next head begins
-      index = 0;
-      head++;
-      seq = -1;
-      tile = tiles;
-    }
-    if (tile >= tiles) {
-      tile = 0;
-      do {
-        if (++seq >= a.v.S) seq = 0;  // there is a tile, so a sequence with one
-        span = span_of(a, seq);
-        tiles = tiles_of(a, span);
-      } while (!tiles);
-    }
-    load_tile(a);
-    return true;
-  }
-};
 
 // Running sum over the block's threads up to and including this one, and the sum of all, through c.totals.
 __device__ long long block_scan(Control& c, long long x, long long& all) {
@@ -199,6 +165,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     }
     mbar_init(smem_u32(&c.pv_done), 1);
     mbar_init(smem_u32(&c.o_done), 1);
+    for (int i = 0; i < kItems; i++) {
+      mbar_init(smem_u32(&c.item_full[i]), 1);
+      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + kCopyThreads + 32);
+    }
     mbar_init(smem_u32(&c.q_empty), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     c.abort = 0;
@@ -286,6 +256,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     gave_up = true;
   };
 
+  // The roles take the block's items from a ring that a warp of its own fills. The reference stays valid until release_item.
+  auto take_item = [&](uint32_t i) -> const Item& {
+    wait(c.item_full[i % kItems], (i / kItems) & 1, 310);
+    return c.items[i % kItems];
+  };
+  auto release_item = [&](uint32_t i) { mbar_arrive(smem_u32(&c.item_empty[i % kItems])); };
   const uint32_t o_tmem = tmem + 256;
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ copies
@@ -293,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     if (works) {
     const int t = tid - kSoftmaxThreads;
     uint32_t unit = 0;       // units asked for so far
-    uint32_t items = 0, blocks = 0;
+    uint32_t blocks = 0;
     auto slot_free = [&]() {  // room for unit `unit`
       if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
     };
@@ -311,34 +287,44 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     const int piece = t % kPieces, row0 = t / kPieces;
     constexpr int kRowStep = kCopyThreads / kPieces;
     const long long row_bytes = (long long)v.n_kv * D * (I8 ? 1 : 2);
-    Walker w;
-    w.start(a, c, begin, end, per_head, n_tiles);
-    do {
-      const long long head_bytes = (long long)w.head * D * (I8 ? 1 : 2);
+    for (uint32_t items = 0;; items++) {
+      const Item& w = take_item(items);
+      if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
+      const int b0 = w.b0, b1 = w.b1, near_key = w.near_key, end_key = w.end_key, sink_blocks = w.sink_blocks, near_block = w.near_block;
+      const int used = w.tokens * group, head = w.head;
+      const long long head_bytes = (long long)head * D * (I8 ? 1 : 2);
       // queries: they are there when the first unit of keys behind them is
       if (items) wait(c.q_empty, (items - 1) & 1, 302);
-      items++;
-      // slots (32 bits: the planner refuses more) of this thread's rows of a block, -1 where no token of the tile sees the key or
-      // nothing is held; asked for a block ahead of their use
-      auto slot_at = [&](int key) {
-        const bool wanted = key < w.ts.end_key && (key >= w.ts.near_key || key < a.sinks);
-        return wanted ? (int)slot_of(v, w.seq, key) : -1;
+      // A block's keys: the page ids are asked for a block ahead of their use, without a branch (a branch would wait for each), and turned into
+      // slots (32 bits: the planner refuses more) when the block is copied; -1 where no token of the tile sees the key or nothing is held.
+      const int32_t* const pages_of = v.table + (long long)w.seq * v.max_pages;
+      auto key_of = [&](int b) { return (b < sink_blocks ? b : near_block + (b - sink_blocks)) * kKeyBlock; };
+      auto ask = [&](int key) {
+        int page;  // volatile: it is to be on its way now, not when it is used
+        asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(page) : "l"(pages_of + page_of(min(key, v.capacity - 1), v.div)));
+        return page;
       };
-      auto slots_of = [&](int b, int (&slot)[kRows]) {
-        const int key0 = tile_block(w.ts, b) * kKeyBlock + row0;
+      auto slot_at = [&](int key, int page) {
+        const bool there = key < end_key && (key >= near_key || key < a.sinks) && page >= 0 && page < v.pages;
+        return there ? page * v.page_size + (key - page_of(key, v.div) * v.page_size) : -1;
+      };
+      int next_page[kRows], next_own;
+      auto ask_block = [&](int b) {
+        const int key0 = key_of(b);
 #pragma unroll
-        for (int i = 0; i < kRows; i++) slot[i] = slot_at(key0 + kRowStep * i);
+        for (int i = 0; i < kRows; i++) next_page[i] = ask(key0 + row0 + kRowStep * i);
+        next_own = ask(key0 + t);
       };
-      int key_slot[kRows], val_slot[kRows], next_slot[kRows], own_slot, next_own;
-      slots_of(w.b0, key_slot);
-      own_slot = slot_at(tile_block(w.ts, w.b0) * kKeyBlock + t);
+      // where this thread's pieces of the keys and of the values of a block start, in bytes behind the cache; negative: zeros
+      long long key_at[kRows], val_at[kRows];
+      ask_block(b0);
       {
-        const int qp = t & 7, used = min(tpt, w.span.n - w.tile * tpt) * group;
+        const int qp = t & 7, q_row = w.row0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
           const int r = (t >> 3) + 16 * i, tok = page_of(r, a.group_div), h = r - tok * group;
           const bool ok = r < used;
-          const uint16_t* src = a.q + ((long long)(w.span.row0 + w.tile * tpt + (ok ? tok : 0)) * a.n_q + w.head * group + (ok ? h : 0)) * D;
+          const uint16_t* src = a.q + ((long long)(q_row + (ok ? tok : 0)) * a.n_q + head * group + (ok ? h : 0)) * D;
 #pragma unroll
           for (int u = 0; u < DC; u++) {
             const int d = u * 64 + qp * 8;
@@ -346,34 +332,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           }
         }
       }
-      auto source = [&](const char* pages, int slot, int d) {
-        return pages + max(slot, 0) * row_bytes + head_bytes + (d < D ? d : 0) * (I8 ? 1 : 2);
-      };
-      auto copy_units = [&](const char* pages, const int (&slot)[kRows]) {  // bf16
+      auto copy_units = [&](const char* pages, const long long (&at)[kRows]) {  // bf16
 #pragma unroll
         for (int u = 0; u < DC; u++) {
           slot_free();
-          const uint32_t dst = ring + (unit % UNITS) * kUnit;
-          const int d = u * 64 + piece * 8;
+          const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128 + ((piece ^ (row0 & 7)) << 4);  // rows of a thread are 16 apart
+          const bool in = u + 1 < DC || u * 64 + piece * 8 < D;
 #pragma unroll
-          for (int i = 0; i < kRows; i++) {
-            const int r = row0 + kRowStep * i;
-            copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), source(pages, slot[i], d), slot[i] >= 0 && d < D);
-          }
+          for (int i = 0; i < kRows; i++)
+            copy16(dst + i * kRowStep * 128, pages + (in ? max(at[i], 0ll) + u * 128 : 0), in && at[i] >= 0);
           hand_over();
         }
       };
       // int8: groups of up to two units go through registers, the next group asked for before one is widened
       constexpr int G = DC > 1 ? 2 : 1;
       uint4 x[I8 ? G : 1][kRows], y[I8 ? G : 1][kRows];
-      auto load = [&](uint4 (&to)[I8 ? G : 1][kRows], const char* pages, const int (&slot)[kRows], int u0) {
+      auto load = [&](uint4 (&to)[I8 ? G : 1][kRows], const char* pages, const long long (&at)[kRows], int u0) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
           if (u0 + g >= DC) continue;
-          const int d = (u0 + g) * 64 + piece * 16;
+          const bool in = u0 + g + 1 < DC || (u0 + g) * 64 + piece * 16 < D;
 #pragma unroll
           for (int i = 0; i < kRows; i++)
-            to[I8 ? g : 0][i] = slot[i] >= 0 && d < D ? __ldg(reinterpret_cast<const uint4*>(source(pages, slot[i], d))) : make_uint4(0, 0, 0, 0);
+            to[I8 ? g : 0][i] = in && at[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(pages + at[i] + (u0 + g) * 64)) : make_uint4(0, 0, 0, 0);
         }
       };
       auto store = [&](const uint4 (&from)[I8 ? G : 1][kRows], int u0) {
@@ -397,57 +378,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       };
       const char* const kp = (const char*)a.k;
       const char* const vp = (const char*)a.vv;
+      int own = 0;
+      float own_k = 0.f, own_v = 0.f;
+      auto turn = [&](int b) {  // the block that was asked for becomes the one to copy
+        const int key0 = key_of(b);
+#pragma unroll
+        for (int i = 0; i < kRows; i++) {
+          const int slot = slot_at(key0 + row0 + kRowStep * i, next_page[i]);
+          val_at[i] = key_at[i];
+          key_at[i] = slot < 0 ? -1 : slot * row_bytes + (head_bytes + piece * 16);
+        }
+        own = slot_at(key0 + t, next_own);
+        if (I8) {
+          const float* sc = a.scales + (long long)max(own, 0) * 2 * v.n_kv + head;
+          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_k) : "l"(sc));
+          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_v) : "l"(sc + v.n_kv));
+        }
+      };
+      turn(b0);
       if (I8) {
-        load(x, kp, key_slot, 0);
+        load(x, kp, key_at, 0);
         asm volatile("cp.async.wait_all;" ::: "memory");  // the queries
       }
-      for (int b = w.b0; b <= w.b1; b++) {
-        const bool keys = b < w.b1, values = b > w.b0, more = b + 1 < w.b1;
-        if (more) {
-          slots_of(b + 1, next_slot);
-          next_own = slot_at(tile_block(w.ts, b + 1) * kKeyBlock + t);
-        }
+      release_item(items);
+      for (int b = b0; b <= b1; b++) {
+        const bool keys = b < b1, values = b > b0, more = b + 1 < b1;
+        if (more) ask_block(b + 1);
         if (keys) {  // what this block's keys are, by one thread a key
           Meta& m = meta[blocks % kMetaBlocks];
           blocks++;
-          const uint32_t bits = __ballot_sync(0xffffffffu, own_slot >= 0);
+          const uint32_t bits = __ballot_sync(0xffffffffu, own >= 0);
           if (lane == 0) m.holds[t >> 5] = bits;
+          if (t == 0) m.key0 = key_of(b);
           if (I8) {
-            const float* sc = a.scales + (long long)max(own_slot, 0) * 2 * v.n_kv + w.head;
-            m.k_scale[t] = own_slot >= 0 ? __ldg(sc) : 0.f;
-            m.v_scale[t] = own_slot >= 0 ? __ldg(sc + v.n_kv) : 0.f;
+            m.k_scale[t] = own >= 0 ? own_k : 0.f;
+            m.v_scale[t] = own >= 0 ? own_v : 0.f;
           }
         }
         if (!I8) {
-          if (keys) copy_units(kp, key_slot);
-          if (values) copy_units(vp, val_slot);
+          if (keys) copy_units(kp, key_at);
+          if (values) copy_units(vp, val_at);
+          if (keys) turn(more ? b + 1 : b);
         } else if (DC <= 2) {
-          if (values) load(y, vp, val_slot, 0);
-          if (keys) store(x, 0);
-          if (more) load(x, kp, next_slot, 0);
+          if (values) load(y, vp, val_at, 0);
+          if (keys) {
+            store(x, 0);
+            turn(more ? b + 1 : b);
+          }
+          if (more) load(x, kp, key_at, 0);
           if (values) store(y, 0);
         } else {
           if (keys) {
-            load(y, kp, key_slot, 2);
+            load(y, kp, key_at, 2);
             store(x, 0);
           }
-          if (values) load(x, vp, val_slot, 0);
+          if (values) load(x, vp, val_at, 0);
           if (keys) store(y, 2);
           if (values) {
-            load(y, vp, val_slot, 2);
+            load(y, vp, val_at, 2);
             store(x, 0);
           }
-          if (more) load(x, kp, next_slot, 0);
+          if (keys) turn(more ? b + 1 : b);
+          if (more) load(x, kp, key_at, 0);
           if (values) store(y, 2);
         }
-#pragma unroll
-        for (int i = 0; i < kRows; i++) {
-          val_slot[i] = key_slot[i];
-          key_slot[i] = next_slot[i];
-        }
-        own_slot = next_own;
       }
-    } while (w.next(a));
+    }
     asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else if (warp >= kSoftmaxWarps + kCopyWarps) {
@@ -458,10 +454,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kKeyBlock >> 3) << 17) | (8u << 24);
     uint32_t unit = 0, blocks = 0;
     auto lo_of = [](uint32_t at) { return ((at & 0x3FFFF) >> 4) | (64u << 16); };
-    Walker w;
-    w.start(a, c, begin, end, per_head, n_tiles);
-    do {
+    for (uint32_t items = 0;; items++) {
+      const Item& w = take_item(items);
       const int n = w.b1 - w.b0;
+      if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
+      release_item(items);
       for (int b = 0; b <= n; b++) {
         if (b < n) {  // scores of block b
           const uint32_t s_tmem = tmem + ((blocks + b) & 1) * 128;
@@ -502,7 +499,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         }
       }
       blocks += n;
-    } while (w.next(a));
+    }
+    } else if (works && warp == kSoftmaxWarps + kCopyWarps + 1 && lane == 0) {
+      // ---------------------------------------------- the block's items
+      long long cur = begin;
+      int head = (int)(begin / per_head), seq = c.start_seq, tile = c.start_tile, index = c.start_index, off = c.start_off;
+      Span span = span_of(a, seq);
+      int tiles = tiles_of(a, span);
+      for (uint32_t i = 0;; i++) {
+        if (i >= kItems) wait(c.item_empty[i % kItems], (i / kItems - 1) & 1, 311);
+        if (gave_up) break;
+        Item& w = c.items[i % kItems];
+        if (cur >= end) {
+          w.tokens = 0;
+          mbar_arrive(smem_u32(&c.item_full[i % kItems]));
+          break;
+        }
+        const TileSpan ts = tile_span(span.ctx, span.n, tile, tpt, a.window, a.sinks, v.capacity);
+        const int b1 = (int)min((long long)ts.blocks, off + (end - cur));
+        w.seq = seq; w.head = head; w.index = index;
+        w.row0 = span.row0 + tile * tpt;
+        w.tokens = min(tpt, span.n - tile * tpt);
+        w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
+        w.near_key = ts.near_key; w.end_key = ts.end_key; w.sink_blocks = ts.sink_blocks; w.near_block = ts.near_block; w.blocks = ts.blocks;
+        w.b0 = off; w.b1 = b1;
+        w.w0 = cur - off;
+        mbar_arrive(smem_u32(&c.item_full[i % kItems]));
+        cur += b1 - off;
+        if (cur >= end) continue;
+        off = 0;
+        tile++;
+        if (++index >= n_tiles) {  // the next head begins
+          index = 0;
+          head++;
+          seq = -1;
+          tile = tiles;
+        }
+        if (tile >= tiles) {
+          tile = 0;
+          do {
+            if (++seq >= v.S) seq = 0;  // there is a tile, so a sequence with one
+            span = span_of(a, seq);
+            tiles = tiles_of(a, span);
+          } while (!tiles);
+        }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -513,15 +554,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     const int tok = page_of(row, a.group_div), pieces = D >> 4;
     const float cexp = a.scale * 1.4426950408889634f;
     uint32_t blocks = 0, items = 0;
-    Walker w;
-    w.start(a, c, begin, end, per_head, n_tiles);
-    do {
-      const int tokens = min(tpt, w.span.n - w.tile * tpt), used = tokens * group, n = w.b1 - w.b0;
+    for (;; items++) {
+      if (tid == 0) {  // one decides for all, who meet at barriers from here on
+        const Item& w = take_item(items);
+        c.stop = gave_up || *(volatile int*)&c.abort || !w.tokens;
+      }
+      named_sync(5, kSoftmaxThreads);
+      if (c.stop) break;
+      const Item& w = c.items[items % kItems];
+      const int tokens = w.tokens, used = tokens * group, n = w.b1 - w.b0, first_pos = w.first_pos;
       const bool warp_used = (warp & 3) * 32 < used;
-      const long long p64 = (long long)w.span.ctx + w.tile * tpt + min(tok, tokens - 1);
-      const int pos = (int)min(p64, 0x7fffffffll);
-      const int first_pos = (int)min((long long)w.span.ctx + w.tile * tpt, 0x7fffffffll);
-      const int last_pos = (int)min((long long)w.span.ctx + w.tile * tpt + tokens - 1, 0x7fffffffll);
+      const int pos = (int)min((long long)first_pos + min(tok, tokens - 1), 0x7fffffffll);
+      const int last_pos = (int)min((long long)first_pos + tokens - 1, 0x7fffffffll);
       const int near = a.window ? max(0, pos - a.window + 1) : 0;  // this row sees keys [near, pos] and those in front of sinks
       float m = -INFINITY, sum = 0.f;
       for (int b = 0; b < n; b++, blocks++) {
@@ -537,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         tmem_ld32_issue(s_tmem, s0);
         tmem_ld32_issue(s_tmem + 32, s1);
         const Meta& mt = meta[blocks % kMetaBlocks];
-        const int block = tile_block(w.ts, w.b0 + b), key0 = block * kKeyBlock + half * 64;
+        const int key0 = mt.key0 + half * 64;
         const uint32_t holds0 = mt.holds[half * 2], holds1 = mt.holds[half * 2 + 1];
         const bool partial = (holds0 & holds1) != 0xffffffffu || key0 + 63 > first_pos ||
                              (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
@@ -604,12 +648,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             unpack_f32(mul_f32x2(add_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), minus), scale2), x, y);
             x = exp2_fast(x);
             y = exp2_fast(y);
-            parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(x, y));
             if (I8) {
+              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(x, y));
               const float2 vs = *reinterpret_cast<const float2*>(v_scale + i);
               unpack_f32(mul_f32x2(pack_f32(x, y), pack_f32(vs.x, vs.y)), x, y);
+              p[i >> 1] = pack_bf16(x, y);
+            } else {  // the sum is that of the weights as they are used: what their rounding does to a row's size cancels
+              const uint32_t w2 = p[i >> 1] = pack_bf16(x, y);
+              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(__uint_as_float(w2 << 16), __uint_as_float(w2 & 0xffff0000u)));
             }
-            p[i >> 1] = pack_bf16(x, y);
           }
           tmem_st16(to, p);
         };
@@ -626,14 +673,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       }
       // ---- the item's rows: finished, or left for whoever finishes the tile
       wait(c.o_done, items & 1, 309);
-      items++;
       tc_fence_after();
       c.top[0][half][row] = sum;
       named_sync(5, kSoftmaxThreads);
       const float l = c.top[0][0][row] + c.top[0][1][row];
       named_sync(5, kSoftmaxThreads);
       const bool mine = row < used;
-      const int my_row = w.span.row0 + w.tile * tpt + tok, my_head = w.head * group + row - tok * group;
+      const int my_row = w.row0 + tok, my_head = w.head * group + row - tok * group;
       uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
       bool finite = true;
       auto store = [&](uint16_t* at, const float (&o)[16], float inv) {
@@ -649,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         to[1] = make_uint4(p[4], p[5], p[6], p[7]);
       };
       bool done = true;
-      if (!w.split()) {
+      if (n == w.blocks) {
         if (warp_used) {
           const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
           for (int i = half; i < pieces; i += 2) {
@@ -663,8 +709,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         }
       } else {
         // partial sums: [four columns][row][4] and (m, l) of every row, in one of this block's two places
-        const long long w0 = w.cur - w.b0;
-        const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.ts.blocks - 1, total, parts);
+        const long long w0 = w.w0;
+        const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.blocks - 1, total, parts);
         auto place = [&](int part) { return part * 2 + (part == first && work_begin(total, part, parts) < w0 ? 1 : 0); };
         const long long floats = (long long)(D + 2) * 128;
         {
@@ -745,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             }
             const int tk = page_of(r, a.group_div);
             finite = true;
-            store(a.out + ((long long)(w.span.row0 + w.tile * tpt + tk) * a.n_q + w.head * group + r - tk * group) * D + pc * 16, o, inv);
+            store(a.out + ((long long)(w.row0 + tk) * a.n_q + w.head * group + r - tk * group) * D + pc * 16, o, inv);
             if (!finite) atomicOr(&c.bad_rows[r >> 5], 1u << (r & 31));
             finite = true;
           }
@@ -760,15 +806,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           for (int r = 0; r < used; r++) {
             if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
             const int tk = page_of(r, a.group_div);
-            const long long p = (long long)w.span.ctx + w.tile * tpt + tk;
-            attend_row(a, plain, tid, w.span.row0 + w.tile * tpt + tk, w.head * group + r - tk * group, w.seq, (int)min(p, 0x7fffffffll), sync);
+            const long long p = (long long)w.first_pos + tk;
+            attend_row(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min(p, 0x7fffffffll), sync);
           }
           if (tid < 4) c.bad_rows[tid] = 0;
         }
       }
       tc_fence_before();
       named_sync(5, kSoftmaxThreads);  // everybody has read O, the exchange and the flags
-    } while (w.next(a));
+      release_item(items);
+    }
     }
   }
   tc_fence_before();
