@@ -388,6 +388,7 @@ struct AttnPagedArgs {
   int* status;
   // filled by attn_paged_shape
   int tokens_per_tile, max_tiles, grid;
+  int box_rows;        // keys that lie one behind another wherever their block starts: the largest power of two in the page size, 8 .. 128, or 0
   PageDivisor group_div;
   // filled by the launchers
   int few_rows;        // sequences with at most so many rows (tokens x query heads of a key/value head) are the other kernel's

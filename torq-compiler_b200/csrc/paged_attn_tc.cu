@@ -18,16 +18,19 @@
 #include "paged.cuh"
 #include "paged_row.cuh"
 #include "tcgen05_ptx.cuh"
+#include "tensor_map.h"
 
 namespace tb200 {
 
 namespace {
 
-// four warpgroups: two for softmax, one that copies, one whose first warp issues matrix instructions; the registers go where they are needed
-// (256 x 176 + 128 x 104 + 128 x 56 of the 512 x 128 that a block starts with)
+// four warpgroups: two for softmax, one that widens int8 caches, one with a warp each for matrix instructions, items and the copy engine; the
+// registers go where they are needed (of the 512 x 128 that a block starts with)
 constexpr int kSoftmaxWarps = 8, kCopyWarps = 4, kThreads = 512;
-constexpr int kSoftmaxRegs = 176, kCopyRegs = 104, kIssueRegs = 56;
-static_assert(kSoftmaxWarps * 32 * kSoftmaxRegs + kCopyWarps * 32 * kCopyRegs + 128 * kIssueRegs <= kThreads * 128, "register split");
+constexpr int kCopyRegs = 104, kIssueRegs = 56;
+constexpr int kSoftmaxRegsI8 = 176, kSoftmaxRegs = 200;  // a bf16 cache's copies leave more
+static_assert(256 * kSoftmaxRegsI8 + 128 * kCopyRegs + 128 * kIssueRegs <= kThreads * 128, "register split, int8");
+static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreads * 128, "register split, bf16");
 constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
 constexpr int kMetaBlocks = 8, kItems = 4;
@@ -49,7 +52,7 @@ struct Item {
   long long w0;             // where the tile's work begins
 };
 struct Control {
-  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_empty, item_full[kItems], item_empty[kItems];
+  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty, item_full[kItems], item_empty[kItems];
   Item items[kItems];
   uint32_t tmem, bad_rows[4], arrived;
   int abort, stop;
@@ -73,6 +76,32 @@ __device__ __forceinline__ Span span_of(const AttnPagedArgs& a, int s) {
 __device__ __forceinline__ int tiles_of(const AttnPagedArgs& a, const Span& s) {
   return s.n * (a.n_q / a.v.n_kv) > a.few_rows ? (s.n + a.tokens_per_tile - 1) / a.tokens_per_tile : 0;
 }
+
+// The keys of an item, and where the cache holds them. Page ids are asked for a block ahead of their use, without a branch (a branch would wait
+// for each); slots have 32 bits (the planner refuses more), -1 where no token of the tile sees the key or nothing is held.
+struct Keys {
+  const int32_t* pages_of;
+  int near_key, end_key, sinks, sink_blocks, near_block, last, pages, page_size;
+  PageDivisor div;
+  __device__ __forceinline__ Keys(const AttnPagedArgs& a, const Item& w)
+      : pages_of(a.v.table + (long long)w.seq * a.v.max_pages), near_key(w.near_key), end_key(w.end_key), sinks(a.sinks), sink_blocks(w.sink_blocks),
+        near_block(w.near_block), last(a.v.capacity - 1), pages(a.v.pages), page_size(a.v.page_size), div(a.v.div) {}
+  __device__ __forceinline__ int first(int b) const { return (b < sink_blocks ? b : near_block + (b - sink_blocks)) * kKeyBlock; }
+  __device__ __forceinline__ int ask(int key) const {
+    int page;  // volatile: it is to be on its way now, not when it is used
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(page) : "l"(pages_of + page_of(min(key, last), div)));
+    return page;
+  }
+  __device__ __forceinline__ bool seen(int key) const { return key < end_key && (key >= near_key || key < sinks); }  // by a token of the tile
+  __device__ __forceinline__ int count_seen(int key, int n) const {  // of keys key .. key + n - 1
+    const int upto = min(key + n, end_key), firsts = max(0, min(min(upto, sinks), near_key) - key);
+    return firsts + max(0, upto - max(key, near_key));
+  }
+  __device__ __forceinline__ int slot(int key, int page) const {
+    const bool there = seen(key) && page >= 0 && page < pages;
+    return there ? page * page_size + (key - page_of(key, div) * page_size) : -1;
+  }
+};
 
 // Running sum over the block's threads up to and including this one, and the sum of all, through c.totals.
 __device__ long long block_scan(Control& c, long long x, long long& all) {
@@ -119,6 +148,16 @@ __device__ __forceinline__ unsigned long long mul_f32x2(unsigned long long a, un
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ unsigned long long fma_f32x2(unsigned long long a, unsigned long long b, unsigned long long d) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(d));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float d) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(d));
+  return r;
+}
 // four int8 -> four bf16, exact: 0x4300 | low seven bits of the biased byte is 128 + those bits, and 128 or 256 comes off again
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   const uint32_t u = w ^ 0x80808080u, low = u & 0x7f7f7f7fu, off = ~u & 0x80808080u;
@@ -131,13 +170,15 @@ __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {  // zeros when not valid
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
+
+// How the copy engine sees the queries and a bf16 cache: boxes of 64 dims by the rows of a tile / by box_rows keys, and single keys.
+struct TileMaps {
+  CUtensorMap q, k, v, k_rows, v_rows;
+};
 
 // DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
 template <int DC, int UNITS, bool I8>
-__global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const AttnPagedArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
   extern __shared__ unsigned char smem_raw[];
   // [Q units][ring units] on 1024-byte boundaries, then the rest
   unsigned char* const base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -156,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   }
   if (tid == 32) {
     for (int i = 0; i < UNITS; i++) {
-      mbar_init(smem_u32(&c.full[i]), I8 ? kCopyThreads : 2 * kCopyThreads);
+      mbar_init(smem_u32(&c.full[i]), I8 ? kCopyThreads : 1);
       mbar_init(smem_u32(&c.empty[i]), 1);
     }
     for (int i = 0; i < 2; i++) {  // a softmax warp may be one block ahead of another: a barrier for each buffer
@@ -167,8 +208,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     mbar_init(smem_u32(&c.o_done), 1);
     for (int i = 0; i < kItems; i++) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + kCopyThreads + 32);
+      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + 64 + (I8 ? kCopyThreads : 0));
     }
+    mbar_init(smem_u32(&c.q_full), 1);
     mbar_init(smem_u32(&c.q_empty), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     c.abort = 0;
@@ -264,143 +306,86 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   auto release_item = [&](uint32_t i) { mbar_arrive(smem_u32(&c.item_empty[i % kItems])); };
   const uint32_t o_tmem = tmem + 256;
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
-    // ------------------------------------------------ copies
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegs));
-    if (works) {
+    // ------------------------------------------------ copies of int8 caches: widened on the way
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(I8 ? kCopyRegs : kIssueRegs));
+    if (I8 && works) {
     const int t = tid - kSoftmaxThreads;
-    uint32_t unit = 0;       // units asked for so far
-    uint32_t blocks = 0;
-    auto slot_free = [&]() {  // room for unit `unit`
-      if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
-    };
-    // This thread's part of unit `unit`: what it has stored itself is handed over with a fence towards the matrix instructions, what its
-    // asynchronous copies bring when they arrive (the issuing warp fences). The plain arrival covers the block's Meta either way.
-    auto hand_over = [&]() {
-      const uint32_t bar = smem_u32(&c.full[unit % UNITS]);
-      if (I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      else asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-      mbar_arrive(bar);
-      unit++;
-    };
-    constexpr int kRows = I8 ? 4 : 8;           // rows of a unit that a thread copies a piece of
-    constexpr int kPieces = I8 ? 4 : 8;         // pieces of 16 bytes in a unit's row
+    uint32_t unit = 0, blocks = 0;
+    constexpr int kRows = 4, kPieces = 4, kRowStep = kCopyThreads / kPieces;  // pieces of 16 bytes: a thread has the same one of four rows
     const int piece = t % kPieces, row0 = t / kPieces;
-    constexpr int kRowStep = kCopyThreads / kPieces;
-    const long long row_bytes = (long long)v.n_kv * D * (I8 ? 1 : 2);
+    const long long row_bytes = (long long)v.n_kv * D;
     for (uint32_t items = 0;; items++) {
       const Item& w = take_item(items);
       if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
-      const int b0 = w.b0, b1 = w.b1, near_key = w.near_key, end_key = w.end_key, sink_blocks = w.sink_blocks, near_block = w.near_block;
-      const int used = w.tokens * group, head = w.head;
-      const long long head_bytes = (long long)head * D * (I8 ? 1 : 2);
-      // queries: they are there when the first unit of keys behind them is
-      if (items) wait(c.q_empty, (items - 1) & 1, 302);
-      // A block's keys: the page ids are asked for a block ahead of their use, without a branch (a branch would wait for each), and turned into
-      // slots (32 bits: the planner refuses more) when the block is copied; -1 where no token of the tile sees the key or nothing is held.
-      const int32_t* const pages_of = v.table + (long long)w.seq * v.max_pages;
-      auto key_of = [&](int b) { return (b < sink_blocks ? b : near_block + (b - sink_blocks)) * kKeyBlock; };
-      auto ask = [&](int key) {
-        int page;  // volatile: it is to be on its way now, not when it is used
-        asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(page) : "l"(pages_of + page_of(min(key, v.capacity - 1), v.div)));
-        return page;
-      };
-      auto slot_at = [&](int key, int page) {
-        const bool there = key < end_key && (key >= near_key || key < a.sinks) && page >= 0 && page < v.pages;
-        return there ? page * v.page_size + (key - page_of(key, v.div) * v.page_size) : -1;
-      };
+      const int b0 = w.b0, b1 = w.b1, head = w.head;
+      const Keys keys_of(a, w);
+      release_item(items);
       int next_page[kRows], next_own;
       auto ask_block = [&](int b) {
-        const int key0 = key_of(b);
+        const int key0 = keys_of.first(b);
 #pragma unroll
-        for (int i = 0; i < kRows; i++) next_page[i] = ask(key0 + row0 + kRowStep * i);
-        next_own = ask(key0 + t);
+        for (int i = 0; i < kRows; i++) next_page[i] = keys_of.ask(key0 + row0 + kRowStep * i);
+        next_own = keys_of.ask(key0 + t);
       };
       // where this thread's pieces of the keys and of the values of a block start, in bytes behind the cache; negative: zeros
       long long key_at[kRows], val_at[kRows];
-      ask_block(b0);
-      {
-        const int qp = t & 7, q_row = w.row0;
+      int own = 0;
+      float own_k = 0.f, own_v = 0.f;
+      auto turn = [&](int b) {  // the block that was asked for becomes the one to copy
+        const int key0 = keys_of.first(b);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int r = (t >> 3) + 16 * i, tok = page_of(r, a.group_div), h = r - tok * group;
-          const bool ok = r < used;
-          const uint16_t* src = a.q + ((long long)(q_row + (ok ? tok : 0)) * a.n_q + head * group + (ok ? h : 0)) * D;
-#pragma unroll
-          for (int u = 0; u < DC; u++) {
-            const int d = u * 64 + qp * 8;
-            copy16(q_smem + u * kUnit + r * 128 + ((qp ^ (r & 7)) << 4), src + (d < D ? d : 0), ok && d < D);
-          }
+        for (int i = 0; i < kRows; i++) {
+          const int slot = keys_of.slot(key0 + row0 + kRowStep * i, next_page[i]);
+          val_at[i] = key_at[i];
+          key_at[i] = slot < 0 ? -1 : slot * row_bytes + ((long long)head * D + piece * 16);
         }
-      }
-      auto copy_units = [&](const char* pages, const long long (&at)[kRows]) {  // bf16
-#pragma unroll
-        for (int u = 0; u < DC; u++) {
-          slot_free();
-          const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128 + ((piece ^ (row0 & 7)) << 4);  // rows of a thread are 16 apart
-          const bool in = u + 1 < DC || u * 64 + piece * 8 < D;
-#pragma unroll
-          for (int i = 0; i < kRows; i++)
-            copy16(dst + i * kRowStep * 128, pages + (in ? max(at[i], 0ll) + u * 128 : 0), in && at[i] >= 0);
-          hand_over();
-        }
+        own = keys_of.slot(key0 + t, next_own);
+        const float* sc = a.scales + (long long)max(own, 0) * 2 * v.n_kv + head;
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_k) : "l"(sc));
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_v) : "l"(sc + v.n_kv));
       };
-      // int8: groups of up to two units go through registers, the next group asked for before one is widened
+      // groups of up to two units go through registers, the next group asked for before one is widened
       constexpr int G = DC > 1 ? 2 : 1;
-      uint4 x[I8 ? G : 1][kRows], y[I8 ? G : 1][kRows];
-      auto load = [&](uint4 (&to)[I8 ? G : 1][kRows], const char* pages, const long long (&at)[kRows], int u0) {
+      uint4 x[G][kRows], y[G][kRows];
+      auto load = [&](uint4 (&to)[G][kRows], const void* pages, const long long (&at)[kRows], int u0) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
           if (u0 + g >= DC) continue;
           const bool in = u0 + g + 1 < DC || (u0 + g) * 64 + piece * 16 < D;
 #pragma unroll
-          for (int i = 0; i < kRows; i++)
-            to[I8 ? g : 0][i] = in && at[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(pages + at[i] + (u0 + g) * 64)) : make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < kRows; i++) {
+            to[g][i] = make_uint4(0, 0, 0, 0);
+            if (in && at[i] >= 0)
+              asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(to[g][i].x), "=r"(to[g][i].y), "=r"(to[g][i].z), "=r"(to[g][i].w)
+                           : "l"((const char*)pages + at[i] + (u0 + g) * 64));
+          }
         }
       };
-      auto store = [&](const uint4 (&from)[I8 ? G : 1][kRows], int u0) {
+      auto store = [&](const uint4 (&from)[G][kRows], int u0) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
           if (u0 + g >= DC) continue;
-          slot_free();
+          if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
           const uint32_t dst = ring + (unit % UNITS) * kUnit;
 #pragma unroll
           for (int i = 0; i < kRows; i++) {
             const int r = row0 + kRowStep * i;
-            const uint4 q = from[I8 ? g : 0][i];
+            const uint4 q = from[g][i];
             uint4 lo, hi;
             widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
             widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
             sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
             sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
           }
-          hand_over();
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(smem_u32(&c.full[unit % UNITS]));
+          unit++;
         }
       };
-      const char* const kp = (const char*)a.k;
-      const char* const vp = (const char*)a.vv;
-      int own = 0;
-      float own_k = 0.f, own_v = 0.f;
-      auto turn = [&](int b) {  // the block that was asked for becomes the one to copy
-        const int key0 = key_of(b);
-#pragma unroll
-        for (int i = 0; i < kRows; i++) {
-          const int slot = slot_at(key0 + row0 + kRowStep * i, next_page[i]);
-          val_at[i] = key_at[i];
-          key_at[i] = slot < 0 ? -1 : slot * row_bytes + (head_bytes + piece * 16);
-        }
-        own = slot_at(key0 + t, next_own);
-        if (I8) {
-          const float* sc = a.scales + (long long)max(own, 0) * 2 * v.n_kv + head;
-          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_k) : "l"(sc));
-          asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_v) : "l"(sc + v.n_kv));
-        }
-      };
+      ask_block(b0);
       turn(b0);
-      if (I8) {
-        load(x, kp, key_at, 0);
-        asm volatile("cp.async.wait_all;" ::: "memory");  // the queries
-      }
-      release_item(items);
+      load(x, a.k, key_at, 0);
       for (int b = b0; b <= b1; b++) {
         const bool keys = b < b1, values = b > b0, more = b + 1 < b1;
         if (more) ask_block(b + 1);
@@ -409,42 +394,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           blocks++;
           const uint32_t bits = __ballot_sync(0xffffffffu, own >= 0);
           if (lane == 0) m.holds[t >> 5] = bits;
-          if (t == 0) m.key0 = key_of(b);
-          if (I8) {
-            m.k_scale[t] = own >= 0 ? own_k : 0.f;
-            m.v_scale[t] = own >= 0 ? own_v : 0.f;
-          }
+          if (t == 0) m.key0 = keys_of.first(b);
+          m.k_scale[t] = own >= 0 ? own_k : 0.f;
+          m.v_scale[t] = own >= 0 ? own_v : 0.f;
         }
-        if (!I8) {
-          if (keys) copy_units(kp, key_at);
-          if (values) copy_units(vp, val_at);
-          if (keys) turn(more ? b + 1 : b);
-        } else if (DC <= 2) {
-          if (values) load(y, vp, val_at, 0);
+        if (DC <= 2) {
+          if (values) load(y, a.vv, val_at, 0);
           if (keys) {
             store(x, 0);
             turn(more ? b + 1 : b);
           }
-          if (more) load(x, kp, key_at, 0);
+          if (more) load(x, a.k, key_at, 0);
           if (values) store(y, 0);
         } else {
           if (keys) {
-            load(y, kp, key_at, 2);
+            load(y, a.k, key_at, 2);
             store(x, 0);
           }
-          if (values) load(x, vp, val_at, 0);
+          if (values) load(x, a.vv, val_at, 0);
           if (keys) store(y, 2);
           if (values) {
-            load(y, vp, val_at, 2);
+            load(y, a.vv, val_at, 2);
             store(x, 0);
           }
           if (keys) turn(more ? b + 1 : b);
-          if (more) load(x, kp, key_at, 0);
+          if (more) load(x, a.k, key_at, 0);
           if (values) store(y, 2);
         }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else if (warp >= kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ matrix instructions
@@ -459,13 +437,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const int n = w.b1 - w.b0;
       if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
       release_item(items);
+      wait(c.q_full, items & 1, 303);
       for (int b = 0; b <= n; b++) {
         if (b < n) {  // scores of block b
           const uint32_t s_tmem = tmem + ((blocks + b) & 1) * 128;
 #pragma unroll
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
-            if (!I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_after();
             const uint32_t qa = lo_of(q_smem + u * kUnit), kb = lo_of(ring + (unit % UNITS) * kUnit);
             const int steps = min(4, (D - u * 64) >> 4);
@@ -483,7 +461,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 306);
-            if (!I8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_after();
             const int width = min(64, D - u * 64);
             const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(width >> 3) << 17) | (8u << 24);
@@ -500,6 +477,124 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       }
       blocks += n;
     }
+    } else if (works && warp == kSoftmaxWarps + kCopyWarps + 2) {
+      // ---------------------------------------------- queries, and bf16 caches, by the copy engine: a lane asks for four rows of 128 bytes at once
+      uint32_t unit = 0, blocks = 0;
+      for (uint32_t items = 0;; items++) {
+        const Item& w = take_item(items);
+        if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
+        const int b0 = w.b0, b1 = w.b1, head = w.head, q_row = w.row0;
+        const Keys keys_of(a, w);
+        release_item(items);
+        if (items) wait(c.q_empty, (items - 1) & 1, 302);
+        __syncwarp();
+        if (lane == 0) {  // rows of the tile's tokens, in the tile's order; those behind the last token are somebody's or nobody's, and are not used
+          const uint32_t bar = smem_u32(&c.q_full);
+          mbar_expect_tx(bar, DC * 128 * tpt * group);
+          for (int u = 0; u < DC; u++) tma_load_3d(q_smem + u * kUnit, &maps.q, u * 64, head * group, q_row, bar);
+        }
+        if (I8) continue;
+        auto begin_unit = [&]() {
+          const uint32_t slot = unit % UNITS;
+          if (unit >= UNITS) wait(c.empty[slot], (unit / UNITS - 1) & 1, 301);
+          __syncwarp();
+          if (lane == 0) mbar_expect_tx(smem_u32(&c.full[slot]), kUnit);
+          __syncwarp();
+          unit++;
+          return slot;
+        };
+        auto tell = [&](int key0, uint32_t held) {  // the block's keys, before its first unit
+          Meta& m = meta[blocks % kMetaBlocks];
+          blocks++;
+          if ((lane & 7) == 0) m.holds[lane >> 3] = held;
+          if (lane == 0) m.key0 = key0;
+          __syncwarp();
+        };
+        auto gather_bits = [&](uint32_t nibble) {  // four keys a lane -> the 32 of its eight lanes
+          uint32_t held = nibble << (4 * (lane & 7));
+          held |= __shfl_xor_sync(0xffffffffu, held, 1);
+          held |= __shfl_xor_sync(0xffffffffu, held, 2);
+          return held | __shfl_xor_sync(0xffffffffu, held, 4);
+        };
+        // four keys to a lane: where pages end anywhere, and for runs of keys that are seen in part
+        auto gather = [&](const CUtensorMap* map, uint32_t slot, int u, int first, const int (&r)[4]) {
+          tma_gather4(ring + slot * kUnit + first * 128, map, u * 64, r[0], r[1], r[2], r[3], smem_u32(&c.full[slot]));
+        };
+        if (!a.box_rows) {
+          int next_page[4], key_row[4], val_row[4] = {};
+          auto ask_block = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) next_page[i] = keys_of.ask(keys_of.first(b) + 4 * lane + i);
+          };
+          ask_block(b0);
+          for (int b = b0; b <= b1; b++) {
+            if (b < b1) {
+              const int key0 = keys_of.first(b);
+              uint32_t nibble = 0;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int slot = keys_of.slot(key0 + 4 * lane + i, next_page[i]);
+                key_row[i] = slot < 0 ? -1 : slot * v.n_kv + head;
+                nibble |= (slot >= 0 ? 1u : 0u) << i;
+              }
+              if (b + 1 < b1) ask_block(b + 1);
+              tell(key0, gather_bits(nibble));
+              for (int u = 0; u < DC; u++) gather(&maps.k_rows, begin_unit(), u, 4 * lane, key_row);
+            }
+            if (b > b0)
+              for (int u = 0; u < DC; u++) gather(&maps.v_rows, begin_unit(), u, 4 * lane, val_row);
+#pragma unroll
+            for (int i = 0; i < 4; i++) val_row[i] = key_row[i];
+          }
+        } else {
+          // a run of box_rows keys to a lane: one box where all are seen (or none: from outside the cache, zeros), else four by four
+          const int R = a.box_rows, runs = kKeyBlock / R, none = v.pages * v.page_size;
+          int next_page, key_run = 0, val_run = 0;  // slot of a run's first key, or `none`
+          uint32_t key_parts = 0, val_parts = 0;    // runs that are seen in part
+          int key_first = 0, val_first = 0;
+          auto copy_units = [&](const CUtensorMap* map, const CUtensorMap* rows, int run, uint32_t parts, int key0) {
+            for (int u = 0; u < DC; u++) {
+              const uint32_t slot = begin_unit();
+              if (lane < runs && !(parts >> lane & 1)) tma_load_3d(ring + slot * kUnit + lane * R * 128, map, u * 64, head, run, smem_u32(&c.full[slot]));
+              for (uint32_t left = parts; left; left &= left - 1) {
+                const int g = __ffs(left) - 1, from = __shfl_sync(0xffffffffu, run, g);
+                if (4 * lane < R) {
+                  int r[4];
+#pragma unroll
+                  for (int i = 0; i < 4; i++) r[i] = keys_of.seen(key0 + g * R + 4 * lane + i) ? (from + 4 * lane + i) * v.n_kv + head : -1;
+                  gather(rows, slot, u, g * R + 4 * lane, r);
+                }
+              }
+            }
+          };
+          auto ask_block = [&](int b) { next_page = keys_of.ask(min(keys_of.first(b) + lane * R, keys_of.last)); };
+          ask_block(b0);
+          for (int b = b0; b <= b1; b++) {
+            if (b < b1) {
+              const int key0 = key_first = keys_of.first(b), mine = key0 + min(lane, runs - 1) * R;
+              // the run of this lane, then the four keys of this lane
+              const bool held = next_page >= 0 && next_page < v.pages && mine <= keys_of.last;
+              const int seen = held ? keys_of.count_seen(mine, R) : 0;
+              key_run = seen ? next_page * v.page_size + (mine - page_of(mine, v.div) * v.page_size) : none;
+              key_parts = __ballot_sync(0xffffffffu, lane < runs && seen > 0 && seen < R);
+              const uint32_t any = __ballot_sync(0xffffffffu, seen > 0);
+              if (b + 1 < b1) ask_block(b + 1);
+              uint32_t nibble = 0;
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const int k = 4 * lane + i;
+                nibble |= ((any >> (k / R) & 1) && keys_of.seen(key0 + k) ? 1u : 0u) << i;
+              }
+              tell(key0, gather_bits(nibble));
+              copy_units(&maps.k, &maps.k_rows, key_run, key_parts, key0);
+            }
+            if (b > b0) copy_units(&maps.v, &maps.v_rows, val_run, val_parts, val_first);
+            val_run = key_run;
+            val_parts = key_parts;
+            val_first = key_first;
+          }
+        }
+      }
     } else if (works && warp == kSoftmaxWarps + kCopyWarps + 1 && lane == 0) {
       // ---------------------------------------------- the block's items
       long long cur = begin;
@@ -546,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(I8 ? kSoftmaxRegsI8 : kSoftmaxRegs));
     if (works) {
     // ------------------------------------------------ softmax: thread = (row, half of the block's keys)
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
@@ -567,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const int pos = (int)min((long long)first_pos + min(tok, tokens - 1), 0x7fffffffll);
       const int last_pos = (int)min((long long)first_pos + tokens - 1, 0x7fffffffll);
       const int near = a.window ? max(0, pos - a.window + 1) : 0;  // this row sees keys [near, pos] and those in front of sinks
-      float m = -INFINITY, sum = 0.f;
+      float m = -INFINITY, base = 0.f, sum = 0.f;  // base: m scaled, what the exponents are taken from
       for (int b = 0; b < n; b++, blocks++) {
         const uint32_t s_tmem = tmem + lanes + (blocks & 1) * 128 + half * 64;
         if (!warp_used) {  // rows of nobody: P keeps what it holds, and so does O
@@ -588,42 +683,55 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         tmem_ld_wait32(s0);
         tmem_ld_wait32(s1);
         if (I8) {
+          auto scaled = [&](uint32_t (&s)[32], const float* k_scale) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&mt.k_scale[half * 64 + i]), y = *reinterpret_cast<const float4*>(&mt.k_scale[half * 64 + 32 + i]);
-            s0[i] = __float_as_uint(__uint_as_float(s0[i]) * x.x); s0[i + 1] = __float_as_uint(__uint_as_float(s0[i + 1]) * x.y);
-            s0[i + 2] = __float_as_uint(__uint_as_float(s0[i + 2]) * x.z); s0[i + 3] = __float_as_uint(__uint_as_float(s0[i + 3]) * x.w);
-            s1[i] = __float_as_uint(__uint_as_float(s1[i]) * y.x); s1[i + 1] = __float_as_uint(__uint_as_float(s1[i + 1]) * y.y);
-            s1[i + 2] = __float_as_uint(__uint_as_float(s1[i + 2]) * y.z); s1[i + 3] = __float_as_uint(__uint_as_float(s1[i + 3]) * y.w);
-          }
+            for (int i = 0; i < 32; i += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(k_scale + i);
+              float f[4];
+              unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), pack_f32(x.x, x.y)), f[0], f[1]);
+              unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), pack_f32(x.z, x.w)), f[2], f[3]);
+#pragma unroll
+              for (int j = 0; j < 4; j++) s[i + j] = __float_as_uint(f[j]);
+            }
+          };
+          scaled(s0, mt.k_scale + half * 64);
+          scaled(s1, mt.k_scale + half * 64 + 32);
         }
         if (partial) {
+          // bits of the keys this row sees: not behind its position, inside the window or among the first, and held
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+          const uint32_t see0 = below(pos - key0 + 1) & (~below(near - key0) | below(a.sinks - key0)) & holds0;
+          const uint32_t see1 = below(pos - key0 - 31) & (~below(near - key0 - 32) | below(a.sinks - key0 - 32)) & holds1;
           const uint32_t none = __float_as_uint(-INFINITY);
 #pragma unroll
           for (int i = 0; i < 32; i++) {
-            const int k0 = key0 + i, k1 = k0 + 32;
-            const bool see0 = k0 <= pos && (k0 >= near || k0 < a.sinks) && (holds0 >> i & 1);
-            const bool see1 = k1 <= pos && (k1 >= near || k1 < a.sinks) && (holds1 >> i & 1);
-            s0[i] = see0 ? s0[i] : none;
-            s1[i] = see1 ? s1[i] : none;
+            s0[i] = see0 >> i & 1 ? s0[i] : none;
+            s1[i] = see1 >> i & 1 ? s1[i] : none;
           }
         }
-        float tops[4];
+        float tops[4] = {__uint_as_float(s0[0]), __uint_as_float(s0[1]), __uint_as_float(s1[0]), __uint_as_float(s1[1])};
 #pragma unroll
-        for (int i = 0; i < 4; i++) tops[i] = fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i]));
-#pragma unroll
-        for (int i = 4; i < 32; i++) tops[i & 3] = fmaxf(tops[i & 3], fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
-        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        for (int i = 2; i < 32; i += 2) {
+          tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+          tops[2 + (i >> 1 & 1)] = max3(tops[2 + (i >> 1 & 1)], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+        }
+        float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
         c.top[blocks & 1][half][row] = top;
         named_sync(1 + (warp & 3), 64);
         top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
         // follow the maximum when p could grow beyond 2^8, or when there was none yet
-        const bool grows = top > m && !((top - m) * cexp <= 8.f);
+        const bool grows = row < used && top > m && !((top - m) * cexp <= 8.f);
         if (b == 0) {
           m = top;
+          base = m == -INFINITY ? 0.f : m * cexp;
         } else if (__any_sync(0xffffffffu, grows)) {
-          const float keep = grows ? (m == -INFINITY ? 0.f : exp2_fast((m - top) * cexp)) : 1.f;
-          if (grows) m = top;
+          float keep = 1.f;
+          if (grows) {
+            const float to = top * cexp;
+            keep = m == -INFINITY ? 0.f : exp2_fast(base - to);
+            m = top;
+            base = to;
+          }
           sum *= keep;
           // these scores were issued behind the sums of the block before the last: its phase is over, the last one's is waited for
           wait(c.pv_done, (blocks - 1) & 1, 308);
@@ -637,26 +745,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           }
           tmem_st_wait();
         }
-        const float from = m == -INFINITY ? 0.f : m;
-        const unsigned long long minus = pack_f32(-from, -from), scale2 = pack_f32(cexp, cexp);
+        // p = 2^(s c - base) in one multiply-add: how base was rounded is the same for every key of the row, so it cancels (where that factor
+        // itself leaves fp32, at scores beyond 10^9, sums come out infinite or zero, which is caught at the end)
+        const unsigned long long scale2 = pack_f32(cexp, cexp), base2 = pack_f32(-base, -base);
         unsigned long long parts2[2] = {0ull, 0ull};  // two pairs of running sums
         auto weights = [&](const uint32_t (&s)[32], const float* v_scale, uint32_t to) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float x, y;
-            unpack_f32(mul_f32x2(add_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), minus), scale2), x, y);
-            x = exp2_fast(x);
-            y = exp2_fast(y);
+            unpack_f32(fma_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, base2), x, y);
+            unsigned long long e = pack_f32(exp2_fast(x), exp2_fast(y));
+            parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], e);
             if (I8) {
-              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(x, y));
               const float2 vs = *reinterpret_cast<const float2*>(v_scale + i);
-              unpack_f32(mul_f32x2(pack_f32(x, y), pack_f32(vs.x, vs.y)), x, y);
-              p[i >> 1] = pack_bf16(x, y);
-            } else {  // the sum is that of the weights as they are used: what their rounding does to a row's size cancels
-              const uint32_t w2 = p[i >> 1] = pack_bf16(x, y);
-              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], pack_f32(__uint_as_float(w2 << 16), __uint_as_float(w2 & 0xffff0000u)));
+              e = mul_f32x2(e, pack_f32(vs.x, vs.y));
             }
+            unpack_f32(e, x, y);
+            p[i >> 1] = pack_bf16(x, y);
           }
           tmem_st16(to, p);
         };
@@ -681,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const bool mine = row < used;
       const int my_row = w.row0 + tok, my_head = w.head * group + row - tok * group;
       uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
-      bool finite = true;
+      bool finite = l != 0.f || m == -INFINITY;  // sums of a row are fit to be used
       auto store = [&](uint16_t* at, const float (&o)[16], float inv) {
         uint32_t p[8];
 #pragma unroll
@@ -708,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           }
         }
       } else {
-        // partial sums: [four columns][row][4] and (m, l) of every row, in one of this block's two places
+        // partial sums: [four columns][row][4] and (base, l) of every row, in one of this block's two places
         const long long w0 = w.w0;
         const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.blocks - 1, total, parts);
         auto place = [&](int part) { return part * 2 + (part == first && work_begin(total, part, parts) < w0 ? 1 : 0); };
@@ -725,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
                 for (int j = 0; j < 4; j++) at[j * 128] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
               }
             }
-            if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m, l);
+            if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
           }
         }
         __threadfence();
@@ -756,11 +862,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll 4
             for (int f = sub; f < count; f += share) {
               const float2 ml = __ldcg(at_ml(f, r0));
-              sums += ml.x == -INFINITY ? 0.f : exp2_fast((ml.x - from) * cexp) * ml.y;
+              sums += ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - from) * ml.y;
             }
           }
           for (int o = 1; o < share; o <<= 1) sums += __shfl_xor_sync(0xffffffffu, sums, o);
           if (r0 < used && sub == 0) {
+            if (sums == 0.f && top != -INFINITY) atomicOr(&c.bad_rows[r0 >> 5], 1u << (r0 & 31));
             c.top[0][0][r0] = from;
             c.top[0][1][r0] = sums > 0.f ? 1.f / sums : (sums == 0.f ? 0.f : sums);
           }
@@ -782,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll
               for (int f = 0; f < 4; f++) {
                 if (mf[f] == -INFINITY) continue;  // that part saw no key of this row
-                const float y = exp2_fast((mf[f] - top_r) * cexp);
+                const float y = exp2_fast(mf[f] - top_r);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                   o[4 * j] += y * x[f][j].x; o[4 * j + 1] += y * x[f][j].y; o[4 * j + 2] += y * x[f][j].z; o[4 * j + 3] += y * x[f][j].w;
@@ -828,6 +935,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   }
 }
 
+// A bf16 tensor [outer][heads][D], fetched in boxes of 64 dims by box_heads by box_outer.
+bool encode_heads(CUtensorMap* map, const void* base, uint64_t outer, int heads, int D, int box_heads, int box_outer) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, outer};
+  cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)heads * D * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_outer};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// The same as rows of one head, one to a box (what a gather of four takes).
+bool encode_rows(CUtensorMap* map, const void* base, uint64_t rows, int D) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)D, rows};
+  cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  cuuint32_t box[2] = {64, 1};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int DC, int UNITS, bool I8>
 cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
   constexpr int smem = 1024 + (DC + UNITS) * kUnit + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(RowScratch) + (int)sizeof(Control);
@@ -840,7 +970,14 @@ cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     mark_used_on_device(attr_done);
   }
-  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a);
+  TileMaps m{};
+  const uint64_t slots = (uint64_t)a.v.pages * a.v.page_size;
+  const int group = a.n_q / a.v.n_kv, run = std::max(a.box_rows, 1);
+  if (!encode_heads(&m.q, a.q, a.v.rows, a.n_q, a.v.D, group, a.tokens_per_tile)) return cudaErrorInvalidValue;
+  if (!I8 && (!encode_heads(&m.k, a.k, slots, a.v.n_kv, a.v.D, 1, run) || !encode_heads(&m.v, a.vv, slots, a.v.n_kv, a.v.D, 1, run) ||
+              !encode_rows(&m.k_rows, a.k, slots * a.v.n_kv, a.v.D) || !encode_rows(&m.v_rows, a.vv, slots * a.v.n_kv, a.v.D)))
+    return cudaErrorInvalidValue;
+  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
 }
 
 }  // namespace
@@ -851,6 +988,9 @@ void attn_paged_shape(AttnPagedArgs& a, int sms) {
   a.group_div = page_divisor(group);
   a.max_tiles = a.v.rows / a.tokens_per_tile + std::min(a.v.S, a.v.rows);
   a.grid = sms;
+  a.box_rows = 128;
+  while (a.box_rows > 4 && a.v.page_size % a.box_rows) a.box_rows /= 2;
+  if (a.box_rows < 8) a.box_rows = 0;
 }
 size_t attn_paged_counter_bytes(const AttnPagedArgs& a) { return (size_t)a.v.n_kv * a.max_tiles * 4; }
 size_t attn_paged_partial_bytes(const AttnPagedArgs& a) { return (size_t)a.grid * 2 * (a.v.D + 2) * 128 * 4; }

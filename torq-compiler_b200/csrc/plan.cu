@@ -1064,6 +1064,7 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
       continue;  // refused below
     AttnPagedArgs a{};
     a.n_q = op.i0; a.v.n_kv = op.i1; a.v.rows = tensors[op.in0].shape[0]; a.v.S = tensors[op.in2].shape[0];
+    a.v.page_size = 1;
     attn_paged_shape(a, 1);
     counters_off[i] = cursor;
     cursor += (attn_paged_counter_bytes(a) + 255) & ~(size_t)255;
@@ -2379,6 +2380,9 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         attn_paged_shape(a, current_sm_count());
         scratch_need = std::max(scratch_need, attn_paged_partial_bytes(a));
         const size_t counters = counters_off[i];
+        // a row of one head is fetched by its 32-bit number
+        if ((long long)c.v.rows * n_q > 0x7fffffffll || (long long)c.v.pages * c.v.page_size * c.v.n_kv > 0x7fffffffll)
+          return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged supports 2^31 - 1 rows x heads, of the queries and of the cache", i);
         Loc lq = loc(op.in0), lo = loc(op.out0);
         const PagedLoc at = paged_loc(op, op.in1, op.in2, loc);
         step.kernel_name = "attn_paged";
