@@ -374,6 +374,14 @@ struct ReadPagedArgs {
   uint16_t* v_out;
 };
 cudaError_t launch_kv_read_paged(const ReadPagedArgs& a, cudaStream_t stream);
+// A tile that several blocks of the grid share, as the first of them writes it down: rows row0 .. of the chunk, `used` of them times query heads
+struct AttnJoin {
+  int parts;  // 0: this block begins no such tile
+  int first, second_place, row0, used, head, seq, first_pos;
+};
+// Every block has two places for partial sums: of a tile it goes on with, and of one it begins behind others.
+TB200_BOTH long long attn_part_floats(int D) { return (long long)(D + 2) * 128; }
+TB200_BOTH int attn_part(int block, bool second_place) { return block * 2 + (second_place ? 1 : 0); }
 struct AttnPagedArgs {
   PagedView v;
   const uint16_t* q;  // [rows][n_q * D]
@@ -383,8 +391,8 @@ struct AttnPagedArgs {
   uint16_t* out;      // [rows][n_q * D]
   int n_q, window, sinks, max_new;  // max_new: most rows of a sequence, 0 = any number
   float scale;
-  float* partial;      // attn_paged_partial_bytes: sums of tiles that several blocks share
-  uint32_t* counters;  // attn_paged_counter_bytes, zero before the first launch and left so
+  float* partial;      // sums of tiles that several blocks share, and what to add up (attn_paged_scratch)
+  AttnJoin* joins;
   int* status;
   // filled by attn_paged_shape
   int tokens_per_tile, max_tiles, grid;
@@ -396,8 +404,8 @@ struct AttnPagedArgs {
 };
 constexpr int kTileMinBlocks = 2;  // least key blocks a block of the grid is started for
 void attn_paged_shape(AttnPagedArgs& a, int sms);
-size_t attn_paged_counter_bytes(const AttnPagedArgs& a);
-size_t attn_paged_partial_bytes(const AttnPagedArgs& a);
+size_t attn_paged_scratch_bytes(const AttnPagedArgs& a);
+void attn_paged_scratch(AttnPagedArgs& a, void* at);
 cudaError_t launch_attn_paged(AttnPagedArgs a, cudaStream_t stream);
 cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream);
 

@@ -33,18 +33,19 @@ static_assert(256 * kSoftmaxRegsI8 + 128 * kCopyRegs + 128 * kIssueRegs <= kThre
 static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreads * 128, "register split, bf16");
 constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
-constexpr int kMetaBlocks = 8, kItems = 4;
+constexpr int kMetaBlocks = 8, kItems = 4, kJoinRows = 16, kAhead = 4;
 static_assert(kSoftmaxThreads == kRowThreads, "the plain row is computed by the softmax warps");
 
 struct alignas(16) Meta {
   float k_scale[kKeyBlock], v_scale[kKeyBlock];
-  uint32_t holds[4];  // a bit for each key of the block: it is seen by a row of the tile, and its page holds something
+  int slot[kKeyBlock];  // where the cache holds the key, -1 where no row of the tile sees it or nothing is held
+  uint32_t holds[4];    // the keys with a slot, a bit each
   int key0;
 };
 static_assert(sizeof(Meta) % 16 == 0 && sizeof(RowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
 // A piece of work of a block of the grid: key blocks b0 .. b1 - 1 of a tile of one key/value head.
 struct Item {
-  int seq, head, index;     // index: of the tile among all tiles
+  int seq, head;
   int row0, tokens;         // the tile's rows of the chunk; tokens 0: there is no more work
   int first_pos;            // position of the first token
   int near_key, end_key, sink_blocks, near_block, blocks;  // tile_span
@@ -52,12 +53,12 @@ struct Item {
   long long w0;             // where the tile's work begins
 };
 struct Control {
-  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty, item_full[kItems], item_empty[kItems];
+  uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty, item_full[kItems], item_empty[kItems], meta_full[kMetaBlocks], meta_empty[kMetaBlocks];
   Item items[kItems];
-  uint32_t tmem, bad_rows[4], arrived;
+  uint32_t tmem, bad_rows[4];
   int abort, stop;
   float top[2][2][128];  // row maxima of the two halves, by parity of the block
-  long long totals[kThreads / 32];
+  int totals[kThreads / 32];
   int start_seq, start_tile, start_index, start_off;
 };
 
@@ -93,10 +94,6 @@ struct Keys {
     return page;
   }
   __device__ __forceinline__ bool seen(int key) const { return key < end_key && (key >= near_key || key < sinks); }  // by a token of the tile
-  __device__ __forceinline__ int count_seen(int key, int n) const {  // of keys key .. key + n - 1
-    const int upto = min(key + n, end_key), firsts = max(0, min(min(upto, sinks), near_key) - key);
-    return firsts + max(0, upto - max(key, near_key));
-  }
   __device__ __forceinline__ int slot(int key, int page) const {
     const bool there = seen(key) && page >= 0 && page < pages;
     return there ? page * page_size + (key - page_of(key, div) * page_size) : -1;
@@ -104,26 +101,20 @@ struct Keys {
 };
 
 // Running sum over the block's threads up to and including this one, and the sum of all, through c.totals.
-__device__ long long block_scan(Control& c, long long x, long long& all) {
+__device__ __noinline__ int block_scan(Control& c, int x, int& all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long v = x;
+  int v = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
   __syncthreads();
   if (lane == 31) c.totals[warp] = v;
   __syncthreads();
-  long long before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; w++) {
-    const long long y = c.totals[w];
-    before += w < warp ? y : 0;
-    all += y;
-  }
-  return before + v;
+  const int y = lane < kThreads / 32 ? c.totals[lane] : 0;
+  all = __reduce_add_sync(0xffffffffu, y);
+  return v + __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -158,15 +149,35 @@ __device__ __forceinline__ float max3(float a, float b, float d) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(d));
   return r;
 }
-// four int8 -> four bf16, exact: 0x4300 | low seven bits of the biased byte is 128 + those bits, and 128 or 256 comes off again
+// four int8 -> four bf16, exact: 0x4300 | the low seven bits is 128 + those bits, and 128 comes off again, or 256 where the byte is negative
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t u = w ^ 0x80808080u, low = u & 0x7f7f7f7fu, off = ~u & 0x80808080u;
+  const uint32_t low = w & 0x7f7f7f7fu, off = w & 0x80808080u;
   const uint32_t a0 = __byte_perm(low, 0x43434343u, 0x4140), a1 = __byte_perm(low, 0x43434343u, 0x4342);
   const uint32_t c0 = __byte_perm(off, 0x43434343u, 0x4140), c1 = __byte_perm(off, 0x43434343u, 0x4342);
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a0), "r"(c0));
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(a1), "r"(c1));
 }
+__device__ __forceinline__ bool pair_any(int id, bool x) {  // of 64 threads
+  int r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, 64, p;\n\t"
+      "selp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((int)x)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {  // zeros when not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -183,7 +194,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   // [Q units][ring units] on 1024-byte boundaries, then the rest
   unsigned char* const base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t q_smem = smem_u32(base), ring = q_smem + DC * kUnit;
-  Meta* const meta = reinterpret_cast<Meta*>(base + (DC + UNITS) * kUnit);
+  unsigned char* const raw = base + (DC + UNITS) * kUnit;  // int8 pieces on their way
+  Meta* const meta = reinterpret_cast<Meta*>(raw + (I8 ? kAhead * kUnit / 2 : 0));
   RowScratch& plain = *reinterpret_cast<RowScratch*>(meta + kMetaBlocks);
   Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(RowScratch));
   int* const first_tile = reinterpret_cast<int*>(base);  // while the work is shared out: tiles in front of each sequence
@@ -208,7 +220,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     mbar_init(smem_u32(&c.o_done), 1);
     for (int i = 0; i < kItems; i++) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + 64 + (I8 ? kCopyThreads : 0));
+      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + 96 + (I8 ? kCopyThreads : 0));
+    }
+    for (int i = 0; i < kMetaBlocks; i++) {
+      mbar_init(smem_u32(&c.meta_full[i]), 1);
+      mbar_init(smem_u32(&c.meta_empty[i]), 1);
     }
     mbar_init(smem_u32(&c.q_full), 1);
     mbar_init(smem_u32(&c.q_empty), 1);
@@ -220,82 +236,70 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   grid_dependency_release();
 
   // ---- the work: tiles of the sequences, key blocks of the tiles ----
-  long long all = 0;
-  int run = 0;
+  int all = 0, run = 0;
   for (int s0 = 0; s0 < v.S; s0 += kThreads) {
-    const int s = s0 + tid;
-    const int upto = run + (int)block_scan(c, s < v.S ? tiles_of(a, span_of(a, s)) : 0, all);
+    const int s = s0 + tid, upto = run + block_scan(c, s < v.S ? tiles_of(a, span_of(a, s)) : 0, all);
     if (s < v.S) first_tile[s + 1] = upto;
-    run += (int)all;
+    run += all;
   }
-  if (tid == 0) first_tile[0] = 0;
+  if (tid == 0) {
+    first_tile[0] = 0;
+    a.joins[blockIdx.x].parts = 0;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = c.tmem;
   const int n_tiles = min(run, a.max_tiles);
-  auto blocks_of = [&](int i, int& seq, int& tile) {
+  int seq0 = 0, tile0 = 0;
+  auto blocks_of = [&](int i) {
     int lo = 0, hi = v.S - 1;  // the last sequence with first_tile[seq] <= i
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (first_tile[mid] <= i) lo = mid;
       else hi = mid - 1;
     }
-    seq = lo;
-    tile = i - first_tile[lo];
-    const Span sp = span_of(a, seq);
-    return tile_span(sp.ctx, sp.n, tile, tpt, a.window, a.sinks, v.capacity).blocks;
+    seq0 = lo;
+    tile0 = i - first_tile[lo];
+    const Span sp = span_of(a, seq0);
+    return tile_span(sp.ctx, sp.n, tile0, tpt, a.window, a.sinks, v.capacity).blocks;
   };
-  int seq0 = 0, tile0 = 0, n0 = tid < n_tiles ? blocks_of(tid, seq0, tile0) : 0;
-  long long upto0 = block_scan(c, n0, all), per_head = all;
-  if (n_tiles > kThreads) {
-    long long mine = 0;
-    for (int i = tid + kThreads; i < n_tiles; i += kThreads) mine += blocks_of(i, seq0, tile0);
-    block_scan(c, mine, all);
+  int per_head = 0;  // the planner refuses what 32 bits do not hold
+  for (int i0 = 0; i0 < n_tiles; i0 += kThreads) {
+    block_scan(c, i0 + tid < n_tiles ? blocks_of(i0 + tid) : 0, all);
     per_head += all;
   }
-  const long long total = per_head * v.n_kv;
+  const long long total = (long long)per_head * v.n_kv;
   const int parts = (int)max(1ll, min((long long)gridDim.x, total / kTileMinBlocks));
   const bool works = total > 0 && (int)blockIdx.x < parts;
   const long long begin = works ? work_begin(total, blockIdx.x, parts) : 0, end = works ? work_begin(total, blockIdx.x + 1, parts) : 0;
-  if (works) {
-    const long long rem = begin % per_head;
-    long long before = 0;
-    for (int i0 = 0; i0 < n_tiles && before <= rem; i0 += kThreads) {
-      const int i = i0 + tid;
-      if (n_tiles > kThreads) {
-        n0 = i < n_tiles ? blocks_of(i, seq0, tile0) : 0;
-        upto0 = block_scan(c, n0, all);
-      }
-      const long long upto = before + upto0;
-      if (n0 && upto > rem && upto - n0 <= rem) {
-        c.start_tile = tile0;
-        c.start_seq = seq0;
-        c.start_index = i;
-        c.start_off = (int)(rem - (upto - n0));
-      }
-      before += n_tiles > kThreads ? all : per_head;
+  const int head0 = works ? (int)(begin / per_head) : 0, rem = (int)(begin - (long long)head0 * per_head);
+  for (int i0 = 0, before = 0; works && i0 < n_tiles && before <= rem; i0 += kThreads) {
+    const int i = i0 + tid, n = i < n_tiles ? blocks_of(i) : 0, upto = before + block_scan(c, n, all);
+    if (n && upto > rem && upto - n <= rem) {
+      c.start_tile = tile0;
+      c.start_seq = seq0;
+      c.start_index = i;
+      c.start_off = rem - (upto - n);
     }
+    before += all;
   }
   __syncthreads();  // the start is known, and first_tile's room is free
 
+  // One wait that runs out ends all others at once: every role then runs through without waiting, and the results are not used. (Kept short: it
+  // stands in many places, and what bounds this kernel next to its copies is how many instructions its roles have in the cache.)
   bool gave_up = false;
   auto wait = [&](uint64_t& bar, uint32_t parity, int code) {
-    // one wait that ran out ends all others at once: every role then runs through without waiting, and the results are not used
-    if (gave_up) return;
     const uint32_t at = smem_u32(&bar);
-    if (mbar_poll(at, parity, 256)) return;
+    if (mbar_poll(at, parity, 16) || gave_up) return;
     const unsigned long long t0 = globaltimer_ns();
-    for (;;) {
-      if (mbar_poll(at, parity, 256)) return;
-      if (*(volatile int*)&c.abort) break;
-      if (globaltimer_ns() - t0 > a.wait_ns) {
-        report_expired_wait(a.status, code);
-        *(volatile int*)&c.abort = 1;
-        break;
+    while (!mbar_poll(at, parity, 64)) {
+      if (globaltimer_ns() - t0 > a.wait_ns) *(volatile int*)&c.abort = code;
+      if (*(volatile int*)&c.abort) {
+        gave_up = true;
+        return;
       }
     }
-    gave_up = true;
   };
 
   // The roles take the block's items from a ring that a warp of its own fills. The reference stays valid until release_item.
@@ -303,126 +307,69 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     wait(c.item_full[i % kItems], (i / kItems) & 1, 310);
     return c.items[i % kItems];
   };
+  auto take_meta = [&](uint32_t block) -> const Meta& {  // it stays until the block's values have been multiplied
+    wait(c.meta_full[block % kMetaBlocks], (block / kMetaBlocks) & 1, 312);
+    return meta[block % kMetaBlocks];
+  };
   auto release_item = [&](uint32_t i) { mbar_arrive(smem_u32(&c.item_empty[i % kItems])); };
   const uint32_t o_tmem = tmem + 256;
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ copies of int8 caches: widened on the way
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(I8 ? kCopyRegs : kIssueRegs));
     if (I8 && works) {
-    const int t = tid - kSoftmaxThreads;
-    uint32_t unit = 0, blocks = 0;
-    constexpr int kRows = 4, kPieces = 4, kRowStep = kCopyThreads / kPieces;  // pieces of 16 bytes: a thread has the same one of four rows
-    const int piece = t % kPieces, row0 = t / kPieces;
+    // A thread has the same piece of 16 bytes of four rows of every unit: what it asks for lands in room of its own, kAhead units ahead of being
+    // widened, so nothing but its own copies has to be waited for.
+    const int t = tid - kSoftmaxThreads, piece = t & 3, row0 = t >> 2;
+    const uint32_t own = smem_u32(raw) + t * 64;
     const long long row_bytes = (long long)v.n_kv * D;
+    uint32_t unit = 0, block0 = 0;
     for (uint32_t items = 0;; items++) {
       const Item& w = take_item(items);
       if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
-      const int b0 = w.b0, b1 = w.b1, head = w.head;
-      const Keys keys_of(a, w);
+      const int n = w.b1 - w.b0, units = 2 * DC * n;
+      const long long head_bytes = (long long)w.head * D + piece * 16;
       release_item(items);
-      int next_page[kRows], next_own;
-      auto ask_block = [&](int b) {
-        const int key0 = keys_of.first(b);
+      auto ask = [&](int i) {  // unit i of the item: the keys of block 0, then those of block b and the values of b - 1, by turns
+        if (i < units) {
+          const int j = i - DC + 2 * DC, b = j / (2 * DC), r = j - b * 2 * DC;
+          const bool keys = r >= DC ? b == 0 : b < n;  // (j is such that b = 0 begins with the keys of block 0 at r = DC)
+          const int block = keys ? b : b - 1, u = r >= DC ? r - DC : r;
+          const Meta& m = take_meta(block0 + block);
+          const char* const pages = (const char*)(keys ? a.k : a.vv) + head_bytes + u * 64;
+          const bool in = u * 64 + piece * 16 < D;
 #pragma unroll
-        for (int i = 0; i < kRows; i++) next_page[i] = keys_of.ask(key0 + row0 + kRowStep * i);
-        next_own = keys_of.ask(key0 + t);
+          for (int k = 0; k < 4; k++) {
+            const int slot = m.slot[row0 + 32 * k];
+            const bool ok = in && slot >= 0;
+            copy16(own + (i % kAhead) * (kUnit / 2) + k * 16, pages + (ok ? slot * row_bytes : 0), ok);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      // where this thread's pieces of the keys and of the values of a block start, in bytes behind the cache; negative: zeros
-      long long key_at[kRows], val_at[kRows];
-      int own = 0;
-      float own_k = 0.f, own_v = 0.f;
-      auto turn = [&](int b) {  // the block that was asked for becomes the one to copy
-        const int key0 = keys_of.first(b);
+#pragma unroll 1
+      for (int i = 0; i < kAhead; i++) ask(i);
+#pragma unroll 1
+      for (int i = 0; i < units; i++, unit++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
+        const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128, from = own + (i % kAhead) * (kUnit / 2);
+        const uint32_t lo_at = ((2 * piece) ^ (row0 & 7)) << 4, hi_at = ((2 * piece + 1) ^ (row0 & 7)) << 4;  // a thread's rows are 32 apart
 #pragma unroll
-        for (int i = 0; i < kRows; i++) {
-          const int slot = keys_of.slot(key0 + row0 + kRowStep * i, next_page[i]);
-          val_at[i] = key_at[i];
-          key_at[i] = slot < 0 ? -1 : slot * row_bytes + ((long long)head * D + piece * 16);
+        for (int k = 0; k < 4; k++) {
+          const uint4 q = lds128(from + k * 16);
+          uint4 lo, hi;
+          widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
+          widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
+          sts128(dst + k * 4096 + lo_at, lo);
+          sts128(dst + k * 4096 + hi_at, hi);
         }
-        own = keys_of.slot(key0 + t, next_own);
-        const float* sc = a.scales + (long long)max(own, 0) * 2 * v.n_kv + head;
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_k) : "l"(sc));
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(own_v) : "l"(sc + v.n_kv));
-      };
-      // groups of up to two units go through registers, the next group asked for before one is widened
-      constexpr int G = DC > 1 ? 2 : 1;
-      uint4 x[G][kRows], y[G][kRows];
-      auto load = [&](uint4 (&to)[G][kRows], const void* pages, const long long (&at)[kRows], int u0) {
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          if (u0 + g >= DC) continue;
-          const bool in = u0 + g + 1 < DC || (u0 + g) * 64 + piece * 16 < D;
-#pragma unroll
-          for (int i = 0; i < kRows; i++) {
-            to[g][i] = make_uint4(0, 0, 0, 0);
-            if (in && at[i] >= 0)
-              asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(to[g][i].x), "=r"(to[g][i].y), "=r"(to[g][i].z), "=r"(to[g][i].w)
-                           : "l"((const char*)pages + at[i] + (u0 + g) * 64));
-          }
-        }
-      };
-      auto store = [&](const uint4 (&from)[G][kRows], int u0) {
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          if (u0 + g >= DC) continue;
-          if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
-          const uint32_t dst = ring + (unit % UNITS) * kUnit;
-#pragma unroll
-          for (int i = 0; i < kRows; i++) {
-            const int r = row0 + kRowStep * i;
-            const uint4 q = from[g][i];
-            uint4 lo, hi;
-            widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
-            widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
-            sts128(dst + r * 128 + (((2 * piece) ^ (r & 7)) << 4), lo);
-            sts128(dst + r * 128 + (((2 * piece + 1) ^ (r & 7)) << 4), hi);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          mbar_arrive(smem_u32(&c.full[unit % UNITS]));
-          unit++;
-        }
-      };
-      ask_block(b0);
-      turn(b0);
-      load(x, a.k, key_at, 0);
-      for (int b = b0; b <= b1; b++) {
-        const bool keys = b < b1, values = b > b0, more = b + 1 < b1;
-        if (more) ask_block(b + 1);
-        if (keys) {  // what this block's keys are, by one thread a key
-          Meta& m = meta[blocks % kMetaBlocks];
-          blocks++;
-          const uint32_t bits = __ballot_sync(0xffffffffu, own >= 0);
-          if (lane == 0) m.holds[t >> 5] = bits;
-          if (t == 0) m.key0 = keys_of.first(b);
-          m.k_scale[t] = own >= 0 ? own_k : 0.f;
-          m.v_scale[t] = own >= 0 ? own_v : 0.f;
-        }
-        if (DC <= 2) {
-          if (values) load(y, a.vv, val_at, 0);
-          if (keys) {
-            store(x, 0);
-            turn(more ? b + 1 : b);
-          }
-          if (more) load(x, a.k, key_at, 0);
-          if (values) store(y, 0);
-        } else {
-          if (keys) {
-            load(y, a.k, key_at, 2);
-            store(x, 0);
-          }
-          if (values) load(x, a.vv, val_at, 0);
-          if (keys) store(y, 2);
-          if (values) {
-            load(y, a.vv, val_at, 2);
-            store(x, 0);
-          }
-          if (keys) turn(more ? b + 1 : b);
-          if (more) load(x, a.k, key_at, 0);
-          if (values) store(y, 2);
-        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&c.full[unit % UNITS]));
+        ask(i + kAhead);
       }
+      block0 += n;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else if (warp >= kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ matrix instructions
@@ -441,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       for (int b = 0; b <= n; b++) {
         if (b < n) {  // scores of block b
           const uint32_t s_tmem = tmem + ((blocks + b) & 1) * 128;
-#pragma unroll
+#pragma unroll 1
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
             tc_fence_after();
@@ -458,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           const uint32_t g = blocks + b - 1, p_tmem = tmem + (g & 1) * 128;
           wait(c.p_ready[g & 1], (g >> 1) & 1, 305);
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 306);
             tc_fence_after();
@@ -472,6 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
             unit++;
           }
           mma_commit_elect(smem_u32(&c.pv_done));
+          mma_commit_elect(smem_u32(&c.meta_empty[g % kMetaBlocks]));
           if (b == n) mma_commit_elect(smem_u32(&c.o_done));
         }
       }
@@ -483,14 +431,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       for (uint32_t items = 0;; items++) {
         const Item& w = take_item(items);
         if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
-        const int b0 = w.b0, b1 = w.b1, head = w.head, q_row = w.row0;
-        const Keys keys_of(a, w);
+        const int n = w.b1 - w.b0, head = w.head, q_row = w.row0;
         release_item(items);
         if (items) wait(c.q_empty, (items - 1) & 1, 302);
         __syncwarp();
         if (lane == 0) {  // rows of the tile's tokens, in the tile's order; those behind the last token are somebody's or nobody's, and are not used
           const uint32_t bar = smem_u32(&c.q_full);
           mbar_expect_tx(bar, DC * 128 * tpt * group);
+#pragma unroll 1
           for (int u = 0; u < DC; u++) tma_load_3d(q_smem + u * kUnit, &maps.q, u * 64, head * group, q_row, bar);
         }
         if (I8) continue;
@@ -503,102 +451,106 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           unit++;
           return slot;
         };
-        auto tell = [&](int key0, uint32_t held) {  // the block's keys, before its first unit
-          Meta& m = meta[blocks % kMetaBlocks];
+        // A run of R = box_rows keys to a lane: one box where all have a slot (they then follow one another) or none has (from outside the
+        // cache: zeros). Runs with some, and all keys where pages end anywhere (no box), go four keys to a lane.
+        const int R = a.box_rows ? a.box_rows : kKeyBlock, runs = a.box_rows ? kKeyBlock >> (31 - __clz(R)) : 0, none = v.pages * v.page_size;
+        auto copy_units = [&](const CUtensorMap* map, const CUtensorMap* rows, uint32_t block) {
+          const Meta& m = meta[block % kMetaBlocks];
+          const int at = min(lane * R, kKeyBlock - 1);
+          const int4 keys = *reinterpret_cast<const int4*>(&m.slot[4 * lane]);  // this lane's four, by themselves
+          // how many of this lane's run have a slot: whole words of the bits, or a part of one
+          bool all_held = true, any_held = false;
+          if (R >= 32) {
+            for (int i = 0; i < R; i += 32) {
+              const uint32_t word = m.holds[min((at + i) >> 5, 3)];
+              all_held = all_held && word == 0xffffffffu;
+              any_held = any_held || word;
+            }
+          } else {
+            const uint32_t mask = (1u << R) - 1, word = m.holds[at >> 5] >> (at & 31) & mask;
+            all_held = word == mask;
+            any_held = word != 0;
+          }
+          const bool in_part = runs ? any_held && !all_held : true;
+          const uint32_t parts = runs ? __ballot_sync(0xffffffffu, lane < runs && in_part) : 0xffffffffu;
+          const int run = all_held ? m.slot[at] : none;
+          const bool one_box = lane < runs && !in_part, four = runs ? parts >> (4 * lane >> (31 - __clz(R))) & 1 : true;
+          int r[4] = {keys.x, keys.y, keys.z, keys.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) r[i] = r[i] < 0 ? -1 : r[i] * v.n_kv + head;
+#pragma unroll 1
+          for (int u = 0; u < DC; u++) {
+            const uint32_t slot = begin_unit(), bar = smem_u32(&c.full[slot]), dst = ring + slot * kUnit;
+            if (one_box) tma_load_3d(dst + lane * R * 128, map, u * 64, head, run, bar);
+            if (four) tma_gather4(dst + lane * 512, rows, u * 64, r[0], r[1], r[2], r[3], bar);
+          }
+        };
+        for (int b = 0; b <= n; b++) {
+          if (b < n) {
+            take_meta(blocks);
+            __syncwarp();
+            copy_units(&maps.k, &maps.k_rows, blocks);
+          }
+          if (b > 0) copy_units(&maps.v, &maps.v_rows, blocks - 1);
           blocks++;
+        }
+        blocks--;
+      }
+    } else if (works && warp == kSoftmaxWarps + kCopyWarps + 3) {
+      // ---------------------------------------------- which keys, and where: four to a lane, a block's page ids asked for a block ahead
+      uint32_t blocks = 0;
+      for (uint32_t items = 0;; items++) {
+        const Item& w = take_item(items);
+        if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
+        const int b0 = w.b0, b1 = w.b1, head = w.head;
+        const Keys keys_of(a, w);
+        release_item(items);
+        int next_page[4];
+        auto ask_block = [&](int b) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) next_page[i] = keys_of.ask(keys_of.first(b) + 4 * lane + i);
+        };
+        ask_block(b0);
+        for (int b = b0; b < b1; b++, blocks++) {
+          const int key0 = keys_of.first(b);
+          int slot[4];
+          uint32_t held = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            slot[i] = keys_of.slot(key0 + 4 * lane + i, next_page[i]);
+            held |= (slot[i] >= 0 ? 1u : 0u) << (4 * (lane & 7) + i);
+          }
+          if (b + 1 < b1) ask_block(b + 1);
+          float ks[4] = {}, vs[4] = {};
+          if (I8) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float* sc = a.scales + (long long)max(slot[i], 0) * 2 * v.n_kv + head;
+              const float k1 = __ldg(sc), v1 = __ldg(sc + v.n_kv);
+              ks[i] = slot[i] < 0 ? 0.f : k1;
+              vs[i] = slot[i] < 0 ? 0.f : v1;
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) held |= __shfl_xor_sync(0xffffffffu, held, o);
+          const uint32_t at = blocks % kMetaBlocks;
+          if (blocks >= kMetaBlocks) wait(c.meta_empty[at], (blocks / kMetaBlocks - 1) & 1, 313);
+          Meta& m = meta[at];
+          *reinterpret_cast<int4*>(&m.slot[4 * lane]) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+          if (I8) {
+            *reinterpret_cast<float4*>(&m.k_scale[4 * lane]) = make_float4(ks[0], ks[1], ks[2], ks[3]);
+            *reinterpret_cast<float4*>(&m.v_scale[4 * lane]) = make_float4(vs[0], vs[1], vs[2], vs[3]);
+          }
           if ((lane & 7) == 0) m.holds[lane >> 3] = held;
           if (lane == 0) m.key0 = key0;
           __syncwarp();
-        };
-        auto gather_bits = [&](uint32_t nibble) {  // four keys a lane -> the 32 of its eight lanes
-          uint32_t held = nibble << (4 * (lane & 7));
-          held |= __shfl_xor_sync(0xffffffffu, held, 1);
-          held |= __shfl_xor_sync(0xffffffffu, held, 2);
-          return held | __shfl_xor_sync(0xffffffffu, held, 4);
-        };
-        // four keys to a lane: where pages end anywhere, and for runs of keys that are seen in part
-        auto gather = [&](const CUtensorMap* map, uint32_t slot, int u, int first, const int (&r)[4]) {
-          tma_gather4(ring + slot * kUnit + first * 128, map, u * 64, r[0], r[1], r[2], r[3], smem_u32(&c.full[slot]));
-        };
-        if (!a.box_rows) {
-          int next_page[4], key_row[4], val_row[4] = {};
-          auto ask_block = [&](int b) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) next_page[i] = keys_of.ask(keys_of.first(b) + 4 * lane + i);
-          };
-          ask_block(b0);
-          for (int b = b0; b <= b1; b++) {
-            if (b < b1) {
-              const int key0 = keys_of.first(b);
-              uint32_t nibble = 0;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const int slot = keys_of.slot(key0 + 4 * lane + i, next_page[i]);
-                key_row[i] = slot < 0 ? -1 : slot * v.n_kv + head;
-                nibble |= (slot >= 0 ? 1u : 0u) << i;
-              }
-              if (b + 1 < b1) ask_block(b + 1);
-              tell(key0, gather_bits(nibble));
-              for (int u = 0; u < DC; u++) gather(&maps.k_rows, begin_unit(), u, 4 * lane, key_row);
-            }
-            if (b > b0)
-              for (int u = 0; u < DC; u++) gather(&maps.v_rows, begin_unit(), u, 4 * lane, val_row);
-#pragma unroll
-            for (int i = 0; i < 4; i++) val_row[i] = key_row[i];
-          }
-        } else {
-          // a run of box_rows keys to a lane: one box where all are seen (or none: from outside the cache, zeros), else four by four
-          const int R = a.box_rows, runs = kKeyBlock / R, none = v.pages * v.page_size;
-          int next_page, key_run = 0, val_run = 0;  // slot of a run's first key, or `none`
-          uint32_t key_parts = 0, val_parts = 0;    // runs that are seen in part
-          int key_first = 0, val_first = 0;
-          auto copy_units = [&](const CUtensorMap* map, const CUtensorMap* rows, int run, uint32_t parts, int key0) {
-            for (int u = 0; u < DC; u++) {
-              const uint32_t slot = begin_unit();
-              if (lane < runs && !(parts >> lane & 1)) tma_load_3d(ring + slot * kUnit + lane * R * 128, map, u * 64, head, run, smem_u32(&c.full[slot]));
-              for (uint32_t left = parts; left; left &= left - 1) {
-                const int g = __ffs(left) - 1, from = __shfl_sync(0xffffffffu, run, g);
-                if (4 * lane < R) {
-                  int r[4];
-#pragma unroll
-                  for (int i = 0; i < 4; i++) r[i] = keys_of.seen(key0 + g * R + 4 * lane + i) ? (from + 4 * lane + i) * v.n_kv + head : -1;
-                  gather(rows, slot, u, g * R + 4 * lane, r);
-                }
-              }
-            }
-          };
-          auto ask_block = [&](int b) { next_page = keys_of.ask(min(keys_of.first(b) + lane * R, keys_of.last)); };
-          ask_block(b0);
-          for (int b = b0; b <= b1; b++) {
-            if (b < b1) {
-              const int key0 = key_first = keys_of.first(b), mine = key0 + min(lane, runs - 1) * R;
-              // the run of this lane, then the four keys of this lane
-              const bool held = next_page >= 0 && next_page < v.pages && mine <= keys_of.last;
-              const int seen = held ? keys_of.count_seen(mine, R) : 0;
-              key_run = seen ? next_page * v.page_size + (mine - page_of(mine, v.div) * v.page_size) : none;
-              key_parts = __ballot_sync(0xffffffffu, lane < runs && seen > 0 && seen < R);
-              const uint32_t any = __ballot_sync(0xffffffffu, seen > 0);
-              if (b + 1 < b1) ask_block(b + 1);
-              uint32_t nibble = 0;
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const int k = 4 * lane + i;
-                nibble |= ((any >> (k / R) & 1) && keys_of.seen(key0 + k) ? 1u : 0u) << i;
-              }
-              tell(key0, gather_bits(nibble));
-              copy_units(&maps.k, &maps.k_rows, key_run, key_parts, key0);
-            }
-            if (b > b0) copy_units(&maps.v, &maps.v_rows, val_run, val_parts, val_first);
-            val_run = key_run;
-            val_parts = key_parts;
-            val_first = key_first;
-          }
+          if (lane == 0) mbar_arrive(smem_u32(&c.meta_full[at]));
         }
       }
     } else if (works && warp == kSoftmaxWarps + kCopyWarps + 1 && lane == 0) {
       // ---------------------------------------------- the block's items
       long long cur = begin;
-      int head = (int)(begin / per_head), seq = c.start_seq, tile = c.start_tile, index = c.start_index, off = c.start_off;
+      int head = head0, seq = c.start_seq, tile = c.start_tile, index = c.start_index, off = c.start_off;
       Span span = span_of(a, seq);
       int tiles = tiles_of(a, span);
       for (uint32_t i = 0;; i++) {
@@ -612,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         }
         const TileSpan ts = tile_span(span.ctx, span.n, tile, tpt, a.window, a.sinks, v.capacity);
         const int b1 = (int)min((long long)ts.blocks, off + (end - cur));
-        w.seq = seq; w.head = head; w.index = index;
+        w.seq = seq; w.head = head;
         w.row0 = span.row0 + tile * tpt;
         w.tokens = min(tpt, span.n - tile * tpt);
         w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
@@ -646,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     // ------------------------------------------------ softmax: thread = (row, half of the block's keys)
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int tok = page_of(row, a.group_div), pieces = D >> 4;
+    const int tok = page_of(row, a.group_div);
     const float cexp = a.scale * 1.4426950408889634f;
     uint32_t blocks = 0, items = 0;
     for (;; items++) {
@@ -672,107 +624,113 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         }
         wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
         tc_fence_after();
-        uint32_t s0[32], s1[32];
-        tmem_ld32_issue(s_tmem, s0);
-        tmem_ld32_issue(s_tmem + 32, s1);
-        const Meta& mt = meta[blocks % kMetaBlocks];
+        const Meta& mt = take_meta(blocks);
         const int key0 = mt.key0 + half * 64;
-        const uint32_t holds0 = mt.holds[half * 2], holds1 = mt.holds[half * 2 + 1];
-        const bool partial = (holds0 & holds1) != 0xffffffffu || key0 + 63 > first_pos ||
+        // whether some row of the tile does not see some key of this half
+        const bool partial = (mt.holds[half * 2] & mt.holds[half * 2 + 1]) != 0xffffffffu || key0 + 63 > first_pos ||
                              (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
-        tmem_ld_wait32(s0);
-        tmem_ld_wait32(s1);
-        if (I8) {
-          auto scaled = [&](uint32_t (&s)[32], const float* k_scale) {
+        // 32 scores, of columns 32 k on: scaled (int8), and those of keys this row does not see at -inf. The loops over them stay rolled up: a
+        // processor's four quarters each run this beside other roles, and what does not fit their instruction buffers is waited for.
+        auto scores = [&](int k, uint32_t (&s)[32]) {
+          tmem_ld32_issue(s_tmem + 32 * k, s);
+          tmem_ld_wait32(s);
+          if (I8) {
+            const float* scale = mt.k_scale + half * 64 + 32 * k;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(k_scale + i);
+              const float4 x = *reinterpret_cast<const float4*>(scale + i);
               float f[4];
               unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), pack_f32(x.x, x.y)), f[0], f[1]);
               unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), pack_f32(x.z, x.w)), f[2], f[3]);
 #pragma unroll
               for (int j = 0; j < 4; j++) s[i + j] = __float_as_uint(f[j]);
             }
-          };
-          scaled(s0, mt.k_scale + half * 64);
-          scaled(s1, mt.k_scale + half * 64 + 32);
-        }
-        if (partial) {
-          // bits of the keys this row sees: not behind its position, inside the window or among the first, and held
-          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
-          const uint32_t see0 = below(pos - key0 + 1) & (~below(near - key0) | below(a.sinks - key0)) & holds0;
-          const uint32_t see1 = below(pos - key0 - 31) & (~below(near - key0 - 32) | below(a.sinks - key0 - 32)) & holds1;
-          const uint32_t none = __float_as_uint(-INFINITY);
-#pragma unroll
-          for (int i = 0; i < 32; i++) {
-            s0[i] = see0 >> i & 1 ? s0[i] : none;
-            s1[i] = see1 >> i & 1 ? s1[i] : none;
           }
-        }
-        float tops[4] = {__uint_as_float(s0[0]), __uint_as_float(s0[1]), __uint_as_float(s1[0]), __uint_as_float(s1[1])};
+          if (partial) {
+            // bits of the keys this row sees: not behind its position, inside the window or among the first, and held
+            auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
+            const int k0 = key0 + 32 * k;
+            const uint32_t see = below(pos - k0 + 1) & (~below(near - k0) | below(a.sinks - k0)) & mt.holds[half * 2 + k];
 #pragma unroll
-        for (int i = 2; i < 32; i += 2) {
-          tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
-          tops[2 + (i >> 1 & 1)] = max3(tops[2 + (i >> 1 & 1)], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
-        }
-        float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-        c.top[blocks & 1][half][row] = top;
-        named_sync(1 + (warp & 3), 64);
-        top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
-        // follow the maximum when p could grow beyond 2^8, or when there was none yet
-        const bool grows = row < used && top > m && !((top - m) * cexp <= 8.f);
-        if (b == 0) {
-          m = top;
-          base = m == -INFINITY ? 0.f : m * cexp;
-        } else if (__any_sync(0xffffffffu, grows)) {
-          float keep = 1.f;
-          if (grows) {
-            const float to = top * cexp;
-            keep = m == -INFINITY ? 0.f : exp2_fast(base - to);
-            m = top;
-            base = to;
+            for (int i = 0; i < 32; i++) s[i] = see >> i & 1 ? s[i] : 0xff800000u;
           }
-          sum *= keep;
-          // these scores were issued behind the sums of the block before the last: its phase is over, the last one's is waited for
-          wait(c.pv_done, (blocks - 1) & 1, 308);
-          tc_fence_after();
-          for (int i = half; i < pieces; i += 2) {
-            uint32_t o[16];
-            tmem_ld16(o_tmem + lanes + i * 16, o);
-#pragma unroll
-            for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-            tmem_st16(o_tmem + lanes + i * 16, o);
-          }
-          tmem_st_wait();
-        }
-        // p = 2^(s c - base) in one multiply-add: how base was rounded is the same for every key of the row, so it cancels (where that factor
-        // itself leaves fp32, at scores beyond 10^9, sums come out infinite or zero, which is caught at the end)
-        const unsigned long long scale2 = pack_f32(cexp, cexp), base2 = pack_f32(-base, -base);
-        unsigned long long parts2[2] = {0ull, 0ull};  // two pairs of running sums
-        auto weights = [&](const uint32_t (&s)[32], const float* v_scale, uint32_t to) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x, y;
-            unpack_f32(fma_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, base2), x, y);
-            unsigned long long e = pack_f32(exp2_fast(x), exp2_fast(y));
-            parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], e);
-            if (I8) {
-              const float2 vs = *reinterpret_cast<const float2*>(v_scale + i);
-              e = mul_f32x2(e, pack_f32(vs.x, vs.y));
-            }
-            unpack_f32(e, x, y);
-            p[i >> 1] = pack_bf16(x, y);
-          }
-          tmem_st16(to, p);
         };
-        weights(s0, mt.v_scale + half * 64, s_tmem);
-        weights(s1, mt.v_scale + half * 64 + 32, s_tmem + 16);
-        {
-          float x, y;
-          unpack_f32(add_f32x2(parts2[0], parts2[1]), x, y);
-          sum += x + y;
+        float part;
+        uint32_t p[32];  // two weights each; they take the place of the scores once these are not needed again
+        for (bool follow = b == 0;;) {
+          if (follow) {  // the row's maximum so far; m follows it where p would grow beyond 2^8, or had none yet
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int k = 0; k < 2; k++) {
+              uint32_t s[32];
+              scores(k, s);
+              float tops[2] = {top, -INFINITY};
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+              top = fmaxf(tops[0], tops[1]);
+            }
+            c.top[blocks & 1][half][row] = top;
+            named_sync(1 + (warp & 3), 64);
+            top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
+            float keep = 1.f;
+            if (top > m && (b == 0 || !((top - m) * cexp <= 8.f))) {
+              const float to = top * cexp;
+              keep = m == -INFINITY ? 0.f : exp2_fast(base - to);
+              m = top;
+              base = to;
+            }
+            if (b > 0) {
+              sum *= keep;
+              // these scores were issued behind the sums of the block before the last: its phase is over, the last one's is waited for
+              wait(c.pv_done, (blocks - 1) & 1, 308);
+              tc_fence_after();
+#pragma unroll 1
+              for (int i = 32 * half; i < D; i += 64) {  // columns behind D belong to nobody
+                uint32_t o[32];
+                tmem_ld32_issue(o_tmem + lanes + i, o);
+                tmem_ld_wait32(o);
+#pragma unroll
+                for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                tmem_st32(o_tmem + lanes + i, o);
+              }
+            }
+          }
+          // p = 2^(s c - base) in one multiply-add: how base was rounded is the same for every key of the row, so it cancels (where that factor
+          // itself leaves fp32, at scores beyond 10^9, sums come out infinite or zero, which is caught at the end)
+          const unsigned long long scale2 = pack_f32(cexp, cexp), base2 = pack_f32(-base, -base);
+          unsigned long long parts2[2] = {0ull, 0ull};  // two pairs of running sums
+          float most = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            uint32_t s[32];
+            scores(k, s);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float x, y;
+              unpack_f32(fma_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, base2), x, y);
+              most = max3(most, x, y);
+              unsigned long long e = pack_f32(exp2_fast(x), exp2_fast(y));
+              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], e);
+              if (I8) {
+                const float2 vs = *reinterpret_cast<const float2*>(mt.v_scale + half * 64 + 32 * k + i);
+                e = mul_f32x2(e, pack_f32(vs.x, vs.y));
+              }
+              unpack_f32(e, x, y);
+              p[16 * k + (i >> 1)] = pack_bf16(x, y);
+            }
+          }
+          {
+            float x, y;
+            unpack_f32(add_f32x2(parts2[0], parts2[1]), x, y);
+            part = x + y;
+          }
+          if (follow) break;
+          // where a weight came out beyond 2^8 (or is a row's first) the pair of warps goes over the block again, with the maximum
+          follow = pair_any(1 + (warp & 3), row < used && (most > 8.f || (m == -INFINITY && most > -INFINITY)));
+          if (!follow) break;
         }
+        sum += part;
+        tmem_st32(s_tmem, p);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
@@ -788,123 +746,49 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const int my_row = w.row0 + tok, my_head = w.head * group + row - tok * group;
       uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
       bool finite = l != 0.f || m == -INFINITY;  // sums of a row are fit to be used
-      auto store = [&](uint16_t* at, const float (&o)[16], float inv) {
-        uint32_t p[8];
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float x = o[j] * inv, y = o[j + 1] * inv;
-          finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
-          p[j >> 1] = pack_bf16(x, y);
+      const bool whole = n == w.blocks;
+      float* to = nullptr;  // partial sums: [four columns][row][4] and (base, l) of every row, in one of this block's two places
+      if (!whole) {
+        const int first = work_owner(w.w0, total, parts), here = (int)blockIdx.x;
+        to = a.partial + (long long)attn_part(here, here == first && begin < w.w0) * attn_part_floats(D);
+        if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
+        if (tid == 0 && here == first) {
+          AttnJoin& j = a.joins[here];
+          j.first = here;
+          j.second_place = begin < w.w0;
+          j.row0 = w.row0; j.used = used; j.head = w.head; j.seq = w.seq; j.first_pos = first_pos;
+          j.parts = work_owner(w.w0 + w.blocks - 1, total, parts) - first + 1;
         }
-        uint4* to = reinterpret_cast<uint4*>(at);
-        to[0] = make_uint4(p[0], p[1], p[2], p[3]);
-        to[1] = make_uint4(p[4], p[5], p[6], p[7]);
-      };
-      bool done = true;
-      if (n == w.blocks) {
-        if (warp_used) {
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-          for (int i = half; i < pieces; i += 2) {
-            uint32_t o[16];
-            tmem_ld16(o_tmem + lanes + i * 16, o);
-            float f[16];
+      }
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      if (warp_used) {
+#pragma unroll 1
+        for (int i = 32 * half; i < D; i += 64) {
+          uint32_t o[32];
+          tmem_ld32_issue(o_tmem + lanes + i, o);
+          tmem_ld_wait32(o);
+          if (!mine) continue;
+          if (!whole) {
 #pragma unroll
-            for (int j = 0; j < 16; j++) f[j] = l == 0.f ? 0.f : __uint_as_float(o[j]);
-            if (mine) store(dst + i * 16, f, inv);
+            for (int j = 0; j < 8; j++)
+              if (i + 4 * j < D) reinterpret_cast<uint4*>(to)[((i >> 2) + j) * 128 + row] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            continue;
           }
-        }
-      } else {
-        // partial sums: [four columns][row][4] and (base, l) of every row, in one of this block's two places
-        const long long w0 = w.w0;
-        const int first = work_owner(w0, total, parts), last = work_owner(w0 + w.blocks - 1, total, parts);
-        auto place = [&](int part) { return part * 2 + (part == first && work_begin(total, part, parts) < w0 ? 1 : 0); };
-        const long long floats = (long long)(D + 2) * 128;
-        {
-          float* const to = a.partial + place(blockIdx.x) * floats;
-          if (warp_used) {
-            for (int i = half; i < pieces; i += 2) {
-              uint32_t o[16];
-              tmem_ld16(o_tmem + lanes + i * 16, o);
-              if (mine) {
-                uint4* at = reinterpret_cast<uint4*>(to) + i * 4 * 128 + row;
 #pragma unroll
-                for (int j = 0; j < 4; j++) at[j * 128] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-              }
+          for (int j = 0; j < 32; j += 8) {
+            if (i + j >= D) continue;
+            uint32_t p[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float x = l == 0.f ? 0.f : __uint_as_float(o[j + 2 * k]) * inv, y = l == 0.f ? 0.f : __uint_as_float(o[j + 2 * k + 1]) * inv;
+              finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
+              p[k] = pack_bf16(x, y);
             }
-            if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
-          }
-        }
-        __threadfence();
-        named_sync(5, kSoftmaxThreads);
-        uint32_t* const counter = a.counters + (long long)w.head * a.max_tiles + w.index;
-        if (tid == 0) {
-          c.arrived = atomicAdd(counter, 1u);
-          if (c.arrived == (uint32_t)(last - first)) *counter = 0;  // as it was found
-        }
-        named_sync(5, kSoftmaxThreads);
-        done = c.arrived == (uint32_t)(last - first);
-        if (done) {
-          __threadfence();
-          // rows' maxima and sums first, `share` threads to a row; then every thread four values at a time, four of them from four parts in flight
-          const int count = last - first + 1;
-          int share = 2;
-          while (share < 32 && used * share * 2 <= kSoftmaxThreads) share *= 2;
-          const int sub = tid & (share - 1), r0 = tid / share;
-          auto at_ml = [&](int f, int r) { return reinterpret_cast<const float2*>(a.partial + place(first + f) * floats + D * 128 + r * 2); };
-          float top = -INFINITY, sums = 0.f;
-          if (r0 < used) {
-#pragma unroll 4
-            for (int f = sub; f < count; f += share) top = fmaxf(top, __ldcg(at_ml(f, r0)).x);
-          }
-          for (int o = 1; o < share; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float from = top == -INFINITY ? 0.f : top;
-          if (r0 < used) {
-#pragma unroll 4
-            for (int f = sub; f < count; f += share) {
-              const float2 ml = __ldcg(at_ml(f, r0));
-              sums += ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - from) * ml.y;
-            }
-          }
-          for (int o = 1; o < share; o <<= 1) sums += __shfl_xor_sync(0xffffffffu, sums, o);
-          if (r0 < used && sub == 0) {
-            if (sums == 0.f && top != -INFINITY) atomicOr(&c.bad_rows[r0 >> 5], 1u << (r0 & 31));
-            c.top[0][0][r0] = from;
-            c.top[0][1][r0] = sums > 0.f ? 1.f / sums : (sums == 0.f ? 0.f : sums);
-          }
-          named_sync(5, kSoftmaxThreads);
-          for (int i = tid; i < used * pieces; i += kSoftmaxThreads) {  // 16 columns of a row
-            const int pc = i / used, r = i - pc * used;
-            const float top_r = c.top[0][0][r], inv = c.top[0][1][r];
-            float o[16] = {};
-            for (int f0 = 0; f0 < count; f0 += 4) {
-              float4 x[4][4];
-              float mf[4];
-#pragma unroll
-              for (int f = 0; f < 4; f++) {
-                const float* part = a.partial + place(first + min(f0 + f, count - 1)) * floats;
-                mf[f] = f0 + f < count ? __ldcg(part + D * 128 + r * 2) : -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; j++) x[f][j] = __ldcg(reinterpret_cast<const float4*>(part) + (pc * 4 + j) * 128 + r);
-              }
-#pragma unroll
-              for (int f = 0; f < 4; f++) {
-                if (mf[f] == -INFINITY) continue;  // that part saw no key of this row
-                const float y = exp2_fast(mf[f] - top_r);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                  o[4 * j] += y * x[f][j].x; o[4 * j + 1] += y * x[f][j].y; o[4 * j + 2] += y * x[f][j].z; o[4 * j + 3] += y * x[f][j].w;
-                }
-              }
-            }
-            const int tk = page_of(r, a.group_div);
-            finite = true;
-            store(a.out + ((long long)(w.row0 + tk) * a.n_q + w.head * group + r - tk * group) * D + pc * 16, o, inv);
-            if (!finite) atomicOr(&c.bad_rows[r >> 5], 1u << (r & 31));
-            finite = true;
+            *reinterpret_cast<uint4*>(dst + i + j) = make_uint4(p[0], p[1], p[2], p[3]);
           }
         }
       }
-      if (done) {
+      if (whole) {
         if (mine && !finite) atomicOr(&c.bad_rows[row >> 5], 1u << (row & 31));
         named_sync(5, kSoftmaxThreads);
         const uint32_t bad[4] = {c.bad_rows[0], c.bad_rows[1], c.bad_rows[2], c.bad_rows[3]};
@@ -913,8 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           for (int r = 0; r < used; r++) {
             if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
             const int tk = page_of(r, a.group_div);
-            const long long p = (long long)w.first_pos + tk;
-            attend_row(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min(p, 0x7fffffffll), sync);
+            attend_row(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min((long long)first_pos + tk, 0x7fffffffll), sync);
           }
           if (tid < 4) c.bad_rows[tid] = 0;
         }
@@ -929,9 +812,89 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   __syncthreads();
   if (warp == 0) {
     __syncwarp();
-    if (*(volatile int*)&c.abort) __nanosleep(1000000);  // let what is in flight land after a failed wait
+    if (*(volatile int*)&c.abort) {
+      if (lane == 0) report_expired_wait(a.status, c.abort);
+      __nanosleep(1000000);  // let what is in flight land after a failed wait
+    }
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Adds up the parts of the tiles that several blocks shared, in their order: 16 rows to a block.
+__global__ void __launch_bounds__(kRowThreads) attn_paged_join_kernel(const AttnPagedArgs a) {
+  grid_dependency_wait();
+  grid_dependency_release();
+  const AttnJoin j = a.joins[blockIdx.x];
+  const int r0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, j.used - r0);
+  if (!j.parts || rows <= 0) return;
+  __shared__ RowScratch plain;
+  __shared__ float tops[kJoinRows], invs[kJoinRows];
+  __shared__ uint32_t bad;
+  const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv;
+  auto part = [&](int f) { return a.partial + (long long)attn_part(j.first + f, f == 0 && j.second_place) * attn_part_floats(D); };
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  {  // 16 threads to a row: its maximum, and the sum against it
+    const int r = tid >> 4, sub = tid & 15;
+    auto ml = [&](int f) { return __ldcg(reinterpret_cast<const float2*>(part(f) + D * 128 + (r0 + r) * 2)); };
+    float top = -INFINITY, sum = 0.f;
+    if (r < rows)
+      for (int f = sub; f < j.parts; f += 16) top = fmaxf(top, ml(f).x);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float from = top == -INFINITY ? 0.f : top;
+    if (r < rows)
+      for (int f = sub; f < j.parts; f += 16) {
+        const float2 x = ml(f);
+        sum += x.x == -INFINITY ? 0.f : exp2_fast(x.x - from) * x.y;
+      }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (r < rows && sub == 0) {
+      tops[r] = from;
+      invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      if (sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
+    }
+  }
+  __syncthreads();
+  const int r = tid & 15;
+  auto out_of = [&](int row, int& tok) {
+    tok = page_of(row, a.group_div);
+    return j.head * group + row - tok * group;
+  };
+  for (int q = tid >> 4; q < D / 4 && r < rows; q += kRowThreads / 16) {  // four columns of a row
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int f0 = 0; f0 < j.parts; f0 += 8) {
+      float4 x[8];
+      float m[8];
+#pragma unroll
+      for (int f = 0; f < 8; f++) {
+        const float* p = part(min(f0 + f, j.parts - 1));
+        m[f] = f0 + f < j.parts ? __ldcg(p + D * 128 + (r0 + r) * 2) : -INFINITY;
+        x[f] = __ldcg(reinterpret_cast<const float4*>(p) + q * 128 + r0 + r);
+      }
+#pragma unroll
+      for (int f = 0; f < 8; f++) {
+        if (m[f] == -INFINITY) continue;  // that part saw no key of this row
+        const float y = exp2_fast(m[f] - tops[r]);
+        o.x += y * x[f].x; o.y += y * x[f].y; o.z += y * x[f].z; o.w += y * x[f].w;
+      }
+    }
+    const float inv = invs[r];
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    if (!(fabsf(o.x) <= 3.0e38f && fabsf(o.y) <= 3.0e38f && fabsf(o.z) <= 3.0e38f && fabsf(o.w) <= 3.0e38f)) atomicOr(&bad, 1u << r);
+    int tok;
+    const int h = out_of(r0 + r, tok);
+    *reinterpret_cast<uint2*>(a.out + ((long long)(j.row0 + tok) * a.n_q + h) * D + q * 4) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+  }
+  __syncthreads();
+  const uint32_t again = bad;
+  for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
+    if (!(again >> i & 1)) continue;
+    int tok;
+    const int h = out_of(r0 + i, tok);
+    attend_row(a, plain, tid, j.row0 + tok, h, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll), [] { __syncthreads(); });
   }
 }
 
@@ -960,7 +923,7 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t rows, int D) {
 
 template <int DC, int UNITS, bool I8>
 cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
-  constexpr int smem = 1024 + (DC + UNITS) * kUnit + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(RowScratch) + (int)sizeof(Control);
+  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? kAhead * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(RowScratch) + (int)sizeof(Control);
   static_assert(smem <= 227 * 1024, "shared memory");
   static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
   auto kernel = attn_paged_tile_kernel<DC, UNITS, I8>;
@@ -977,7 +940,9 @@ cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
   if (!I8 && (!encode_heads(&m.k, a.k, slots, a.v.n_kv, a.v.D, 1, run) || !encode_heads(&m.v, a.vv, slots, a.v.n_kv, a.v.D, 1, run) ||
               !encode_rows(&m.k_rows, a.k, slots * a.v.n_kv, a.v.D) || !encode_rows(&m.v_rows, a.vv, slots * a.v.n_kv, a.v.D)))
     return cudaErrorInvalidValue;
-  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
+  const cudaError_t e = launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(attn_paged_join_kernel, dim3(a.grid, 128 / kJoinRows), dim3(kRowThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -992,17 +957,22 @@ void attn_paged_shape(AttnPagedArgs& a, int sms) {
   while (a.box_rows > 4 && a.v.page_size % a.box_rows) a.box_rows /= 2;
   if (a.box_rows < 8) a.box_rows = 0;
 }
-size_t attn_paged_counter_bytes(const AttnPagedArgs& a) { return (size_t)a.v.n_kv * a.max_tiles * 4; }
-size_t attn_paged_partial_bytes(const AttnPagedArgs& a) { return (size_t)a.grid * 2 * (a.v.D + 2) * 128 * 4; }
+size_t attn_paged_scratch_bytes(const AttnPagedArgs& a) {
+  return (size_t)a.grid * 2 * attn_part_floats(a.v.D) * sizeof(float) + (size_t)a.grid * sizeof(AttnJoin);
+}
+void attn_paged_scratch(AttnPagedArgs& a, void* at) {
+  a.partial = (float*)at;
+  a.joins = (AttnJoin*)(a.partial + (size_t)a.grid * 2 * attn_part_floats(a.v.D));
+}
 
 cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream) {
   a.wait_ns = wait_limit_ns();
   const int units = (a.v.D + 63) / 64;
   if (a.scales)
     return units == 1 ? run_tile<1, 8, true>(a, stream) : units == 2 ? run_tile<2, 8, true>(a, stream)
-         : units == 3 ? run_tile<3, 9, true>(a, stream) : run_tile<4, 9, true>(a, stream);
+         : units == 3 ? run_tile<3, 6, true>(a, stream) : run_tile<4, 6, true>(a, stream);
   return units == 1 ? run_tile<1, 8, false>(a, stream) : units == 2 ? run_tile<2, 8, false>(a, stream)
-       : units == 3 ? run_tile<3, 9, false>(a, stream) : run_tile<4, 9, false>(a, stream);
+       : units == 3 ? run_tile<3, 8, false>(a, stream) : run_tile<4, 8, false>(a, stream);
 }
 
 }  // namespace tb200

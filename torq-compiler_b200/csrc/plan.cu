@@ -1056,19 +1056,6 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
       plan.tensor_loc[id] = Loc{Loc::ARENA, cursor};
       cursor += (bytes_of(id) + 255) & ~(size_t)255;
     }
-  // counters that attn_paged keeps between launches (arrivals at a tile): zero before the first dispatch and left so by every one
-  std::vector<size_t> counters_off(ops.size(), 0);
-  for (size_t i = 0; i < ops.size(); i++) {
-    const auto& op = ops[i];
-    if (op.kind != TB200_OP_ATTN_PAGED || !b.is_t(op.in0, TB200_BF16, 2) || !b.is_t(op.in2, TB200_I32, 1) || op.i1 < 1 || op.i0 < op.i1 || op.i0 / op.i1 > 64)
-      continue;  // refused below
-    AttnPagedArgs a{};
-    a.n_q = op.i0; a.v.n_kv = op.i1; a.v.rows = tensors[op.in0].shape[0]; a.v.S = tensors[op.in2].shape[0];
-    a.v.page_size = 1;
-    attn_paged_shape(a, 1);
-    counters_off[i] = cursor;
-    cursor += (attn_paged_counter_bytes(a) + 255) & ~(size_t)255;
-  }
   plan.state_bytes = cursor;
   {
     struct Block { size_t off, size; int id; };
@@ -2378,18 +2365,20 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         a.v = c.v;
         a.n_q = n_q; a.window = op.i3; a.sinks = op.pad_b; a.max_new = op.pad_l; a.scale = op.f0;
         attn_paged_shape(a, current_sm_count());
-        scratch_need = std::max(scratch_need, attn_paged_partial_bytes(a));
-        const size_t counters = counters_off[i];
+        // the blocks of work of one head are counted in 32 bits
+        if ((long long)a.max_tiles * (c.v.capacity / kKeyBlock + 2) > 0x7fffffffll)
+          return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged: too many rows times positions", i);
+        scratch_need = std::max(scratch_need, attn_paged_scratch_bytes(a));
         // a row of one head is fetched by its 32-bit number
         if ((long long)c.v.rows * n_q > 0x7fffffffll || (long long)c.v.pages * c.v.page_size * c.v.n_kv > 0x7fffffffll)
           return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged supports 2^31 - 1 rows x heads, of the queries and of the cache", i);
         Loc lq = loc(op.in0), lo = loc(op.out0);
         const PagedLoc at = paged_loc(op, op.in1, op.in2, loc);
         step.kernel_name = "attn_paged";
+        step.launches = 2;
         step.launch = [=](const ExecContext& x) {
           AttnPagedArgs k = a;
-          k.partial = (float*)x.scratch;
-          k.counters = (uint32_t*)(x.arena + counters);
+          attn_paged_scratch(k, x.scratch);
           k.status = x.status;
           k.v = at.view(c, x);
           k.q = (const uint16_t*)lq.resolve(x);
