@@ -67,6 +67,8 @@ TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int
   if (s.blocks < 1) s.blocks = 1;
   return s;
 }
+// A tile counts as its blocks and, in front of them, kTileCost more: what it takes to begin it and to store its rows.
+constexpr int kTileCost = 1;
 TB200_BOTH int tile_block(const TileSpan& s, int i) { return i < s.sink_blocks ? i : s.near_block + (i - s.sink_blocks); }
 // `total` pieces of work in one row, shared out to `parts`: part i begins here
 TB200_BOTH long long work_begin(long long total, int i, int parts) { return total * i / parts; }

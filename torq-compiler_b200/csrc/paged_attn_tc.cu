@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     seq0 = lo;
     tile0 = i - first_tile[lo];
     const Span sp = span_of(a, seq0);
-    return tile_span(sp.ctx, sp.n, tile0, tpt, a.window, a.sinks, v.capacity).blocks;
+    return kTileCost + tile_span(sp.ctx, sp.n, tile0, tpt, a.window, a.sinks, v.capacity).blocks;
   };
   int per_head = 0;  // the planner refuses what 32 bits do not hold
   for (int i0 = 0; i0 < n_tiles; i0 += kThreads) {
@@ -331,18 +331,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       release_item(items);
       auto ask = [&](int i) {  // unit i of the item: the keys of block 0, then those of block b and the values of b - 1, by turns
         if (i < units) {
-          const int j = i - DC + 2 * DC, b = j / (2 * DC), r = j - b * 2 * DC;
-          const bool keys = r >= DC ? b == 0 : b < n;  // (j is such that b = 0 begins with the keys of block 0 at r = DC)
+          const int j = i + DC, b = j / (2 * DC), r = j - b * 2 * DC;  // (so that b = 0 begins with the keys of block 0 at r = DC)
+          const bool keys = r >= DC ? b == 0 : b < n;
           const int block = keys ? b : b - 1, u = r >= DC ? r - DC : r;
           const Meta& m = take_meta(block0 + block);
           const char* const pages = (const char*)(keys ? a.k : a.vv) + head_bytes + u * 64;
           const bool in = u * 64 + piece * 16 < D;
+          int slot[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int slot = m.slot[row0 + 32 * k];
-            const bool ok = in && slot >= 0;
-            copy16(own + (i % kAhead) * (kUnit / 2) + k * 16, pages + (ok ? slot * row_bytes : 0), ok);
-          }
+          for (int k = 0; k < 4; k++) slot[k] = in ? m.slot[row0 + 32 * k] : -1;
+          const uint32_t dst = own + (i % kAhead) * (kUnit / 2);
+#pragma unroll
+          for (int k = 0; k < 4; k++) copy16(dst + k * 16, pages + max(slot[k], 0) * row_bytes, slot[k] >= 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
@@ -354,9 +354,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
         if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
         const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128, from = own + (i % kAhead) * (kUnit / 2);
         const uint32_t lo_at = ((2 * piece) ^ (row0 & 7)) << 4, hi_at = ((2 * piece + 1) ^ (row0 & 7)) << 4;  // a thread's rows are 32 apart
+        uint4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = lds128(from + k * 16);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const uint4 q = lds128(from + k * 16);
+          const uint4 q = x[k];
           uint4 lo, hi;
           widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
           widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
@@ -563,16 +566,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           break;
         }
         const TileSpan ts = tile_span(span.ctx, span.n, tile, tpt, a.window, a.sinks, v.capacity);
-        const int b1 = (int)min((long long)ts.blocks, off + (end - cur));
-        w.seq = seq; w.head = head;
-        w.row0 = span.row0 + tile * tpt;
-        w.tokens = min(tpt, span.n - tile * tpt);
-        w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
-        w.near_key = ts.near_key; w.end_key = ts.end_key; w.sink_blocks = ts.sink_blocks; w.near_block = ts.near_block; w.blocks = ts.blocks;
-        w.b0 = off; w.b1 = b1;
-        w.w0 = cur - off;
-        mbar_arrive(smem_u32(&c.item_full[i % kItems]));
-        cur += b1 - off;
+        const int upto = (int)min((long long)ts.blocks + kTileCost, off + (end - cur)), b0 = max(off - kTileCost, 0), b1 = upto - kTileCost;
+        if (b1 > b0) {
+          w.seq = seq; w.head = head;
+          w.row0 = span.row0 + tile * tpt;
+          w.tokens = min(tpt, span.n - tile * tpt);
+          w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
+          w.near_key = ts.near_key; w.end_key = ts.end_key; w.sink_blocks = ts.sink_blocks; w.near_block = ts.near_block; w.blocks = ts.blocks;
+          w.b0 = b0; w.b1 = b1;
+          w.w0 = cur - off + kTileCost;
+          mbar_arrive(smem_u32(&c.item_full[i % kItems]));
+        } else {
+          i--;  // only the front of a tile whose blocks are the next one's
+        }
+        cur += upto - off;
         if (cur >= end) continue;
         off = 0;
         tile++;
@@ -865,17 +872,21 @@ __global__ void __launch_bounds__(kRowThreads) attn_paged_join_kernel(const Attn
   };
   for (int q = tid >> 4; q < D / 4 && r < rows; q += kRowThreads / 16) {  // four columns of a row
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int f0 = 0; f0 < j.parts; f0 += 8) {
-      float4 x[8];
-      float m[8];
+    for (int f0 = 0; f0 < j.parts; f0 += 4) {
+      float4 x[4];
+      float m[4];
 #pragma unroll
-      for (int f = 0; f < 8; f++) {
-        const float* p = part(min(f0 + f, j.parts - 1));
-        m[f] = f0 + f < j.parts ? __ldcg(p + D * 128 + (r0 + r) * 2) : -INFINITY;
+      for (int f = 0; f < 4; f++) {
+        if (f0 + f >= j.parts) {
+          m[f] = -INFINITY;
+          continue;
+        }
+        const float* p = part(f0 + f);
+        m[f] = __ldcg(p + D * 128 + (r0 + r) * 2);
         x[f] = __ldcg(reinterpret_cast<const float4*>(p) + q * 128 + r0 + r);
       }
 #pragma unroll
-      for (int f = 0; f < 8; f++) {
+      for (int f = 0; f < 4; f++) {
         if (m[f] == -INFINITY) continue;  // that part saw no key of this row
         const float y = exp2_fast(m[f] - tops[r]);
         o.x += y * x[f].x; o.y += y * x[f].y; o.z += y * x[f].z; o.w += y * x[f].w;

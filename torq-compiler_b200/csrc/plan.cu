@@ -2366,7 +2366,7 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         a.n_q = n_q; a.window = op.i3; a.sinks = op.pad_b; a.max_new = op.pad_l; a.scale = op.f0;
         attn_paged_shape(a, current_sm_count());
         // the blocks of work of one head are counted in 32 bits
-        if ((long long)a.max_tiles * (c.v.capacity / kKeyBlock + 2) > 0x7fffffffll)
+        if ((long long)a.max_tiles * (c.v.capacity / kKeyBlock + 2 + kTileCost) > 0x7fffffffll)
           return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged: too many rows times positions", i);
         scratch_need = std::max(scratch_need, attn_paged_scratch_bytes(a));
         // a row of one head is fetched by its 32-bit number
