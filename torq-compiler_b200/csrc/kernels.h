@@ -380,7 +380,7 @@ struct AttnJoin {
   int first, second_place, row0, used, head, seq, first_pos;
 };
 // Every block has two places for partial sums: of a tile it goes on with, and of one it begins behind others.
-TB200_BOTH long long attn_part_floats(int D) { return (long long)(D + 2) * 128; }
+TB200_BOTH long long attn_part_floats(int D, int rows) { return (long long)(D + 2) * rows; }  // [D / 4][rows][4], then (base, sum) of the rows
 TB200_BOTH int attn_part(int block, bool second_place) { return block * 2 + (second_place ? 1 : 0); }
 struct AttnPagedArgs {
   PagedView v;
@@ -391,22 +391,21 @@ struct AttnPagedArgs {
   uint16_t* out;      // [rows][n_q * D]
   int n_q, window, sinks, max_new;  // max_new: most rows of a sequence, 0 = any number
   float scale;
-  float* partial;      // sums of tiles that several blocks share, and what to add up (attn_paged_scratch)
-  AttnJoin* joins;
   int* status;
-  // filled by attn_paged_shape
+  // filled by the launchers
+  float* partial;      // sums of tiles that several blocks share
+  AttnJoin* joins;     // and what is to be added up, by block
   int tokens_per_tile, max_tiles, grid;
   int box_rows;        // keys that lie one behind another wherever their block starts: the largest power of two in the page size, 8 .. 128, or 0
-  PageDivisor group_div;
-  // filled by the launchers
-  int few_rows;        // sequences with at most so many rows (tokens x query heads of a key/value head) are the other kernel's
+  int few_rows;        // sequences with at most so many rows (tokens x query heads of a key/value head) go to the kernel for few rows
+  int takes_few;       // this is that kernel
+  int min_blocks;      // least work a block of the grid is started for
+  PageDivisor group_div, piece_div;
   unsigned long long wait_ns;
 };
-constexpr int kTileMinBlocks = 2;  // least key blocks a block of the grid is started for
-void attn_paged_shape(AttnPagedArgs& a, int sms);
-size_t attn_paged_scratch_bytes(const AttnPagedArgs& a);
-void attn_paged_scratch(AttnPagedArgs& a, void* at);
-cudaError_t launch_attn_paged(AttnPagedArgs a, cudaStream_t stream);
+size_t attn_paged_scratch_bytes(const AttnPagedArgs& a, int sms);
+int attn_paged_launches(const AttnPagedArgs& a, int sms);
+cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStream_t stream);
 cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream);
 
 // ---- whole decode step as one persistent kernel (decode_step.cu) ----

@@ -35,6 +35,7 @@ struct PagedView {
   const int32_t* context;    // [S]
   const int32_t* table;      // [S][max_pages]
   int rows, S, max_pages, page_size, pages, n_kv, D;
+  int i8;                    // the caches hold int8
   int capacity;              // max_pages * page_size, at most 2^30
   PageDivisor div;
 };

@@ -1,11 +1,586 @@
-// Which kernel takes which rows of attn_paged.
+// attn_paged: which kernel takes which rows, the kernel for sequences of few rows (a decode step), and the launch that joins what several
+// blocks have done of one tile. paged.h says how the work is cut, paged_attn_tc.cu has the kernel for many rows.
+//
+// Few rows (new tokens times query heads of a key/value head, at most 16): what bounds it is the cache's way from HBM, so every SM has its share
+// of all keys in flight. A tile is up to 8 or 16 rows; each of a block's four warps takes 16 keys of it at a time, by itself: copies into a ring of
+// its own, S^T = K Q^T (keys are the 16-row operand of mma.sync m16n8k16, rows the 8-column one), its own running maximum, O^T += V^T P^T. What
+// is a column of S^T is a column of O^T, so a thread keeps the same two rows throughout; P^T changes its layout by movmatrix and enters in two
+// bf16 terms (2^-17 of it is lost). int8 caches are widened in registers: keys 16 bytes to a thread, the order of the dims inside a step being
+// free as long as the queries follow it; values 2 bytes a tile of 16 dims, dims 8 apart in steps of D / 8. Warps meet in shared memory, in their
+// order. Tiles that several blocks share are joined by the launch behind.
+#include <algorithm>
+
+#include "dependent_launch.cuh"
 #include "kernels.h"
+#include "paged_row.cuh"
+#include "paged_work.cuh"
 
 namespace tb200 {
 
-cudaError_t launch_attn_paged(AttnPagedArgs a, cudaStream_t stream) {
-  a.few_rows = 0;
-  return launch_attn_paged_tile(a, stream);
+namespace {
+
+constexpr int kFewWarps = 4, kFewThreads = kFewWarps * 32, kChunk = 16;  // keys a warp takes at a time
+constexpr int kFewRows = 16;                                               // rows that a tile's partial sums have room for
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // an 8 x 8 tile of 16-bit values, two of a row to a thread
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma_16x8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// How a head of D dims lies in shared memory: dims in steps of 16 (int8: keys in groups of 64, values in groups of 32, what is behind D being
+// finite and unused), rows apart so that no bank is hit twice.
+struct FewShape {
+  int k_pitch, v_pitch, q_pitch, stages, smem, ring;
+};
+TB200_BOTH FewShape few_shape(int D, bool i8, int stages) {
+  FewShape s;
+  if (i8) {
+    s.k_pitch = (D + 63) / 64 * 64;
+    s.k_pitch += s.k_pitch % 128 == 0 ? 64 : 0;   // 64 modulo 128
+    s.v_pitch = (D + 127) / 128 * 128 + 16;       // 16 modulo 128
+  } else {
+    s.k_pitch = s.v_pitch = (2 * D + 127) / 128 * 128 + 16;
+  }
+  s.q_pitch = ((D + 63) / 64 * 64) * 2 + 16;
+  s.stages = stages;
+  s.ring = kFewWarps * stages * kChunk * (s.k_pitch + s.v_pitch);
+  const int meet = kFewWarps * kFewRows * D * 4;  // the warps' sums take the rings' place
+  s.ring = s.ring > meet ? s.ring : meet;
+  s.ring = (s.ring + 15) / 16 * 16;
+  s.smem = s.ring + kFewRows * s.q_pitch + kFewWarps * stages * kChunk * 8 + kFewWarps * kFewRows * 8;
+  return s;
+}
+
+// NT: steps of 16 dims a head has at most. RT: groups of 8 rows of a tile.
+template <int NT, int RT, int STAGES, bool I8>
+__global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnPagedArgs a) {
+  extern __shared__ __align__(16) unsigned char sm[];
+  __shared__ WorkShared shared;
+  __shared__ RowScratch<kFewThreads> plain;
+  __shared__ uint32_t held_bits[kFewWarps][STAGES], bad;
+  const PagedView& v = a.v;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+  const int D = v.D, group = a.n_q / v.n_kv, steps = D >> 4;
+  const FewShape sh = few_shape(D, I8, STAGES);
+  unsigned char* const ring = sm + warp * (STAGES * kChunk * (sh.k_pitch + sh.v_pitch));
+  unsigned char* const qs = sm + sh.ring;
+  float2* const scales = reinterpret_cast<float2*>(qs + kFewRows * sh.q_pitch) + warp * STAGES * kChunk;  // of a chunk's keys and values
+  float2* const meet = reinterpret_cast<float2*>(qs + kFewRows * sh.q_pitch) + kFewWarps * STAGES * kChunk;  // (base, sum) of every warp's rows
+  grid_dependency_wait();
+  grid_dependency_release();
+  if (tid == 0) {
+    a.joins[blockIdx.x].parts = 0;
+    bad = 0;
+  }
+  const Work work = share_out<kFewThreads>(a, shared, reinterpret_cast<int*>(sm));
+  __syncthreads();
+  if (!work.works) return;
+  const float cexp = a.scale * 1.4426950408889634f;
+  const int row_bytes = D * (I8 ? 1 : 2), pieces = row_bytes >> 4;
+  const long long slot_bytes = (long long)v.n_kv * row_bytes;
+  ItemCursor cursor(a, work, shared);
+  Item w;
+  while (cursor.take(a, work, w)) {
+    const int used = w.tokens * group;
+    // queries, rows behind the last and dims behind D as zeros
+    for (int i = tid; i < kFewRows * ((D + 63) / 64 * 8); i += kFewThreads) {
+      const int r = i / ((D + 63) / 64 * 8), c = i - r * ((D + 63) / 64 * 8), tok = page_of(r, a.group_div);
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < used && c * 8 < D)
+        x = __ldg(reinterpret_cast<const uint4*>(a.q + ((long long)(w.row0 + tok) * a.n_q + w.head * group + r - tok * group) * D) + c);
+      *reinterpret_cast<uint4*>(qs + r * sh.q_pitch + c * 16) = x;
+    }
+    // chunks of 16 keys, by turns to the warps; those that no row sees are passed over
+    const Keys keys(a, w);
+    const int n_chunks = (w.b1 - w.b0) * (kKeyBlock / kChunk);
+    auto key_of = [&](int ci) { return keys.first(w.b0 + ci / (kKeyBlock / kChunk)) + (ci % (kKeyBlock / kChunk)) * kChunk; };
+    auto next_chunk = [&](int ci) {
+      for (; ci < n_chunks; ci += kFewWarps) {
+        const int k = key_of(ci);
+        if (k < keys.end_key && (k + kChunk > keys.near_key || k < keys.sinks)) break;
+      }
+      return ci;
+    };
+    int asked = next_chunk(warp), asked_page = 0;  // the chunk whose page ids are on their way: one key to a lane
+    auto ask = [&]() {
+      if (asked < n_chunks) asked_page = keys.ask(key_of(asked) + (lane & 15));
+    };
+    int filled = 0;
+    auto fill = [&]() {  // copies the chunk that was asked for into the next stage, and asks for the one behind it
+      if (asked < n_chunks) {
+        const int stage = filled % STAGES, slot = keys.slot(key_of(asked) + (lane & 15), asked_page);
+        unsigned char* const kd = ring + stage * kChunk * (sh.k_pitch + sh.v_pitch);
+        unsigned char* const vd = kd + kChunk * sh.k_pitch;
+        const long long head_bytes = (long long)w.head * row_bytes;
+        if (I8 && lane < kChunk) {
+          const float* sc = a.scales + (long long)max(slot, 0) * 2 * v.n_kv + w.head;
+          const uint32_t to = smem_at(scales + stage * kChunk + lane);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(sc), "r"(slot >= 0 ? 4 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4), "l"(sc + v.n_kv), "r"(slot >= 0 ? 4 : 0) : "memory");
+        }
+        const unsigned held = __ballot_sync(0xffffffffu, slot >= 0);  // the keys twice over
+        if (lane == 0) held_bits[warp][stage] = held;
+        // (shuffles by every lane in every turn: the pieces of 16 keys are a multiple of 16, not of 32)
+        for (int p0 = 0; p0 < kChunk * pieces; p0 += 32) {
+          const int p = p0 + lane, key = min((int)page_of(p, a.piece_div), kChunk - 1), c = p - key * pieces;
+          const int s = __shfl_sync(0xffffffffu, slot, key);
+          if (p < kChunk * pieces) {
+            const long long from = max(s, 0) * slot_bytes + head_bytes + c * 16;
+            copy16(smem_at(kd + key * sh.k_pitch + c * 16), (const char*)a.k + from, s >= 0);
+            copy16(smem_at(vd + key * sh.v_pitch + c * 16), (const char*)a.vv + from, s >= 0);
+          }
+        }
+        asked = next_chunk(asked + kFewWarps);
+        ask();
+      }
+      filled++;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    ask();
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; i++) fill();
+    __syncthreads();  // the queries are there
+
+    // this thread's rows, 2 tig and 2 tig + 1 of each group of 8
+    int pos[RT][2], near[RT][2];
+    float m[RT][2], sum[RT][2];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int tok = min(page_of(8 * t + 2 * tig + j, a.group_div), w.tokens - 1);
+        pos[t][j] = (int)min((long long)w.first_pos + tok, 0x7fffffffll);
+        near[t][j] = a.window ? max(0, pos[t][j] - a.window + 1) : 0;
+        m[t][j] = -INFINITY;
+        sum[t][j] = 0.f;
+      }
+    float o[NT][RT][4];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[i][t][j] = 0.f;
+
+    int done = 0;
+    for (int ci = next_chunk(warp); ci < n_chunks; ci = next_chunk(ci + kFewWarps), done++) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncwarp();
+      const int stage = done % STAGES, key0 = key_of(ci);
+      unsigned char* const kd = ring + stage * kChunk * (sh.k_pitch + sh.v_pitch);
+      unsigned char* const vd = kd + kChunk * sh.k_pitch;
+      float s[RT][4];
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[t][j] = 0.f;
+      if (!I8) {
+        const uint32_t k_at = smem_at(kd + (lane & 15) * sh.k_pitch + (lane >> 4) * 16);
+        const uint32_t q_at = smem_at(qs + (lane & 7) * sh.q_pitch + (lane >> 3) * 16);
+#pragma unroll
+        for (int i = 0; i < NT; i += 2) {
+          if (i >= steps) continue;
+          uint32_t ka[4], kb[4];
+          ldsm4(ka, k_at + i * 32);
+          if (i + 1 < steps) ldsm4(kb, k_at + i * 32 + 32);
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            uint32_t q[4];
+            ldsm4(q, q_at + t * 8 * sh.q_pitch + i * 32);
+            mma_16x8(s[t], ka[0], ka[1], ka[2], ka[3], q[0], q[1]);
+            if (i + 1 < steps) mma_16x8(s[t], kb[0], kb[1], kb[2], kb[3], q[2], q[3]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < (NT + 3) / 4; i++) {  // 64 dims: this thread's 16 of them, of keys g and g + 8
+          if (i * 4 >= steps) continue;
+          const uint4 lo = *reinterpret_cast<const uint4*>(kd + g * sh.k_pitch + i * 64 + tig * 16);
+          const uint4 hi = *reinterpret_cast<const uint4*>(kd + (g + 8) * sh.k_pitch + i * 64 + tig * 16);
+          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t a0, a1, a2, a3;
+            widen4(wl[j], a0, a2);
+            widen4(wh[j], a1, a3);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+              const uint2 q = *reinterpret_cast<const uint2*>(qs + (8 * t + g) * sh.q_pitch + (i * 64 + tig * 16 + j * 4) * 2);
+              mma_16x8(s[t], a0, a1, a2, a3, q.x, q.y);
+            }
+          }
+        }
+      }
+      // s[t][0], [1]: key g, rows 2 tig, 2 tig + 1; s[t][2], [3]: key g + 8
+      float2 sc[2] = {make_float2(1.f, 1.f), make_float2(1.f, 1.f)};
+      if (I8) {
+        sc[0] = scales[stage * kChunk + g];
+        sc[1] = scales[stage * kChunk + g + 8];
+      }
+      const int ka = key0 + g, kb = ka + 8;
+      bool held[2];
+      {
+        const unsigned bits = held_bits[warp][stage];
+        held[0] = bits >> g & 1;
+        held[1] = bits >> (g + 8) & 1;
+      }
+      uint32_t p_hi[RT][2], p_lo[RT][2];
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        float keep[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const bool see_a = held[0] && ka <= pos[t][j] && (ka >= near[t][j] || ka < a.sinks);
+          const bool see_b = held[1] && kb <= pos[t][j] && (kb >= near[t][j] || kb < a.sinks);
+          const float x = see_a ? s[t][j] * sc[0].x * cexp : -INFINITY, y = see_b ? s[t][2 + j] * sc[1].x * cexp : -INFINITY;
+          float top = fmaxf(x, y);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+          top = fmaxf(top, m[t][j]);
+          const float from = top == -INFINITY ? 0.f : top;
+          keep[j] = m[t][j] == top ? 1.f : exp2_fast(m[t][j] - from);
+          m[t][j] = top;
+          const float px = exp2_fast(x - from), py = exp2_fast(y - from);
+          sum[t][j] = sum[t][j] * keep[j] + px + py;
+          s[t][j] = see_a ? px * sc[0].y : 0.f;
+          s[t][2 + j] = see_b ? py * sc[1].y : 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t hi = pack_bf16(s[t][2 * h], s[t][2 * h + 1]);
+          const uint32_t lo = pack_bf16(s[t][2 * h] - __uint_as_float(hi << 16), s[t][2 * h + 1] - __uint_as_float(hi & 0xffff0000u));
+          p_hi[t][h] = transpose8(hi);
+          p_lo[t][h] = transpose8(lo);
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1];
+            o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
+          }
+        }
+      }
+      if (!I8) {
+        const uint32_t v_at = smem_at(vd + ((lane & 7) + (lane >> 4) * 8) * sh.v_pitch + ((lane >> 3) & 1) * 16);
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+          if (i >= steps) continue;
+          uint32_t va[4];
+          ldsm4_trans(va, v_at + i * 32);
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            mma_16x8(o[i][t], va[0], va[1], va[2], va[3], p_hi[t][0], p_hi[t][1]);
+            mma_16x8(o[i][t], va[0], va[1], va[2], va[3], p_lo[t][0], p_lo[t][1]);
+          }
+        }
+      } else {
+        // dim D' / 8 * g + j (D' = D rounded up to 32) of keys 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9, four j at a time: tiles 2 i, 2 i + 1 of 16 dims
+        const int per = (D + 31) / 32 * 4;
+#pragma unroll
+        for (int i = 0; i < NT / 2; i++) {
+          if (4 * i >= per) continue;
+          uint32_t lo[4], hi[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            widen4(*reinterpret_cast<const uint32_t*>(vd + (2 * tig + (k & 1) + (k >> 1) * 8) * sh.v_pitch + g * per + 4 * i), lo[k], hi[k]);
+          const uint32_t a0 = __byte_perm(lo[0], lo[1], 0x5410), a1 = __byte_perm(lo[0], lo[1], 0x7632);
+          const uint32_t a2 = __byte_perm(lo[2], lo[3], 0x5410), a3 = __byte_perm(lo[2], lo[3], 0x7632);
+          const uint32_t b0 = __byte_perm(hi[0], hi[1], 0x5410), b1 = __byte_perm(hi[0], hi[1], 0x7632);
+          const uint32_t b2 = __byte_perm(hi[2], hi[3], 0x5410), b3 = __byte_perm(hi[2], hi[3], 0x7632);
+#pragma unroll
+          for (int t = 0; t < RT; t++) {
+            mma_16x8(o[2 * i][t], a0, a1, a2, a3, p_hi[t][0], p_hi[t][1]);
+            mma_16x8(o[2 * i][t], a0, a1, a2, a3, p_lo[t][0], p_lo[t][1]);
+            mma_16x8(o[2 * i + 1][t], b0, b1, b2, b3, p_hi[t][0], p_hi[t][1]);
+            mma_16x8(o[2 * i + 1][t], b0, b1, b2, b3, p_lo[t][0], p_lo[t][1]);
+          }
+        }
+      }
+      __syncwarp();
+      fill();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // every warp is through with its ring
+    // [warp][row][D], and (base, sum) of every warp's rows
+    float* const parts = reinterpret_cast<float*>(sm);
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) sum[t][j] += __shfl_xor_sync(0xffffffffu, sum[t][j], off);
+        const int row = 8 * t + 2 * tig + j;
+        if (g == 0) meet[warp * kFewRows + row] = make_float2(m[t][j], sum[t][j]);
+        if (row < used) {
+          float* const to = parts + (warp * kFewRows + row) * D;
+          const int per = (D + 31) / 32 * 4;
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            const int d = I8 ? per * g + 2 * i : 16 * i + g, d2 = I8 ? d + 1 : d + 8;
+            const bool in = I8 ? 2 * i < per : i < steps;
+            if (in && d < D) to[d] = o[i][t][j];
+            if (in && d2 < D) to[d2] = o[i][t][2 + j];
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = w.b1 - w.b0 == w.blocks;
+    const int here = (int)blockIdx.x, first = whole ? here : work_owner(w.w0, work.total, work.parts);
+    float* const to = a.partial + (long long)attn_part(here, here == first && work.begin < w.w0) * attn_part_floats(D, kFewRows);
+    for (int i = tid; i < used * (D >> 2); i += kFewThreads) {  // four dims of a row, the warps in their order
+      const int row = i / (D >> 2), q = i - row * (D >> 2);
+      float top = -INFINITY, all = 0.f;
+#pragma unroll
+      for (int k = 0; k < kFewWarps; k++) top = fmaxf(top, meet[k * kFewRows + row].x);
+      const float from = top == -INFINITY ? 0.f : top;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kFewWarps; k++) {
+        const float2 ml = meet[k * kFewRows + row];
+        if (ml.x == -INFINITY) continue;  // the warp saw no key of this row
+        const float f = exp2_fast(ml.x - from);
+        const float4 y = *reinterpret_cast<const float4*>(parts + (k * kFewRows + row) * D + q * 4);
+        all += f * ml.y;
+        x.x += f * y.x; x.y += f * y.y; x.z += f * y.z; x.w += f * y.w;
+      }
+      if (!whole) {
+        reinterpret_cast<float4*>(to)[q * kFewRows + row] = x;
+        if (q == 0) *reinterpret_cast<float2*>(to + D * kFewRows + row * 2) = make_float2(top, all);
+        continue;
+      }
+      const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);
+      x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+      if (!(fabsf(x.x) <= 3.0e38f && fabsf(x.y) <= 3.0e38f && fabsf(x.z) <= 3.0e38f && fabsf(x.w) <= 3.0e38f) || (all == 0.f && top != -INFINITY))
+        atomicOr(&bad, 1u << row);
+      const int tok = page_of(row, a.group_div);
+      *reinterpret_cast<uint2*>(a.out + ((long long)(w.row0 + tok) * a.n_q + w.head * group + row - tok * group) * D + q * 4) =
+          make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+    }
+    if (!whole && tid == 0 && here == first) write_join(a, work, w, first, used);
+    __syncthreads();  // the rings are free again
+    const uint32_t again = bad;
+    if (again) {  // rare: an infinity or a NaN among the values
+      for (int r = 0; r < used; r++) {
+        if (!(again >> r & 1)) continue;
+        const int tok = page_of(r, a.group_div);
+        attend_row<kFewThreads>(a, plain, tid, w.row0 + tok, w.head * group + r - tok * group, w.seq, (int)min((long long)w.first_pos + tok, 0x7fffffffll), 0, D,
+                                [] { __syncthreads(); });
+      }
+      if (tid == 0) bad = 0;
+    }
+  }
+}
+
+// Adds up the parts of the tiles that several blocks shared, in their order: a block has 16 rows and 64 dims of a tile. What bounds it is how many
+// loads of parts are under way at once, so where rows are few the parts are spread over the threads that this leaves.
+constexpr int kJoinRows = 16, kJoinDims = 64, kJoinThreads = 256;
+struct JoinSet {
+  const float* partial;
+  const AttnJoin* joins;
+  int count, pitch;  // blocks that may have begun a shared tile; rows that partial sums have room for
+};
+__global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const AttnPagedArgs a, const JoinSet many, const JoinSet few) {
+  extern __shared__ __align__(16) unsigned char join_sm[];
+  __shared__ RowScratch<kJoinThreads> plain;
+  __shared__ float4 meet[kJoinThreads];
+  __shared__ float tops[kJoinRows], invs[kJoinRows];
+  __shared__ uint32_t bad;
+  grid_dependency_wait();
+  grid_dependency_release();
+  constexpr int kChunks = 128 / kJoinRows;
+  const bool is_many = (int)blockIdx.x < many.count * kChunks;
+  const JoinSet set = is_many ? many : few;
+  const int at = is_many ? blockIdx.x / kChunks : blockIdx.x - many.count * kChunks, r0 = is_many ? blockIdx.x % kChunks * kJoinRows : 0;
+  const AttnJoin j = set.joins[at];
+  const int rows = min(kJoinRows, j.used - r0);
+  if (!j.parts || rows <= 0) return;
+  const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv, d0 = blockIdx.y * kJoinDims;
+  float2* const ml = reinterpret_cast<float2*>(join_sm);  // [part][16 rows]: (base, sum), then (factor, -)
+  auto part = [&](int f) { return set.partial + (long long)attn_part(j.first + f, f == 0 && j.second_place) * attn_part_floats(D, set.pitch); };
+  if (tid == 0) bad = 0;
+#pragma unroll 4
+  for (int i = tid; i < j.parts * kJoinRows; i += kJoinThreads) {
+    const int f = i / kJoinRows, r = i % kJoinRows;
+    ml[i] = r < rows ? __ldcg(reinterpret_cast<const float2*>(part(f) + D * set.pitch + (r0 + r) * 2)) : make_float2(-INFINITY, 0.f);
+  }
+  __syncthreads();
+  {  // 16 threads to a row: its maximum, and the sum against it
+    const int r = tid >> 4, sub = tid & 15;
+    float top = -INFINITY, sum = 0.f;
+    for (int f = sub; f < j.parts; f += 16) top = fmaxf(top, ml[f * kJoinRows + r].x);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float from = top == -INFINITY ? 0.f : top;
+    for (int f = sub; f < j.parts; f += 16) {
+      float2& x = ml[f * kJoinRows + r];
+      x.x = x.x == -INFINITY ? 0.f : exp2_fast(x.x - from);
+      sum += x.x == 0.f ? 0.f : x.x * x.y;
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (sub == 0) {
+      tops[r] = top;
+      invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      if (r < rows && sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
+    }
+  }
+  __syncthreads();
+  int span = 1;  // a power of two that holds the rows
+  while (span < rows) span *= 2;
+  const int groups = kJoinRows / span, r = tid & (span - 1), q = tid / span & 15, mine = tid / (span * 16);
+  const bool on = r < rows && d0 + q * 4 < D;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (on) {
+    for (int f0 = mine; f0 < j.parts; f0 += 4 * groups) {
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int f = f0 + k * groups;
+        x[k] = f < j.parts ? __ldcg(reinterpret_cast<const float4*>(part(f)) + (d0 / 4 + q) * set.pitch + r0 + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int f = f0 + k * groups;
+        const float y = f < j.parts ? ml[f * kJoinRows + r].x : 0.f;
+        if (y == 0.f) continue;  // that part saw no key of this row
+        o.x += y * x[k].x; o.y += y * x[k].y; o.z += y * x[k].z; o.w += y * x[k].w;
+      }
+    }
+  }
+  meet[tid] = o;
+  __syncthreads();
+  if (mine == 0 && on) {
+    for (int k = 1; k < groups; k++) {
+      const float4 x = meet[tid + k * span * 16];
+      o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+    }
+    const float inv = invs[r];
+    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+    if (!(fabsf(o.x) <= 3.0e38f && fabsf(o.y) <= 3.0e38f && fabsf(o.z) <= 3.0e38f && fabsf(o.w) <= 3.0e38f)) atomicOr(&bad, 1u << r);
+    const int tok = page_of(r0 + r, a.group_div);
+    *reinterpret_cast<uint2*>(a.out + ((long long)(j.row0 + tok) * a.n_q + j.head * group + r0 + r - tok * group) * D + d0 + q * 4) =
+        make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+  }
+  __syncthreads();
+  const uint32_t again = bad;
+  for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
+    if (!(again >> i & 1)) continue;
+    const int tok = page_of(r0 + i, a.group_div);
+    attend_row<kJoinThreads>(a, plain, tid, j.row0 + tok, j.head * group + r0 + i - tok * group, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll), d0,
+                             d0 + kJoinDims, [] { __syncthreads(); });
+  }
+}
+
+// Which kernels run, and how they are cut. Sequences of up to 8 * rt rows (new tokens times query heads of a key/value head) are the kernel
+// for few rows'. Where no sequence can have more, it runs alone; where sequences fill tiles of 128 rows on average, the other one takes all.
+struct Choice {
+  bool few, many;
+  int rt, few_blocks;
+};
+int few_stages(int D, bool i8) { return i8 && D > 128 ? 2 : 3; }
+Choice choose(const AttnPagedArgs& a, int sms) {
+  const int group = a.n_q / a.v.n_kv;
+  const long long most = (long long)(a.max_new ? std::min(a.max_new, a.v.rows) : a.v.rows) * group;
+  Choice c{};
+  c.few = group <= kFewRows;
+  c.many = !c.few || most > kFewRows;
+  if (c.many && (long long)a.v.rows * group / a.v.S >= 128) c.few = false;
+  c.rt = most <= 8 ? 1 : 2;
+  const bool i8 = a.v.i8 != 0;
+  const int per_sm = (227 * 1024) / (few_shape(a.v.D, i8, few_stages(a.v.D, i8)).smem + 4 * 1024);
+  c.few_blocks = c.few ? sms * std::max(1, std::min(3, per_sm)) : 0;
+  return c;
+}
+size_t part_bytes(const AttnPagedArgs& a, int blocks, int rows) {
+  return ((size_t)blocks * 2 * attn_part_floats(a.v.D, rows) * sizeof(float) + 255) & ~(size_t)255;
+}
+
+template <int NT, int RT, int STAGES, bool I8>
+cudaError_t run_few(const AttnPagedArgs& a, int blocks, cudaStream_t stream) {
+  auto kernel = attn_paged_few_kernel<NT, RT, STAGES, I8>;
+  static std::atomic<unsigned long long> attr_done;
+  if (first_use_on_device(attr_done)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few_shape(NT * 16, I8, STAGES).smem);
+    if (e != cudaSuccess) return e;
+    mark_used_on_device(attr_done);
+  }
+  return launch_dependent(kernel, dim3(blocks), dim3(kFewThreads), few_shape(a.v.D, I8, STAGES).smem, stream, a);
+}
+template <int RT>
+cudaError_t run_few(const AttnPagedArgs& a, int blocks, cudaStream_t stream) {
+  const int steps = a.v.D / 16;
+  if (a.scales)
+    return steps <= 4 ? run_few<4, RT, 3, true>(a, blocks, stream) : steps <= 8 ? run_few<8, RT, 3, true>(a, blocks, stream) : run_few<16, RT, 2, true>(a, blocks, stream);
+  return steps <= 4 ? run_few<4, RT, 3, false>(a, blocks, stream) : steps <= 8 ? run_few<8, RT, 3, false>(a, blocks, stream) : run_few<16, RT, 3, false>(a, blocks, stream);
+}
+
+}  // namespace
+
+size_t attn_paged_scratch_bytes(const AttnPagedArgs& a, int sms) {
+  const Choice c = choose(a, sms);
+  return (c.many ? part_bytes(a, sms, 128) : 0) + part_bytes(a, c.few_blocks, kFewRows) + (size_t)(sms + c.few_blocks) * sizeof(AttnJoin);
+}
+int attn_paged_launches(const AttnPagedArgs& a, int sms) {
+  const Choice c = choose(a, sms);
+  return 1 + (c.few ? 1 : 0) + (c.many ? 1 : 0);
+}
+
+cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStream_t stream) {
+  const Choice c = choose(a, sms);
+  const int group = a.n_q / a.v.n_kv;
+  a.group_div = page_divisor(group);
+  a.few_rows = c.few ? 8 * c.rt : 0;
+  a.wait_ns = wait_limit_ns();
+  char* at = (char*)scratch;
+  JoinSet sets[2] = {{(float*)at, nullptr, c.many ? sms : 0, 128}, {(float*)(at + (c.many ? part_bytes(a, sms, 128) : 0)), nullptr, c.few_blocks, kFewRows}};
+  AttnJoin* const joins = (AttnJoin*)((char*)sets[1].partial + part_bytes(a, c.few_blocks, kFewRows));
+  sets[0].joins = joins;
+  sets[1].joins = joins + sms;
+  auto shaped = [&](int tokens, int blocks, const JoinSet& set, int takes_few, int min_blocks) {
+    AttnPagedArgs k = a;
+    k.tokens_per_tile = tokens;
+    k.max_tiles = a.v.rows / tokens + std::min(a.v.S, a.v.rows);
+    k.grid = blocks;
+    k.takes_few = takes_few;
+    k.min_blocks = min_blocks;
+    k.partial = const_cast<float*>(set.partial);
+    k.joins = const_cast<AttnJoin*>(set.joins);
+    return k;
+  };
+  if (c.few) {
+    AttnPagedArgs k = shaped(8 * c.rt / group > 0 ? 8 * c.rt / group : 1, c.few_blocks, sets[1], 1, 1);
+    k.piece_div = page_divisor(a.v.D * (a.scales ? 1 : 2) / 16);
+    const cudaError_t e = c.rt == 1 ? run_few<1>(k, c.few_blocks, stream) : run_few<2>(k, c.few_blocks, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (c.many) {
+    const cudaError_t e = launch_attn_paged_tile(shaped(128 / group, sms, sets[0], 0, 2), stream);
+    if (e != cudaSuccess) return e;
+  }
+  const int join_smem = std::max(sets[0].count, sets[1].count) * kJoinRows * (int)sizeof(float2);
+  static std::atomic<unsigned long long> attr_done;
+  if (first_use_on_device(attr_done)) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_paged_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    if (e != cudaSuccess) return e;
+    mark_used_on_device(attr_done);
+  }
+  return launch_dependent(attn_paged_join_kernel, dim3(sets[0].count * (128 / kJoinRows) + sets[1].count, (a.v.D + kJoinDims - 1) / kJoinDims), dim3(kJoinThreads),
+                          join_smem, stream, a, sets[0], sets[1]);
 }
 
 }  // namespace tb200

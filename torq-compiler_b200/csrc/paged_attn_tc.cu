@@ -15,8 +15,8 @@
 
 #include "dependent_launch.cuh"
 #include "kernels.h"
-#include "paged.cuh"
 #include "paged_row.cuh"
+#include "paged_work.cuh"
 #include "tcgen05_ptx.cuh"
 #include "tensor_map.h"
 
@@ -33,8 +33,8 @@ static_assert(256 * kSoftmaxRegsI8 + 128 * kCopyRegs + 128 * kIssueRegs <= kThre
 static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreads * 128, "register split, bf16");
 constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
-constexpr int kMetaBlocks = 8, kItems = 4, kJoinRows = 16, kAhead = 4;
-static_assert(kSoftmaxThreads == kRowThreads, "the plain row is computed by the softmax warps");
+constexpr int kMetaBlocks = 8, kItems = 4, kAhead = 4;
+using TileRowScratch = RowScratch<kSoftmaxThreads>;  // the plain row is computed by the softmax warps
 
 struct alignas(16) Meta {
   float k_scale[kKeyBlock], v_scale[kKeyBlock];
@@ -42,86 +42,16 @@ struct alignas(16) Meta {
   uint32_t holds[4];    // the keys with a slot, a bit each
   int key0;
 };
-static_assert(sizeof(Meta) % 16 == 0 && sizeof(RowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
-// A piece of work of a block of the grid: key blocks b0 .. b1 - 1 of a tile of one key/value head.
-struct Item {
-  int seq, head;
-  int row0, tokens;         // the tile's rows of the chunk; tokens 0: there is no more work
-  int first_pos;            // position of the first token
-  int near_key, end_key, sink_blocks, near_block, blocks;  // tile_span
-  int b0, b1;
-  long long w0;             // where the tile's work begins
-};
+static_assert(sizeof(Meta) % 16 == 0 && sizeof(TileRowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
 struct Control {
   uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty, item_full[kItems], item_empty[kItems], meta_full[kMetaBlocks], meta_empty[kMetaBlocks];
   Item items[kItems];
   uint32_t tmem, bad_rows[4];
   int abort, stop;
   float top[2][2][128];  // row maxima of the two halves, by parity of the block
-  int totals[kThreads / 32];
-  int start_seq, start_tile, start_index, start_off;
+  WorkShared work;
 };
 
-// what a sequence brings
-struct Span {
-  int row0, n, ctx;
-};
-__device__ __forceinline__ Span span_of(const AttnPagedArgs& a, int s) {
-  Span r;
-  r.row0 = max(a.v.row_start[s], 0);
-  r.n = max(0, min(a.v.row_start[s + 1], a.v.rows) - r.row0);
-  if (a.max_new) r.n = min(r.n, a.max_new);
-  r.ctx = max(a.v.context[s], 0);
-  return r;
-}
-__device__ __forceinline__ int tiles_of(const AttnPagedArgs& a, const Span& s) {
-  return s.n * (a.n_q / a.v.n_kv) > a.few_rows ? (s.n + a.tokens_per_tile - 1) / a.tokens_per_tile : 0;
-}
-
-// The keys of an item, and where the cache holds them. Page ids are asked for a block ahead of their use, without a branch (a branch would wait
-// for each); slots have 32 bits (the planner refuses more), -1 where no token of the tile sees the key or nothing is held.
-struct Keys {
-  const int32_t* pages_of;
-  int near_key, end_key, sinks, sink_blocks, near_block, last, pages, page_size;
-  PageDivisor div;
-  __device__ __forceinline__ Keys(const AttnPagedArgs& a, const Item& w)
-      : pages_of(a.v.table + (long long)w.seq * a.v.max_pages), near_key(w.near_key), end_key(w.end_key), sinks(a.sinks), sink_blocks(w.sink_blocks),
-        near_block(w.near_block), last(a.v.capacity - 1), pages(a.v.pages), page_size(a.v.page_size), div(a.v.div) {}
-  __device__ __forceinline__ int first(int b) const { return (b < sink_blocks ? b : near_block + (b - sink_blocks)) * kKeyBlock; }
-  __device__ __forceinline__ int ask(int key) const {
-    int page;  // volatile: it is to be on its way now, not when it is used
-    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(page) : "l"(pages_of + page_of(min(key, last), div)));
-    return page;
-  }
-  __device__ __forceinline__ bool seen(int key) const { return key < end_key && (key >= near_key || key < sinks); }  // by a token of the tile
-  __device__ __forceinline__ int slot(int key, int page) const {
-    const bool there = seen(key) && page >= 0 && page < pages;
-    return there ? page * page_size + (key - page_of(key, div) * page_size) : -1;
-  }
-};
-
-// Running sum over the block's threads up to and including this one, and the sum of all, through c.totals.
-__device__ __noinline__ int block_scan(Control& c, int x, int& all) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int v = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  __syncthreads();
-  if (lane == 31) c.totals[warp] = v;
-  __syncthreads();
-  const int y = lane < kThreads / 32 ? c.totals[lane] : 0;
-  all = __reduce_add_sync(0xffffffffu, y);
-  return v + __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // two fp32 operations in one instruction
 __device__ __forceinline__ unsigned long long pack_f32(float x, float y) {
   unsigned long long r;
@@ -149,14 +79,6 @@ __device__ __forceinline__ float max3(float a, float b, float d) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(d));
   return r;
 }
-// four int8 -> four bf16, exact: 0x4300 | the low seven bits is 128 + those bits, and 128 comes off again, or 256 where the byte is negative
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t low = w & 0x7f7f7f7fu, off = w & 0x80808080u;
-  const uint32_t a0 = __byte_perm(low, 0x43434343u, 0x4140), a1 = __byte_perm(low, 0x43434343u, 0x4342);
-  const uint32_t c0 = __byte_perm(off, 0x43434343u, 0x4140), c1 = __byte_perm(off, 0x43434343u, 0x4342);
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a0), "r"(c0));
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(a1), "r"(c1));
-}
 __device__ __forceinline__ bool pair_any(int id, bool x) {  // of 64 threads
   int r;
   asm volatile(
@@ -170,14 +92,6 @@ __device__ __forceinline__ bool pair_any(int id, bool x) {  // of 64 threads
   return r != 0;
 }
 __device__ __forceinline__ void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {  // zeros when not valid
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -196,8 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   const uint32_t q_smem = smem_u32(base), ring = q_smem + DC * kUnit;
   unsigned char* const raw = base + (DC + UNITS) * kUnit;  // int8 pieces on their way
   Meta* const meta = reinterpret_cast<Meta*>(raw + (I8 ? kAhead * kUnit / 2 : 0));
-  RowScratch& plain = *reinterpret_cast<RowScratch*>(meta + kMetaBlocks);
-  Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(RowScratch));
+  TileRowScratch& plain = *reinterpret_cast<TileRowScratch*>(meta + kMetaBlocks);
+  Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(TileRowScratch));
   int* const first_tile = reinterpret_cast<int*>(base);  // while the work is shared out: tiles in front of each sequence
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -235,56 +149,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   grid_dependency_wait();
   grid_dependency_release();
 
-  // ---- the work: tiles of the sequences, key blocks of the tiles ----
-  int all = 0, run = 0;
-  for (int s0 = 0; s0 < v.S; s0 += kThreads) {
-    const int s = s0 + tid, upto = run + block_scan(c, s < v.S ? tiles_of(a, span_of(a, s)) : 0, all);
-    if (s < v.S) first_tile[s + 1] = upto;
-    run += all;
-  }
-  if (tid == 0) {
-    first_tile[0] = 0;
-    a.joins[blockIdx.x].parts = 0;
-  }
+  if (tid == 0) a.joins[blockIdx.x].parts = 0;
+  const Work work = share_out<kThreads>(a, c.work, first_tile);
+  const bool works = work.works;
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();  // the first item is known, and first_tile's room is free
   tc_fence_after();
   const uint32_t tmem = c.tmem;
-  const int n_tiles = min(run, a.max_tiles);
-  int seq0 = 0, tile0 = 0;
-  auto blocks_of = [&](int i) {
-    int lo = 0, hi = v.S - 1;  // the last sequence with first_tile[seq] <= i
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first_tile[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
-    seq0 = lo;
-    tile0 = i - first_tile[lo];
-    const Span sp = span_of(a, seq0);
-    return kTileCost + tile_span(sp.ctx, sp.n, tile0, tpt, a.window, a.sinks, v.capacity).blocks;
-  };
-  int per_head = 0;  // the planner refuses what 32 bits do not hold
-  for (int i0 = 0; i0 < n_tiles; i0 += kThreads) {
-    block_scan(c, i0 + tid < n_tiles ? blocks_of(i0 + tid) : 0, all);
-    per_head += all;
-  }
-  const long long total = (long long)per_head * v.n_kv;
-  const int parts = (int)max(1ll, min((long long)gridDim.x, total / kTileMinBlocks));
-  const bool works = total > 0 && (int)blockIdx.x < parts;
-  const long long begin = works ? work_begin(total, blockIdx.x, parts) : 0, end = works ? work_begin(total, blockIdx.x + 1, parts) : 0;
-  const int head0 = works ? (int)(begin / per_head) : 0, rem = (int)(begin - (long long)head0 * per_head);
-  for (int i0 = 0, before = 0; works && i0 < n_tiles && before <= rem; i0 += kThreads) {
-    const int i = i0 + tid, n = i < n_tiles ? blocks_of(i) : 0, upto = before + block_scan(c, n, all);
-    if (n && upto > rem && upto - n <= rem) {
-      c.start_tile = tile0;
-      c.start_seq = seq0;
-      c.start_index = i;
-      c.start_off = rem - (upto - n);
-    }
-    before += all;
-  }
-  __syncthreads();  // the start is known, and first_tile's room is free
 
   // One wait that runs out ends all others at once: every role then runs through without waiting, and the results are not used. (Kept short: it
   // stands in many places, and what bounds this kernel next to its copies is how many instructions its roles have in the cache.)
@@ -552,51 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       }
     } else if (works && warp == kSoftmaxWarps + kCopyWarps + 1 && lane == 0) {
       // ---------------------------------------------- the block's items
-      long long cur = begin;
-      int head = head0, seq = c.start_seq, tile = c.start_tile, index = c.start_index, off = c.start_off;
-      Span span = span_of(a, seq);
-      int tiles = tiles_of(a, span);
+      ItemCursor cursor(a, work, c.work);
       for (uint32_t i = 0;; i++) {
         if (i >= kItems) wait(c.item_empty[i % kItems], (i / kItems - 1) & 1, 311);
         if (gave_up) break;
-        Item& w = c.items[i % kItems];
-        if (cur >= end) {
-          w.tokens = 0;
-          mbar_arrive(smem_u32(&c.item_full[i % kItems]));
-          break;
-        }
-        const TileSpan ts = tile_span(span.ctx, span.n, tile, tpt, a.window, a.sinks, v.capacity);
-        const int upto = (int)min((long long)ts.blocks + kTileCost, off + (end - cur)), b0 = max(off - kTileCost, 0), b1 = upto - kTileCost;
-        if (b1 > b0) {
-          w.seq = seq; w.head = head;
-          w.row0 = span.row0 + tile * tpt;
-          w.tokens = min(tpt, span.n - tile * tpt);
-          w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
-          w.near_key = ts.near_key; w.end_key = ts.end_key; w.sink_blocks = ts.sink_blocks; w.near_block = ts.near_block; w.blocks = ts.blocks;
-          w.b0 = b0; w.b1 = b1;
-          w.w0 = cur - off + kTileCost;
-          mbar_arrive(smem_u32(&c.item_full[i % kItems]));
-        } else {
-          i--;  // only the front of a tile whose blocks are the next one's
-        }
-        cur += upto - off;
-        if (cur >= end) continue;
-        off = 0;
-        tile++;
-        if (++index >= n_tiles) {  // the next head begins
-          index = 0;
-          head++;
-          seq = -1;
-          tile = tiles;
-        }
-        if (tile >= tiles) {
-          tile = 0;
-          do {
-            if (++seq >= v.S) seq = 0;  // there is a tile, so a sequence with one
-            span = span_of(a, seq);
-            tiles = tiles_of(a, span);
-          } while (!tiles);
-        }
+        const bool more = cursor.take(a, work, c.items[i % kItems]);
+        mbar_arrive(smem_u32(&c.item_full[i % kItems]));
+        if (!more) break;
       }
     }
   } else {
@@ -756,16 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       const bool whole = n == w.blocks;
       float* to = nullptr;  // partial sums: [four columns][row][4] and (base, l) of every row, in one of this block's two places
       if (!whole) {
-        const int first = work_owner(w.w0, total, parts), here = (int)blockIdx.x;
-        to = a.partial + (long long)attn_part(here, here == first && begin < w.w0) * attn_part_floats(D);
+        const int first = work_owner(w.w0, work.total, work.parts), here = (int)blockIdx.x;
+        to = a.partial + (long long)attn_part(here, here == first && work.begin < w.w0) * attn_part_floats(D, 128);
         if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
-        if (tid == 0 && here == first) {
-          AttnJoin& j = a.joins[here];
-          j.first = here;
-          j.second_place = begin < w.w0;
-          j.row0 = w.row0; j.used = used; j.head = w.head; j.seq = w.seq; j.first_pos = first_pos;
-          j.parts = work_owner(w.w0 + w.blocks - 1, total, parts) - first + 1;
-        }
+        if (tid == 0 && here == first) write_join(a, work, w, first, used);
       }
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       if (warp_used) {
@@ -804,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           for (int r = 0; r < used; r++) {
             if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
             const int tk = page_of(r, a.group_div);
-            attend_row(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min((long long)first_pos + tk, 0x7fffffffll), sync);
+            attend_row<kSoftmaxThreads>(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min((long long)first_pos + tk, 0x7fffffffll), 0, D, sync);
           }
           if (tid < 4) c.bad_rows[tid] = 0;
         }
@@ -825,87 +652,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     }
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  }
-}
-
-// Adds up the parts of the tiles that several blocks shared, in their order: 16 rows to a block.
-__global__ void __launch_bounds__(kRowThreads) attn_paged_join_kernel(const AttnPagedArgs a) {
-  grid_dependency_wait();
-  grid_dependency_release();
-  const AttnJoin j = a.joins[blockIdx.x];
-  const int r0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, j.used - r0);
-  if (!j.parts || rows <= 0) return;
-  __shared__ RowScratch plain;
-  __shared__ float tops[kJoinRows], invs[kJoinRows];
-  __shared__ uint32_t bad;
-  const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv;
-  auto part = [&](int f) { return a.partial + (long long)attn_part(j.first + f, f == 0 && j.second_place) * attn_part_floats(D); };
-  if (tid == 0) bad = 0;
-  __syncthreads();
-  {  // 16 threads to a row: its maximum, and the sum against it
-    const int r = tid >> 4, sub = tid & 15;
-    auto ml = [&](int f) { return __ldcg(reinterpret_cast<const float2*>(part(f) + D * 128 + (r0 + r) * 2)); };
-    float top = -INFINITY, sum = 0.f;
-    if (r < rows)
-      for (int f = sub; f < j.parts; f += 16) top = fmaxf(top, ml(f).x);
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float from = top == -INFINITY ? 0.f : top;
-    if (r < rows)
-      for (int f = sub; f < j.parts; f += 16) {
-        const float2 x = ml(f);
-        sum += x.x == -INFINITY ? 0.f : exp2_fast(x.x - from) * x.y;
-      }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (r < rows && sub == 0) {
-      tops[r] = from;
-      invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      if (sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
-    }
-  }
-  __syncthreads();
-  const int r = tid & 15;
-  auto out_of = [&](int row, int& tok) {
-    tok = page_of(row, a.group_div);
-    return j.head * group + row - tok * group;
-  };
-  for (int q = tid >> 4; q < D / 4 && r < rows; q += kRowThreads / 16) {  // four columns of a row
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int f0 = 0; f0 < j.parts; f0 += 4) {
-      float4 x[4];
-      float m[4];
-#pragma unroll
-      for (int f = 0; f < 4; f++) {
-        if (f0 + f >= j.parts) {
-          m[f] = -INFINITY;
-          continue;
-        }
-        const float* p = part(f0 + f);
-        m[f] = __ldcg(p + D * 128 + (r0 + r) * 2);
-        x[f] = __ldcg(reinterpret_cast<const float4*>(p) + q * 128 + r0 + r);
-      }
-#pragma unroll
-      for (int f = 0; f < 4; f++) {
-        if (m[f] == -INFINITY) continue;  // that part saw no key of this row
-        const float y = exp2_fast(m[f] - tops[r]);
-        o.x += y * x[f].x; o.y += y * x[f].y; o.z += y * x[f].z; o.w += y * x[f].w;
-      }
-    }
-    const float inv = invs[r];
-    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-    if (!(fabsf(o.x) <= 3.0e38f && fabsf(o.y) <= 3.0e38f && fabsf(o.z) <= 3.0e38f && fabsf(o.w) <= 3.0e38f)) atomicOr(&bad, 1u << r);
-    int tok;
-    const int h = out_of(r0 + r, tok);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(j.row0 + tok) * a.n_q + h) * D + q * 4) = make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
-  }
-  __syncthreads();
-  const uint32_t again = bad;
-  for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
-    if (!(again >> i & 1)) continue;
-    int tok;
-    const int h = out_of(r0 + i, tok);
-    attend_row(a, plain, tid, j.row0 + tok, h, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll), [] { __syncthreads(); });
   }
 }
 
@@ -934,7 +680,7 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t rows, int D) {
 
 template <int DC, int UNITS, bool I8>
 cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
-  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? kAhead * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(RowScratch) + (int)sizeof(Control);
+  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? kAhead * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(TileRowScratch) + (int)sizeof(Control);
   static_assert(smem <= 227 * 1024, "shared memory");
   static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
   auto kernel = attn_paged_tile_kernel<DC, UNITS, I8>;
@@ -951,33 +697,15 @@ cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
   if (!I8 && (!encode_heads(&m.k, a.k, slots, a.v.n_kv, a.v.D, 1, run) || !encode_heads(&m.v, a.vv, slots, a.v.n_kv, a.v.D, 1, run) ||
               !encode_rows(&m.k_rows, a.k, slots * a.v.n_kv, a.v.D) || !encode_rows(&m.v_rows, a.vv, slots * a.v.n_kv, a.v.D)))
     return cudaErrorInvalidValue;
-  const cudaError_t e = launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
-  if (e != cudaSuccess) return e;
-  return launch_dependent(attn_paged_join_kernel, dim3(a.grid, 128 / kJoinRows), dim3(kRowThreads), 0, stream, a);
+  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
 }
 
 }  // namespace
 
-void attn_paged_shape(AttnPagedArgs& a, int sms) {
-  const int group = a.n_q / a.v.n_kv;
-  a.tokens_per_tile = 128 / group;
-  a.group_div = page_divisor(group);
-  a.max_tiles = a.v.rows / a.tokens_per_tile + std::min(a.v.S, a.v.rows);
-  a.grid = sms;
+cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream) {
   a.box_rows = 128;
   while (a.box_rows > 4 && a.v.page_size % a.box_rows) a.box_rows /= 2;
   if (a.box_rows < 8) a.box_rows = 0;
-}
-size_t attn_paged_scratch_bytes(const AttnPagedArgs& a) {
-  return (size_t)a.grid * 2 * attn_part_floats(a.v.D) * sizeof(float) + (size_t)a.grid * sizeof(AttnJoin);
-}
-void attn_paged_scratch(AttnPagedArgs& a, void* at) {
-  a.partial = (float*)at;
-  a.joins = (AttnJoin*)(a.partial + (size_t)a.grid * 2 * attn_part_floats(a.v.D));
-}
-
-cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream) {
-  a.wait_ns = wait_limit_ns();
   const int units = (a.v.D + 63) / 64;
   if (a.scales)
     return units == 1 ? run_tile<1, 8, true>(a, stream) : units == 2 ? run_tile<2, 8, true>(a, stream)

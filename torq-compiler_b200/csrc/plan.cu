@@ -425,6 +425,7 @@ bool paged_plan(Builder& b, const tb200_op_t& op, int row_start, int context, in
   c.v.page_size = p.shape[2];
   c.v.n_kv = n_kv;
   c.v.D = D;
+  c.v.i8 = c.i8;
   c.v.capacity = c.v.max_pages * c.v.page_size;
   c.v.div = page_divisor(c.v.page_size);
   const size_t slots = (size_t)layer * p.shape[1] * p.shape[2];
@@ -2364,21 +2365,20 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         AttnPagedArgs a{};
         a.v = c.v;
         a.n_q = n_q; a.window = op.i3; a.sinks = op.pad_b; a.max_new = op.pad_l; a.scale = op.f0;
-        attn_paged_shape(a, current_sm_count());
+        const int sms = current_sm_count();
         // the blocks of work of one head are counted in 32 bits
-        if ((long long)a.max_tiles * (c.v.capacity / kKeyBlock + 2 + kTileCost) > 0x7fffffffll)
+        if ((c.v.rows + (long long)c.v.S) * (c.v.capacity / kKeyBlock + 2 + kTileCost) > 0x7fffffffll)
           return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged: too many rows times positions", i);
-        scratch_need = std::max(scratch_need, attn_paged_scratch_bytes(a));
+        scratch_need = std::max(scratch_need, attn_paged_scratch_bytes(a, sms));
         // a row of one head is fetched by its 32-bit number
         if ((long long)c.v.rows * n_q > 0x7fffffffll || (long long)c.v.pages * c.v.page_size * c.v.n_kv > 0x7fffffffll)
           return b.fail(TB200_UNIMPLEMENTED, "op %d: attn_paged supports 2^31 - 1 rows x heads, of the queries and of the cache", i);
         Loc lq = loc(op.in0), lo = loc(op.out0);
         const PagedLoc at = paged_loc(op, op.in1, op.in2, loc);
         step.kernel_name = "attn_paged";
-        step.launches = 2;
+        step.launches = attn_paged_launches(a, sms);
         step.launch = [=](const ExecContext& x) {
           AttnPagedArgs k = a;
-          attn_paged_scratch(k, x.scratch);
           k.status = x.status;
           k.v = at.view(c, x);
           k.q = (const uint16_t*)lq.resolve(x);
@@ -2386,7 +2386,7 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.vv = (const char*)at.v.resolve(x) + c.layer_bytes;
           k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.out = (uint16_t*)lo.resolve(x);
-          report(launch_attn_paged(k, x.stream), x);
+          report(launch_attn_paged(k, sms, x.scratch, x.stream), x);
         };
         break;
       }
