@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
 
     // this thread's rows, 2 tig and 2 tig + 1 of each group of 8
     int pos[RT][2], near[RT][2];
-    float m[RT][2], sum[RT][2];
+    float m[RT][2], base[RT][2], sum[RT][2];  // m: from where on a score moves base, the scaled score that exponents are taken from
+    const int last_near = a.window ? max(0, (int)min((long long)w.first_pos + w.tokens - 1, 0x7fffffffll) - a.window + 1) : 0;
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
         pos[t][j] = (int)min((long long)w.first_pos + tok, 0x7fffffffll);
         near[t][j] = a.window ? max(0, pos[t][j] - a.window + 1) : 0;
         m[t][j] = -INFINITY;
-        sum[t][j] = 0.f;
+        base[t][j] = sum[t][j] = 0.f;
       }
     float o[NT][RT][4];
 #pragma unroll
@@ -231,33 +232,66 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
         sc[0] = scales[stage * kChunk + g];
         sc[1] = scales[stage * kChunk + g + 8];
       }
-      const int ka = key0 + g, kb = ka + 8;
-      bool held[2];
-      {
-        const unsigned bits = held_bits[warp][stage];
-        held[0] = bits >> g & 1;
-        held[1] = bits >> (g + 8) & 1;
+      // x = scores in units of log2; keys that a row does not see at -inf. Only chunks at an edge of what the tile sees need looking at key by key.
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          s[t][j] *= sc[0].x;
+          s[t][2 + j] *= sc[1].x;
+        }
+      const bool edge = held_bits[warp][stage] != 0xffffffffu || key0 + kChunk - 1 > w.first_pos || (key0 < last_near && key0 + kChunk > a.sinks);
+      if (edge) {
+        const bool held_a = held_bits[warp][stage] >> g & 1, held_b = held_bits[warp][stage] >> (g + 8) & 1;
+        const int ka = key0 + g, kb = ka + 8;
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            if (!(held_a && ka <= pos[t][j] && (ka >= near[t][j] || ka < a.sinks))) s[t][j] = -INFINITY;
+            if (!(held_b && kb <= pos[t][j] && (kb >= near[t][j] || kb < a.sinks))) s[t][2 + j] = -INFINITY;
+          }
+      }
+      // m follows a row's maximum only where a weight would grow beyond 2^8 (or is the row's first): a bound serves as well, and costs no shuffles
+      bool grows = false;
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) grows = grows || fmaxf(s[t][j], s[t][2 + j]) > m[t][j];
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          float keep[2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            float top = fmaxf(s[t][j], s[t][2 + j]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            keep[j] = 1.f;
+            if (top > m[t][j]) {
+              const float to = top * cexp;
+              keep[j] = m[t][j] == -INFINITY ? 0.f : exp2_fast(base[t][j] - to);
+              base[t][j] = to;
+              m[t][j] = top + 8.f / cexp;
+              sum[t][j] *= keep[j];
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < NT; i++) {
+            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1];
+            o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
+          }
+        }
       }
       uint32_t p_hi[RT][2], p_lo[RT][2];
 #pragma unroll
       for (int t = 0; t < RT; t++) {
-        float keep[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const bool see_a = held[0] && ka <= pos[t][j] && (ka >= near[t][j] || ka < a.sinks);
-          const bool see_b = held[1] && kb <= pos[t][j] && (kb >= near[t][j] || kb < a.sinks);
-          const float x = see_a ? s[t][j] * sc[0].x * cexp : -INFINITY, y = see_b ? s[t][2 + j] * sc[1].x * cexp : -INFINITY;
-          float top = fmaxf(x, y);
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-          top = fmaxf(top, m[t][j]);
-          const float from = top == -INFINITY ? 0.f : top;
-          keep[j] = m[t][j] == top ? 1.f : exp2_fast(m[t][j] - from);
-          m[t][j] = top;
-          const float px = exp2_fast(x - from), py = exp2_fast(y - from);
-          sum[t][j] = sum[t][j] * keep[j] + px + py;
-          s[t][j] = see_a ? px * sc[0].y : 0.f;
-          s[t][2 + j] = see_b ? py * sc[1].y : 0.f;
+        for (int j = 0; j < 2; j++) {  // (a row without a key has base 0 and scores of -inf: weights of zero)
+          const float x = exp2_fast(fmaf(s[t][j], cexp, -base[t][j])), y = exp2_fast(fmaf(s[t][2 + j], cexp, -base[t][j]));
+          sum[t][j] += x + y;
+          s[t][j] = I8 ? (x == 0.f ? 0.f : x * sc[0].y) : x;
+          s[t][2 + j] = I8 ? (y == 0.f ? 0.f : y * sc[1].y) : y;
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -265,13 +299,6 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
           const uint32_t lo = pack_bf16(s[t][2 * h] - __uint_as_float(hi << 16), s[t][2 * h + 1] - __uint_as_float(hi & 0xffff0000u));
           p_hi[t][h] = transpose8(hi);
           p_lo[t][h] = transpose8(lo);
-        }
-        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
-#pragma unroll
-          for (int i = 0; i < NT; i++) {
-            o[i][t][0] *= keep[0]; o[i][t][1] *= keep[1];
-            o[i][t][2] *= keep[0]; o[i][t][3] *= keep[1];
-          }
         }
       }
       if (!I8) {
@@ -293,14 +320,13 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
 #pragma unroll
         for (int i = 0; i < NT / 2; i++) {
           if (4 * i >= per) continue;
-          uint32_t lo[4], hi[4];
+          uint32_t x[4], a0, a1, a2, a3, b0, b1, b2, b3;
 #pragma unroll
-          for (int k = 0; k < 4; k++)
-            widen4(*reinterpret_cast<const uint32_t*>(vd + (2 * tig + (k & 1) + (k >> 1) * 8) * sh.v_pitch + g * per + 4 * i), lo[k], hi[k]);
-          const uint32_t a0 = __byte_perm(lo[0], lo[1], 0x5410), a1 = __byte_perm(lo[0], lo[1], 0x7632);
-          const uint32_t a2 = __byte_perm(lo[2], lo[3], 0x5410), a3 = __byte_perm(lo[2], lo[3], 0x7632);
-          const uint32_t b0 = __byte_perm(hi[0], hi[1], 0x5410), b1 = __byte_perm(hi[0], hi[1], 0x7632);
-          const uint32_t b2 = __byte_perm(hi[2], hi[3], 0x5410), b3 = __byte_perm(hi[2], hi[3], 0x7632);
+          for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const uint32_t*>(vd + (2 * tig + (k & 1) + (k >> 1) * 8) * sh.v_pitch + g * per + 4 * i);
+          widen4(__byte_perm(x[0], x[1], 0x5140), a0, a1);  // two keys' bytes side by side, then widened
+          widen4(__byte_perm(x[0], x[1], 0x7362), b0, b1);
+          widen4(__byte_perm(x[2], x[3], 0x5140), a2, a3);
+          widen4(__byte_perm(x[2], x[3], 0x7362), b2, b3);
 #pragma unroll
           for (int t = 0; t < RT; t++) {
             mma_16x8(o[2 * i][t], a0, a1, a2, a3, p_hi[t][0], p_hi[t][1]);
@@ -324,7 +350,7 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) sum[t][j] += __shfl_xor_sync(0xffffffffu, sum[t][j], off);
         const int row = 8 * t + 2 * tig + j;
-        if (g == 0) meet[warp * kFewRows + row] = make_float2(m[t][j], sum[t][j]);
+        if (g == 0) meet[warp * kFewRows + row] = make_float2(m[t][j] == -INFINITY ? m[t][j] : base[t][j], sum[t][j]);
         if (row < used) {
           float* const to = parts + (warp * kFewRows + row) * D;
           const int per = (D + 31) / 32 * 4;
@@ -398,18 +424,21 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Att
   extern __shared__ __align__(16) unsigned char join_sm[];
   __shared__ RowScratch<kJoinThreads> plain;
   __shared__ float4 meet[kJoinThreads];
-  __shared__ float tops[kJoinRows], invs[kJoinRows];
+  __shared__ float invs[kJoinRows];
   __shared__ uint32_t bad;
   grid_dependency_wait();
   grid_dependency_release();
   constexpr int kChunks = 128 / kJoinRows;
   const bool is_many = (int)blockIdx.x < many.count * kChunks;
   const JoinSet set = is_many ? many : few;
-  const int at = is_many ? blockIdx.x / kChunks : blockIdx.x - many.count * kChunks, r0 = is_many ? blockIdx.x % kChunks * kJoinRows : 0;
+  // tiles of many rows: 16 of them to a block, all dims one after another; tiles of few rows: 64 dims to a block
+  const int rest = (int)blockIdx.x - many.count * kChunks, dim_blocks = (a.v.D + kJoinDims - 1) / kJoinDims;
+  const int at = is_many ? blockIdx.x / kChunks : rest / dim_blocks, r0 = is_many ? blockIdx.x % kChunks * kJoinRows : 0;
+  const int first_dim = is_many ? 0 : rest % dim_blocks * kJoinDims, end_dim = is_many ? a.v.D : min(a.v.D, first_dim + kJoinDims);
   const AttnJoin j = set.joins[at];
   const int rows = min(kJoinRows, j.used - r0);
   if (!j.parts || rows <= 0) return;
-  const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv, d0 = blockIdx.y * kJoinDims;
+  const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv;
   float2* const ml = reinterpret_cast<float2*>(join_sm);  // [part][16 rows]: (base, sum), then (factor, -)
   auto part = [&](int f) { return set.partial + (long long)attn_part(j.first + f, f == 0 && j.second_place) * attn_part_floats(D, set.pitch); };
   if (tid == 0) bad = 0;
@@ -434,7 +463,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Att
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sub == 0) {
-      tops[r] = top;
       invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
       if (r < rows && sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
     }
@@ -443,6 +471,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Att
   int span = 1;  // a power of two that holds the rows
   while (span < rows) span *= 2;
   const int groups = kJoinRows / span, r = tid & (span - 1), q = tid / span & 15, mine = tid / (span * 16);
+  for (int d0 = first_dim; d0 < end_dim; d0 += kJoinDims) {
   const bool on = r < rows && d0 + q * 4 < D;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (on) {
@@ -477,12 +506,13 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Att
         make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
   }
   __syncthreads();
+  }
   const uint32_t again = bad;
   for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
     if (!(again >> i & 1)) continue;
     const int tok = page_of(r0 + i, a.group_div);
-    attend_row<kJoinThreads>(a, plain, tid, j.row0 + tok, j.head * group + r0 + i - tok * group, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll), d0,
-                             d0 + kJoinDims, [] { __syncthreads(); });
+    attend_row<kJoinThreads>(a, plain, tid, j.row0 + tok, j.head * group + r0 + i - tok * group, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll),
+                             first_dim, end_dim, [] { __syncthreads(); });
   }
 }
 
@@ -579,7 +609,7 @@ cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStrea
     if (e != cudaSuccess) return e;
     mark_used_on_device(attr_done);
   }
-  return launch_dependent(attn_paged_join_kernel, dim3(sets[0].count * (128 / kJoinRows) + sets[1].count, (a.v.D + kJoinDims - 1) / kJoinDims), dim3(kJoinThreads),
+  return launch_dependent(attn_paged_join_kernel, dim3(sets[0].count * (128 / kJoinRows) + sets[1].count * ((a.v.D + kJoinDims - 1) / kJoinDims)), dim3(kJoinThreads),
                           join_smem, stream, a, sets[0], sets[1]);
 }
 
