@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
   if (!work.works) return;
   const float cexp = a.scale * 1.4426950408889634f;
   const int row_bytes = D * (I8 ? 1 : 2), pieces = row_bytes >> 4;
-  const long long slot_bytes = (long long)v.n_kv * row_bytes;
+  const unsigned slot_bytes = (unsigned)v.n_kv * row_bytes;
+  const int lane_key = page_of(lane, a.piece_div), lane_piece = lane - lane_key * pieces, step_keys = page_of(32, a.piece_div), step_pieces = 32 - step_keys * pieces;
   ItemCursor cursor(a, work, shared);
   Item w;
   while (cursor.take(a, work, w)) {
@@ -134,14 +135,28 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
         }
         const unsigned held = __ballot_sync(0xffffffffu, slot >= 0);  // the keys twice over
         if (lane == 0) held_bits[warp][stage] = held;
-        // (shuffles by every lane in every turn: the pieces of 16 keys are a multiple of 16, not of 32)
-        for (int p0 = 0; p0 < kChunk * pieces; p0 += 32) {
-          const int p = p0 + lane, key = min((int)page_of(p, a.piece_div), kChunk - 1), c = p - key * pieces;
-          const int s = __shfl_sync(0xffffffffu, slot, key);
-          if (p < kChunk * pieces) {
-            const long long from = max(s, 0) * slot_bytes + head_bytes + c * 16;
-            copy16(smem_at(kd + key * sh.k_pitch + c * 16), (const char*)a.k + from, s >= 0);
-            copy16(smem_at(vd + key * sh.v_pitch + c * 16), (const char*)a.vv + from, s >= 0);
+        // piece by piece, 32 at a time: a lane steps from (key, piece) to the one 32 further on
+        int key = lane_key, c = lane_piece;
+        uint32_t k_to = smem_at(kd + key * sh.k_pitch + c * 16), v_to = smem_at(vd + key * sh.v_pitch + c * 16);
+        const char* const k_from = (const char*)a.k + head_bytes;
+        const char* const v_from = (const char*)a.vv + head_bytes;
+#pragma unroll 2
+        for (int p0 = 0; p0 < kChunk * pieces; p0 += 32) {  // (every lane shuffles in every turn: 16 keys' pieces need not be a multiple of 32)
+          const int s = __shfl_sync(0xffffffffu, slot, key & 15);
+          if (key < kChunk) {
+            const unsigned long long from = (unsigned long long)(unsigned)max(s, 0) * slot_bytes + (unsigned)(c * 16);
+            copy16(k_to, k_from + from, s >= 0);
+            copy16(v_to, v_from + from, s >= 0);
+          }
+          key += step_keys;
+          c += step_pieces;
+          k_to += step_keys * sh.k_pitch + step_pieces * 16;
+          v_to += step_keys * sh.v_pitch + step_pieces * 16;
+          if (c >= pieces) {
+            c -= pieces;
+            key++;
+            k_to += sh.k_pitch - pieces * 16;
+            v_to += sh.v_pitch - pieces * 16;
           }
         }
         asked = next_chunk(asked + kFewWarps);
@@ -214,14 +229,18 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
           const uint4 hi = *reinterpret_cast<const uint4*>(kd + (g + 8) * sh.k_pitch + i * 64 + tig * 16);
           const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            uint32_t a0, a1, a2, a3;
-            widen4(wl[j], a0, a2);
-            widen4(wh[j], a1, a3);
+          for (int j = 0; j < 4; j += 2) {
+            uint32_t a0[2], a1[2], a2[2], a3[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              widen4(wl[j + k], a0[k], a2[k]);
+              widen4(wh[j + k], a1[k], a3[k]);
+            }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-              const uint2 q = *reinterpret_cast<const uint2*>(qs + (8 * t + g) * sh.q_pitch + (i * 64 + tig * 16 + j * 4) * 2);
-              mma_16x8(s[t], a0, a1, a2, a3, q.x, q.y);
+              const uint4 q = *reinterpret_cast<const uint4*>(qs + (8 * t + g) * sh.q_pitch + (i * 64 + tig * 16 + j * 4) * 2);
+              mma_16x8(s[t], a0[0], a1[0], a2[0], a3[0], q.x, q.y);
+              mma_16x8(s[t], a0[1], a1[1], a2[1], a3[1], q.z, q.w);
             }
           }
         }
@@ -317,12 +336,9 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
       } else {
         // dim D' / 8 * g + j (D' = D rounded up to 32) of keys 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9, four j at a time: tiles 2 i, 2 i + 1 of 16 dims
         const int per = (D + 31) / 32 * 4;
-#pragma unroll
-        for (int i = 0; i < NT / 2; i++) {
-          if (4 * i >= per) continue;
-          uint32_t x[4], a0, a1, a2, a3, b0, b1, b2, b3;
-#pragma unroll
-          for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const uint32_t*>(vd + (2 * tig + (k & 1) + (k >> 1) * 8) * sh.v_pitch + g * per + 4 * i);
+        const unsigned char* const from = vd + 2 * tig * sh.v_pitch + g * per;
+        auto four = [&](int i, const uint32_t (&x)[4]) {
+          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
           widen4(__byte_perm(x[0], x[1], 0x5140), a0, a1);  // two keys' bytes side by side, then widened
           widen4(__byte_perm(x[0], x[1], 0x7362), b0, b1);
           widen4(__byte_perm(x[2], x[3], 0x5140), a2, a3);
@@ -333,6 +349,28 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
             mma_16x8(o[2 * i][t], a0, a1, a2, a3, p_lo[t][0], p_lo[t][1]);
             mma_16x8(o[2 * i + 1][t], b0, b1, b2, b3, p_hi[t][0], p_hi[t][1]);
             mma_16x8(o[2 * i + 1][t], b0, b1, b2, b3, p_lo[t][0], p_lo[t][1]);
+          }
+        };
+        if (NT >= 8 && per % 16 == 0) {  // 16 bytes of a key at once
+#pragma unroll
+          for (int i = 0; i < NT / 2; i += 4) {
+            if (4 * i >= per) continue;
+            uint4 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) y[k] = *reinterpret_cast<const uint4*>(from + ((k & 1) + (k >> 1) * 8) * sh.v_pitch + 4 * i);
+            four(i, {y[0].x, y[1].x, y[2].x, y[3].x});
+            four(i + 1, {y[0].y, y[1].y, y[2].y, y[3].y});
+            four(i + 2, {y[0].z, y[1].z, y[2].z, y[3].z});
+            four(i + 3, {y[0].w, y[1].w, y[2].w, y[3].w});
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NT / 2; i++) {
+            if (4 * i >= per) continue;
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = *reinterpret_cast<const uint32_t*>(from + ((k & 1) + (k >> 1) * 8) * sh.v_pitch + 4 * i);
+            four(i, x);
           }
         }
       }
