@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     mbar_init(smem_u32(&c.o_done), 1);
     for (int i = 0; i < kItems; i++) {
       mbar_init(smem_u32(&c.item_full[i]), 1);
-      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + 96 + (I8 ? kCopyThreads : 0));
+      mbar_init(smem_u32(&c.item_empty[i]), kSoftmaxThreads + 96 + kCopyThreads);
     }
     for (int i = 0; i < kMetaBlocks; i++) {
       mbar_init(smem_u32(&c.meta_full[i]), 1);
@@ -245,6 +245,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    if (!I8 && works) {
+    // bf16: by the copy engine, the units by turns to the warps (one warp's round of waiting for room and asking takes 0.3 us, which alone would
+    // bound the copies at 52 GB/s an SM; two warps reached 100, four 128 on all SMs at once).
+    // A run of R = box_rows keys to a lane: one box where all have a slot (they then follow one another) or none has (from outside the
+    // cache: zeros). Runs with some, and all keys where pages end anywhere (no box), go four keys to a lane.
+    const int own = warp - kSoftmaxWarps;
+    const int R = a.box_rows ? a.box_rows : kKeyBlock, log_r = 31 - __clz(R), runs = a.box_rows ? kKeyBlock >> log_r : 0, none = v.pages * v.page_size;
+    uint32_t unit0 = 0, block0 = 0;
+    for (uint32_t items = 0;; items++) {
+      const Item& w = take_item(items);
+      if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
+      const int n = w.b1 - w.b0, units = 2 * DC * n, head = w.head;
+      release_item(items);
+#pragma unroll 1
+      for (int i = (own - (int)unit0) & (kCopyWarps - 1); i < units; i += kCopyWarps) {
+        const int j = i + DC, b = j / (2 * DC), r0 = j - b * 2 * DC;  // as for int8: K(0), K(1), V(0), K(2), V(1), ...
+        const bool keys = r0 >= DC ? b == 0 : b < n;
+        const int block = keys ? b : b - 1, u = r0 >= DC ? r0 - DC : r0;
+        const uint32_t unit = unit0 + i, slot = unit % UNITS, bar = smem_u32(&c.full[slot]), dst = ring + slot * kUnit;
+        if (unit >= UNITS) wait(c.empty[slot], (unit / UNITS - 1) & 1, 301);
+        // (behind the wait for room: a warp passes over blocks, and a parity is told from the one before the last only while it is near)
+        const Meta& m = take_meta(block0 + block);
+        __syncwarp();
+        if (lane == 0) mbar_expect_tx(bar, kUnit);
+        // how many of this lane's run have a slot: whole words of the bits, or a part of one
+        const int at = min(lane << log_r, kKeyBlock - 1);
+        bool all_held = true, any_held = false;
+        if (R >= 32) {
+          for (int k = 0; k < R; k += 32) {
+            const uint32_t word = m.holds[min((at + k) >> 5, 3)];
+            all_held = all_held && word == 0xffffffffu;
+            any_held = any_held || word;
+          }
+        } else {
+          const uint32_t mask = (1u << R) - 1, word = m.holds[at >> 5] >> (at & 31) & mask;
+          all_held = word == mask;
+          any_held = word != 0;
+        }
+        const bool in_part = any_held && !all_held;
+        const uint32_t parts = runs ? __ballot_sync(0xffffffffu, lane < runs && in_part) : 0xffffffffu;
+        __syncwarp();
+        if (lane < runs && !in_part) tma_load_3d(dst + (lane << log_r) * 128, keys ? &maps.k : &maps.v, u * 64, head, all_held ? m.slot[at] : none, bar);
+        if (parts && (!runs || (parts >> (4 * lane >> log_r) & 1))) {
+          const int4 x = *reinterpret_cast<const int4*>(&m.slot[4 * lane]);  // this lane's four, by themselves
+          auto row = [&](int s) { return s < 0 ? -1 : s * v.n_kv + head; };
+          tma_gather4(dst + lane * 512, keys ? &maps.k_rows : &maps.v_rows, u * 64, row(x.x), row(x.y), row(x.z), row(x.w), bar);
+        }
+      }
+      unit0 += units;
+      block0 += n;
+    }
+    }
   } else if (warp >= kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ matrix instructions
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
@@ -300,12 +352,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
       blocks += n;
     }
     } else if (works && warp == kSoftmaxWarps + kCopyWarps + 2) {
-      // ---------------------------------------------- queries, and bf16 caches, by the copy engine: a lane asks for four rows of 128 bytes at once
-      uint32_t unit = 0, blocks = 0;
+      // ---------------------------------------------- queries, by the copy engine
       for (uint32_t items = 0;; items++) {
         const Item& w = take_item(items);
         if (__any_sync(0xffffffffu, gave_up || !w.tokens)) break;
-        const int n = w.b1 - w.b0, head = w.head, q_row = w.row0;
+        const int head = w.head, q_row = w.row0;
         release_item(items);
         if (items) wait(c.q_empty, (items - 1) & 1, 302);
         __syncwarp();
@@ -315,60 +366,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
 #pragma unroll 1
           for (int u = 0; u < DC; u++) tma_load_3d(q_smem + u * kUnit, &maps.q, u * 64, head * group, q_row, bar);
         }
-        if (I8) continue;
-        auto begin_unit = [&]() {
-          const uint32_t slot = unit % UNITS;
-          if (unit >= UNITS) wait(c.empty[slot], (unit / UNITS - 1) & 1, 301);
-          __syncwarp();
-          if (lane == 0) mbar_expect_tx(smem_u32(&c.full[slot]), kUnit);
-          __syncwarp();
-          unit++;
-          return slot;
-        };
-        // A run of R = box_rows keys to a lane: one box where all have a slot (they then follow one another) or none has (from outside the
-        // cache: zeros). Runs with some, and all keys where pages end anywhere (no box), go four keys to a lane.
-        const int R = a.box_rows ? a.box_rows : kKeyBlock, runs = a.box_rows ? kKeyBlock >> (31 - __clz(R)) : 0, none = v.pages * v.page_size;
-        auto copy_units = [&](const CUtensorMap* map, const CUtensorMap* rows, uint32_t block) {
-          const Meta& m = meta[block % kMetaBlocks];
-          const int at = min(lane * R, kKeyBlock - 1);
-          const int4 keys = *reinterpret_cast<const int4*>(&m.slot[4 * lane]);  // this lane's four, by themselves
-          // how many of this lane's run have a slot: whole words of the bits, or a part of one
-          bool all_held = true, any_held = false;
-          if (R >= 32) {
-            for (int i = 0; i < R; i += 32) {
-              const uint32_t word = m.holds[min((at + i) >> 5, 3)];
-              all_held = all_held && word == 0xffffffffu;
-              any_held = any_held || word;
-            }
-          } else {
-            const uint32_t mask = (1u << R) - 1, word = m.holds[at >> 5] >> (at & 31) & mask;
-            all_held = word == mask;
-            any_held = word != 0;
-          }
-          const bool in_part = runs ? any_held && !all_held : true;
-          const uint32_t parts = runs ? __ballot_sync(0xffffffffu, lane < runs && in_part) : 0xffffffffu;
-          const int run = all_held ? m.slot[at] : none;
-          const bool one_box = lane < runs && !in_part, four = runs ? parts >> (4 * lane >> (31 - __clz(R))) & 1 : true;
-          int r[4] = {keys.x, keys.y, keys.z, keys.w};
-#pragma unroll
-          for (int i = 0; i < 4; i++) r[i] = r[i] < 0 ? -1 : r[i] * v.n_kv + head;
-#pragma unroll 1
-          for (int u = 0; u < DC; u++) {
-            const uint32_t slot = begin_unit(), bar = smem_u32(&c.full[slot]), dst = ring + slot * kUnit;
-            if (one_box) tma_load_3d(dst + lane * R * 128, map, u * 64, head, run, bar);
-            if (four) tma_gather4(dst + lane * 512, rows, u * 64, r[0], r[1], r[2], r[3], bar);
-          }
-        };
-        for (int b = 0; b <= n; b++) {
-          if (b < n) {
-            take_meta(blocks);
-            __syncwarp();
-            copy_units(&maps.k, &maps.k_rows, blocks);
-          }
-          if (b > 0) copy_units(&maps.v, &maps.v_rows, blocks - 1);
-          blocks++;
-        }
-        blocks--;
       }
     } else if (works && warp == kSoftmaxWarps + kCopyWarps + 3) {
       // ---------------------------------------------- which keys, and where: four to a lane, a block's page ids asked for a block ahead
