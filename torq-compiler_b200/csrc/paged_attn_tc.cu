@@ -26,14 +26,18 @@ namespace {
 
 // four warpgroups: two for softmax, one that widens int8 caches, one with a warp each for matrix instructions, items and the copy engine; the
 // registers go where they are needed (of the 512 x 128 that a block starts with)
-constexpr int kSoftmaxWarps = 8, kCopyWarps = 4, kThreads = 512;
-constexpr int kCopyRegs = 104, kIssueRegs = 56;
-constexpr int kSoftmaxRegsI8 = 176, kSoftmaxRegs = 200;  // a bf16 cache's copies leave more
-static_assert(256 * kSoftmaxRegsI8 + 128 * kCopyRegs + 128 * kIssueRegs <= kThreads * 128, "register split, int8");
-static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreads * 128, "register split, bf16");
-constexpr int kCopyThreads = kCopyWarps * 32, kSoftmaxThreads = kSoftmaxWarps * 32;
+constexpr int kSoftmaxWarps = 8;
+template <bool I8>
+constexpr int kCopyWarpsOf = I8 ? 8 : 4;  // four widening warps took twice as long over a block as all else
+template <bool I8>
+constexpr int kThreadsOf = (kSoftmaxWarps + kCopyWarpsOf<I8> + 4) * 32;
+// a block starts with 128 (bf16) or 96 (int8) registers a thread
+constexpr int kSoftmaxRegs = 200, kSoftmaxRegsI8 = 136, kCopyRegsI8 = 64, kIssueRegs = 56;
+static_assert(256 * kSoftmaxRegsI8 + 256 * kCopyRegsI8 + 128 * kIssueRegs <= kThreadsOf<true> * 96, "register split, int8");
+static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreadsOf<false> * 128, "register split, bf16");
+constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
-constexpr int kMetaBlocks = 8, kItems = 4, kAhead = 4;
+constexpr int kMetaBlocks = 6, kItems = 4;
 using TileRowScratch = RowScratch<kSoftmaxThreads>;  // the plain row is computed by the softmax warps
 
 struct alignas(16) Meta {
@@ -102,14 +106,15 @@ struct TileMaps {
 };
 
 // DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
-template <int DC, int UNITS, bool I8>
-__global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+template <int DC, int UNITS, int AHEAD, bool I8>
+__global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+  constexpr int kCopyWarps = kCopyWarpsOf<I8>, kCopyThreads = kCopyWarps * 32, kThreads = kThreadsOf<I8>;
   extern __shared__ unsigned char smem_raw[];
   // [Q units][ring units] on 1024-byte boundaries, then the rest
   unsigned char* const base = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t q_smem = smem_u32(base), ring = q_smem + DC * kUnit;
   unsigned char* const raw = base + (DC + UNITS) * kUnit;  // int8 pieces on their way
-  Meta* const meta = reinterpret_cast<Meta*>(raw + (I8 ? kAhead * kUnit / 2 : 0));
+  Meta* const meta = reinterpret_cast<Meta*>(raw + (I8 ? AHEAD * kUnit / 2 : 0));
   TileRowScratch& plain = *reinterpret_cast<TileRowScratch*>(meta + kMetaBlocks);
   Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(TileRowScratch));
   int* const first_tile = reinterpret_cast<int*>(base);  // while the work is shared out: tiles in front of each sequence
@@ -186,12 +191,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
   const uint32_t o_tmem = tmem + 256;
   if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kCopyWarps) {
     // ------------------------------------------------ copies of int8 caches: widened on the way
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(I8 ? kCopyRegs : kIssueRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(I8 ? kCopyRegsI8 : kIssueRegs));
     if (I8 && works) {
-    // A thread has the same piece of 16 bytes of four rows of every unit: what it asks for lands in room of its own, kAhead units ahead of being
+    // A thread has the same piece of 16 bytes of two rows of every unit: what it asks for lands in room of its own, AHEAD units ahead of being
     // widened, so nothing but its own copies has to be waited for.
     const int t = tid - kSoftmaxThreads, piece = t & 3, row0 = t >> 2;
-    const uint32_t own = smem_u32(raw) + t * 64;
+    const uint32_t own = smem_u32(raw) + t * 32;
     const long long row_bytes = (long long)v.n_kv * D;
     uint32_t unit = 0, block0 = 0;
     for (uint32_t items = 0;; items++) {
@@ -208,38 +213,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           const Meta& m = take_meta(block0 + block);
           const char* const pages = (const char*)(keys ? a.k : a.vv) + head_bytes + u * 64;
           const bool in = u * 64 + piece * 16 < D;
-          int slot[4];
+          int slot[2];
 #pragma unroll
-          for (int k = 0; k < 4; k++) slot[k] = in ? m.slot[row0 + 32 * k] : -1;
-          const uint32_t dst = own + (i % kAhead) * (kUnit / 2);
+          for (int k = 0; k < 2; k++) slot[k] = in ? m.slot[row0 + 64 * k] : -1;
+          const uint32_t dst = own + (i % AHEAD) * (kUnit / 2);
 #pragma unroll
-          for (int k = 0; k < 4; k++) copy16(dst + k * 16, pages + max(slot[k], 0) * row_bytes, slot[k] >= 0);
+          for (int k = 0; k < 2; k++) copy16(dst + k * 16, pages + max(slot[k], 0) * row_bytes, slot[k] >= 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
 #pragma unroll 1
-      for (int i = 0; i < kAhead; i++) ask(i);
+      for (int i = 0; i < AHEAD; i++) ask(i);
 #pragma unroll 1
       for (int i = 0; i < units; i++, unit++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
         if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
-        const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128, from = own + (i % kAhead) * (kUnit / 2);
-        const uint32_t lo_at = ((2 * piece) ^ (row0 & 7)) << 4, hi_at = ((2 * piece + 1) ^ (row0 & 7)) << 4;  // a thread's rows are 32 apart
-        uint4 x[4];
+        const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128, from = own + (i % AHEAD) * (kUnit / 2);
+        const uint32_t lo_at = ((2 * piece) ^ (row0 & 7)) << 4, hi_at = ((2 * piece + 1) ^ (row0 & 7)) << 4;  // a thread's rows are 64 apart
+        uint4 x[2];
 #pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = lds128(from + k * 16);
+        for (int k = 0; k < 2; k++) x[k] = lds128(from + k * 16);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 2; k++) {
           const uint4 q = x[k];
           uint4 lo, hi;
           widen4(q.x, lo.x, lo.y); widen4(q.y, lo.z, lo.w);
           widen4(q.z, hi.x, hi.y); widen4(q.w, hi.z, hi.w);
-          sts128(dst + k * 4096 + lo_at, lo);
-          sts128(dst + k * 4096 + hi_at, hi);
+          sts128(dst + k * 8192 + lo_at, lo);
+          sts128(dst + k * 8192 + hi_at, hi);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(smem_u32(&c.full[unit % UNITS]));
-        ask(i + kAhead);
+        ask(i + AHEAD);
       }
       block0 += n;
     }
@@ -301,10 +306,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
     // ------------------------------------------------ matrix instructions
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     if (works && warp == kSoftmaxWarps + kCopyWarps) {
-    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row groups 1024 bytes apart, sm_100 descriptor, 128-byte swizzle
+    // operands of 128-byte rows, 8-row groups 1024 bytes apart, 128-byte swizzle; values as MN-major: 64 dims, then the next unit
+    auto desc = [](uint32_t at, uint32_t lead) {
+      return (uint64_t)(((at & 0x3FFFF) >> 4) | (lead >> 4 << 16)) | (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;
+    };
     const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kKeyBlock >> 3) << 17) | (8u << 24);
+    const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
     uint32_t unit = 0, blocks = 0;
-    auto lo_of = [](uint32_t at) { return ((at & 0x3FFFF) >> 4) | (64u << 16); };
     for (uint32_t items = 0;; items++) {
       const Item& w = take_item(items);
       const int n = w.b1 - w.b0;
@@ -318,32 +326,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           for (int u = 0; u < DC; u++) {
             wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
             tc_fence_after();
-            const uint32_t qa = lo_of(q_smem + u * kUnit), kb = lo_of(ring + (unit % UNITS) * kUnit);
-            const int steps = min(4, (D - u * 64) >> 4);
-            for (int k = 0; k < steps; k++) mma_f16_elect(s_tmem, qa + 2 * k, hi, kb + 2 * k, hi, idesc_s, (u | k) ? 1u : 0u);
+            const uint64_t qa = desc(q_smem + u * kUnit, 16), kb = desc(ring + (unit % UNITS) * kUnit, 16);
+            if ((u + 1) * 64 <= D) {
+              mma_f16x4_elect(s_tmem, qa, kb, idesc_s, u ? 1u : 0u);
+            } else {
+#pragma unroll 1
+              for (int k = 0; k < ((D - u * 64) >> 4); k++) mma_f16_elect(s_tmem, qa + 2 * k, kb + 2 * k, idesc_s, (u | k) ? 1u : 0u);
+            }
             mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
             unit++;
           }
           mma_commit_elect(smem_u32(&c.s_full[(blocks + b) & 1]));
           if (b == n - 1) mma_commit_elect(smem_u32(&c.q_empty));
         }
-        if (b > 0) {  // sums of block b - 1
+        if (b > 0) {  // sums of block b - 1: all dims in one instruction (the ring holds a block's units one behind another)
           const uint32_t g = blocks + b - 1, p_tmem = tmem + (g & 1) * 128;
           wait(c.p_ready[g & 1], (g >> 1) & 1, 305);
-          tc_fence_after();
 #pragma unroll 1
-          for (int u = 0; u < DC; u++) {
-            wait(c.full[unit % UNITS], (unit / UNITS) & 1, 306);
-            tc_fence_after();
-            const int width = min(64, D - u * 64);
-            const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(width >> 3) << 17) | (8u << 24);
-            const uint32_t vb = lo_of(ring + (unit % UNITS) * kUnit);
-#pragma unroll
-            for (int k = 0; k < 8; k++)  // keys 0..63 of P lie in columns 0..31, keys 64..127 in columns 64..95
-              mma_f16_ts_elect(o_tmem + u * 64, p_tmem + (k < 4 ? k * 8 : 64 + (k - 4) * 8), vb + k * (2048 >> 4), hi, idesc_o, (b > 1 || k > 0) ? 1u : 0u);
-            mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
-            unit++;
-          }
+          for (int u = 0; u < DC; u++) wait(c.full[(unit + u) % UNITS], ((unit + u) / UNITS) & 1, 306);
+          tc_fence_after();
+          const uint64_t vb = desc(ring + (unit % UNITS) * kUnit, kUnit);
+          // keys 0..63 of P lie in columns 0..31, keys 64..127 in columns 64..95
+          mma_f16x4_ts_elect(o_tmem, p_tmem, vb, 2048 >> 4, idesc_o, b > 1 ? 1u : 0u);
+          mma_f16x4_ts_elect(o_tmem, p_tmem + 64, vb + 4 * (2048 >> 4), 2048 >> 4, idesc_o, 1u);
+#pragma unroll 1
+          for (int u = 0; u < DC; u++, unit++) mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
           mma_commit_elect(smem_u32(&c.pv_done));
           mma_commit_elect(smem_u32(&c.meta_empty[g % kMetaBlocks]));
           if (b == n) mma_commit_elect(smem_u32(&c.o_done));
@@ -459,13 +466,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_paged_tile_kernel(const Attn
           mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
           continue;
         }
-        wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
-        tc_fence_after();
         const Meta& mt = take_meta(blocks);
         const int key0 = mt.key0 + half * 64;
         // whether some row of the tile does not see some key of this half
         const bool partial = (mt.holds[half * 2] & mt.holds[half * 2 + 1]) != 0xffffffffu || key0 + 63 > first_pos ||
                              (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
+        wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
+        tc_fence_after();
         // 32 scores, of columns 32 k on: scaled (int8), and those of keys this row does not see at -inf. The loops over them stay rolled up: a
         // processor's four quarters each run this beside other roles, and what does not fit their instruction buffers is waited for.
         auto scores = [&](int k, uint32_t (&s)[32]) {
@@ -675,12 +682,13 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t rows, int D) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DC, int UNITS, bool I8>
+template <int DC, int UNITS, int AHEAD, bool I8>
 cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
-  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? kAhead * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(TileRowScratch) + (int)sizeof(Control);
+  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? AHEAD * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(TileRowScratch) + (int)sizeof(Control);
   static_assert(smem <= 227 * 1024, "shared memory");
+  static_assert(UNITS % DC == 0, "a block's units lie one behind another");
   static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
-  auto kernel = attn_paged_tile_kernel<DC, UNITS, I8>;
+  auto kernel = attn_paged_tile_kernel<DC, UNITS, AHEAD, I8>;
   static std::atomic<unsigned long long> attr_done;
   if (first_use_on_device(attr_done)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -694,7 +702,7 @@ cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
   if (!I8 && (!encode_heads(&m.k, a.k, slots, a.v.n_kv, a.v.D, 1, run) || !encode_heads(&m.v, a.vv, slots, a.v.n_kv, a.v.D, 1, run) ||
               !encode_rows(&m.k_rows, a.k, slots * a.v.n_kv, a.v.D) || !encode_rows(&m.v_rows, a.vv, slots * a.v.n_kv, a.v.D)))
     return cudaErrorInvalidValue;
-  return launch_dependent(kernel, dim3(a.grid), dim3(kThreads), smem, stream, a, m);
+  return launch_dependent(kernel, dim3(a.grid), dim3(kThreadsOf<I8>), smem, stream, a, m);
 }
 
 }  // namespace
@@ -705,10 +713,10 @@ cudaError_t launch_attn_paged_tile(AttnPagedArgs a, cudaStream_t stream) {
   if (a.box_rows < 8) a.box_rows = 0;
   const int units = (a.v.D + 63) / 64;
   if (a.scales)
-    return units == 1 ? run_tile<1, 8, true>(a, stream) : units == 2 ? run_tile<2, 8, true>(a, stream)
-         : units == 3 ? run_tile<3, 6, true>(a, stream) : run_tile<4, 6, true>(a, stream);
-  return units == 1 ? run_tile<1, 8, false>(a, stream) : units == 2 ? run_tile<2, 8, false>(a, stream)
-       : units == 3 ? run_tile<3, 8, false>(a, stream) : run_tile<4, 8, false>(a, stream);
+    return units == 1 ? run_tile<1, 8, 4, true>(a, stream) : units == 2 ? run_tile<2, 8, 4, true>(a, stream)
+         : units == 3 ? run_tile<3, 6, 4, true>(a, stream) : run_tile<4, 8, 2, true>(a, stream);
+  return units == 1 ? run_tile<1, 8, 1, false>(a, stream) : units == 2 ? run_tile<2, 8, 1, false>(a, stream)
+       : units == 3 ? run_tile<3, 6, 1, false>(a, stream) : run_tile<4, 8, 1, false>(a, stream);
 }
 
 }  // namespace tb200
