@@ -164,6 +164,19 @@ def test_attention_scores_of_any_size(device):
     check(device, b, q=to_bf16(q))
 
 
+@pytest.mark.parametrize("max_new", [0, 1])
+@pytest.mark.parametrize("heads", [(4, 1, 256), (8, 2, 64), (3, 3, 96)])
+def test_attention_scales_that_the_cache_was_given(device, heads, max_new):
+    """Scales are the caller's: zeros over integers that are none, negative ones, ones whose products underflow, among keys that are hidden."""
+    n_q, n_kv, d = heads
+    b = Batch([1, 1] if max_new else [90, 5], [300, 40], n_q=n_q, n_kv=n_kv, d=d, page=16, i8=True)
+    kind = b.rng.integers(0, 6, b.scales.shape)
+    b.scales = np.where(kind == 0, 0.0, np.where(kind == 1, -b.scales, np.where(kind == 2, 1e-44, b.scales))).astype(np.float32)
+    check(device, b, window=100, sinks=4, max_new=max_new)
+    b.scales[...] = 0.0  # every key the same, every value zero
+    assert not from_bf16(check(device, b, max_new=max_new)[:int(b.row_start[-1])]).any()
+
+
 @pytest.mark.parametrize("i8", [False, True])
 def test_attention_repeats_bit_by_bit(device, i8):
     b = Batch([1] * 7 + [60], [900, 3, 50, 2000, 128, 7, 64, 1500], n_q=8, n_kv=2, d=128, page=16, i8=i8)

@@ -32,7 +32,7 @@ constexpr int kCopyWarpsOf = I8 ? 8 : 4;  // four widening warps took twice as l
 template <bool I8>
 constexpr int kThreadsOf = (kSoftmaxWarps + kCopyWarpsOf<I8> + 4) * 32;
 // a block starts with 128 (bf16) or 96 (int8) registers a thread
-constexpr int kSoftmaxRegs = 200, kSoftmaxRegsI8 = 136, kCopyRegsI8 = 64, kIssueRegs = 56;
+constexpr int kSoftmaxRegs = 200, kSoftmaxRegsI8 = 144, kCopyRegsI8 = 64, kIssueRegs = 56;
 static_assert(256 * kSoftmaxRegsI8 + 256 * kCopyRegsI8 + 128 * kIssueRegs <= kThreadsOf<true> * 96, "register split, int8");
 static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreadsOf<false> * 128, "register split, bf16");
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
@@ -108,6 +108,7 @@ struct TileMaps {
 // DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
 template <int DC, int UNITS, int AHEAD, bool I8>
 __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+  constexpr int GROUPS = UNITS / DC;  // a block's keys, or its values, lie one behind another: a group
   constexpr int kCopyWarps = kCopyWarpsOf<I8>, kCopyThreads = kCopyWarps * 32, kThreads = kThreadsOf<I8>;
   extern __shared__ unsigned char smem_raw[];
   // [Q units][ring units] on 1024-byte boundaries, then the rest
@@ -127,13 +128,13 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
-    for (int i = 0; i < UNITS; i++) {
-      mbar_init(smem_u32(&c.full[i]), I8 ? kCopyThreads : 1);
+    for (int i = 0; i < GROUPS; i++) {
+      mbar_init(smem_u32(&c.full[i]), I8 ? kCopyWarps * DC : DC);
       mbar_init(smem_u32(&c.empty[i]), 1);
     }
     for (int i = 0; i < 2; i++) {  // a softmax warp may be one block ahead of another: a barrier for each buffer
       mbar_init(smem_u32(&c.s_full[i]), 1);
-      mbar_init(smem_u32(&c.p_ready[i]), kSoftmaxThreads);
+      mbar_init(smem_u32(&c.p_ready[i]), kSoftmaxWarps);
     }
     mbar_init(smem_u32(&c.pv_done), 1);
     mbar_init(smem_u32(&c.o_done), 1);
@@ -227,7 +228,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
 #pragma unroll 1
       for (int i = 0; i < units; i++, unit++) {
         asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
-        if (unit >= UNITS) wait(c.empty[unit % UNITS], (unit / UNITS - 1) & 1, 301);
+        const uint32_t part = unit / DC;
+        if (part >= GROUPS) wait(c.empty[part % GROUPS], (part / GROUPS - 1) & 1, 301);
         const uint32_t dst = ring + (unit % UNITS) * kUnit + row0 * 128, from = own + (i % AHEAD) * (kUnit / 2);
         const uint32_t lo_at = ((2 * piece) ^ (row0 & 7)) << 4, hi_at = ((2 * piece + 1) ^ (row0 & 7)) << 4;  // a thread's rows are 64 apart
         uint4 x[2];
@@ -243,7 +245,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
           sts128(dst + k * 8192 + hi_at, hi);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(smem_u32(&c.full[unit % UNITS]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c.full[part % GROUPS]));
         ask(i + AHEAD);
       }
       block0 += n;
@@ -268,8 +271,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
         const int j = i + DC, b = j / (2 * DC), r0 = j - b * 2 * DC;  // as for int8: K(0), K(1), V(0), K(2), V(1), ...
         const bool keys = r0 >= DC ? b == 0 : b < n;
         const int block = keys ? b : b - 1, u = r0 >= DC ? r0 - DC : r0;
-        const uint32_t unit = unit0 + i, slot = unit % UNITS, bar = smem_u32(&c.full[slot]), dst = ring + slot * kUnit;
-        if (unit >= UNITS) wait(c.empty[slot], (unit / UNITS - 1) & 1, 301);
+        const uint32_t unit = unit0 + i, part = unit / DC, bar = smem_u32(&c.full[part % GROUPS]), dst = ring + unit % UNITS * kUnit;
+        if (part >= GROUPS) wait(c.empty[part % GROUPS], (part / GROUPS - 1) & 1, 301);
         // (behind the wait for room: a warp passes over blocks, and a parity is told from the one before the last only while it is near)
         const Meta& m = take_meta(block0 + block);
         __syncwarp();
@@ -312,7 +315,20 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
     };
     const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kKeyBlock >> 3) << 17) | (8u << 24);
     const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-    uint32_t unit = 0, blocks = 0;
+    // (what bounds this role is its own instructions, one behind another: descriptors and phases are stepped, not worked out)
+    const uint64_t q0 = desc(q_smem, 16), k0 = desc(ring, 16), v0 = desc(ring, kUnit);
+    uint32_t group_at = 0, turn = 0, blocks = 0;  // the group to be used next, its phase
+    auto take_group = [&](int code) {
+      wait(c.full[group_at], turn, code);
+      tc_fence_after();
+    };
+    auto release_group = [&]() {
+      mma_commit_elect(smem_u32(&c.empty[group_at]));
+      if (++group_at == GROUPS) {
+        group_at = 0;
+        turn ^= 1;
+      }
+    };
     for (uint32_t items = 0;; items++) {
       const Item& w = take_item(items);
       const int n = w.b1 - w.b0;
@@ -322,36 +338,32 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
       for (int b = 0; b <= n; b++) {
         if (b < n) {  // scores of block b
           const uint32_t s_tmem = tmem + ((blocks + b) & 1) * 128;
+          const uint64_t kb = k0 + group_at * (DC * (kUnit >> 4));
+          take_group(304);
+          if (D == DC * 64) {
+#pragma unroll
+            for (int u = 0; u < DC; u++) mma_f16x4_elect(s_tmem, q0 + u * (kUnit >> 4), kb + u * (kUnit >> 4), idesc_s, u ? 1u : 0u);
+          } else {
 #pragma unroll 1
-          for (int u = 0; u < DC; u++) {
-            wait(c.full[unit % UNITS], (unit / UNITS) & 1, 304);
-            tc_fence_after();
-            const uint64_t qa = desc(q_smem + u * kUnit, 16), kb = desc(ring + (unit % UNITS) * kUnit, 16);
-            if ((u + 1) * 64 <= D) {
-              mma_f16x4_elect(s_tmem, qa, kb, idesc_s, u ? 1u : 0u);
-            } else {
-#pragma unroll 1
-              for (int k = 0; k < ((D - u * 64) >> 4); k++) mma_f16_elect(s_tmem, qa + 2 * k, kb + 2 * k, idesc_s, (u | k) ? 1u : 0u);
+            for (int k = 0; k < (D >> 4); k++) {
+              const uint32_t at = (k >> 2) * (kUnit >> 4) + (k & 3) * 2;
+              mma_f16_elect(s_tmem, q0 + at, kb + at, idesc_s, k ? 1u : 0u);
             }
-            mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
-            unit++;
           }
           mma_commit_elect(smem_u32(&c.s_full[(blocks + b) & 1]));
+          release_group();
           if (b == n - 1) mma_commit_elect(smem_u32(&c.q_empty));
         }
-        if (b > 0) {  // sums of block b - 1: all dims in one instruction (the ring holds a block's units one behind another)
+        if (b > 0) {  // sums of block b - 1: all dims in one instruction
           const uint32_t g = blocks + b - 1, p_tmem = tmem + (g & 1) * 128;
+          const uint64_t vb = v0 + group_at * (DC * (kUnit >> 4));
           wait(c.p_ready[g & 1], (g >> 1) & 1, 305);
-#pragma unroll 1
-          for (int u = 0; u < DC; u++) wait(c.full[(unit + u) % UNITS], ((unit + u) / UNITS) & 1, 306);
-          tc_fence_after();
-          const uint64_t vb = desc(ring + (unit % UNITS) * kUnit, kUnit);
+          take_group(306);
           // keys 0..63 of P lie in columns 0..31, keys 64..127 in columns 64..95
           mma_f16x4_ts_elect(o_tmem, p_tmem, vb, 2048 >> 4, idesc_o, b > 1 ? 1u : 0u);
           mma_f16x4_ts_elect(o_tmem, p_tmem + 64, vb + 4 * (2048 >> 4), 2048 >> 4, idesc_o, 1u);
-#pragma unroll 1
-          for (int u = 0; u < DC; u++, unit++) mma_commit_elect(smem_u32(&c.empty[unit % UNITS]));
           mma_commit_elect(smem_u32(&c.pv_done));
+          release_group();
           mma_commit_elect(smem_u32(&c.meta_empty[g % kMetaBlocks]));
           if (b == n) mma_commit_elect(smem_u32(&c.o_done));
         }
@@ -405,7 +417,10 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
             for (int i = 0; i < 4; i++) {
               const float* sc = a.scales + (long long)max(slot[i], 0) * 2 * v.n_kv + head;
               const float k1 = __ldg(sc), v1 = __ldg(sc + v.n_kv);
-              ks[i] = slot[i] < 0 ? 0.f : k1;
+              // what makes a key's scores units of log2; it must not be zero where it meets a hidden key's -inf, and the smallest
+              // number in its place leaves every finite score below 2^-20
+              const float k2 = k1 * (a.scale * 1.4426950408889634f);
+              ks[i] = slot[i] < 0 || k2 == 0.f ? __int_as_float(1) : k2;
               vs[i] = slot[i] < 0 ? 0.f : v1;
             }
           }
@@ -458,12 +473,13 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
       const int pos = (int)min((long long)first_pos + min(tok, tokens - 1), 0x7fffffffll);
       const int last_pos = (int)min((long long)first_pos + tokens - 1, 0x7fffffffll);
       const int near = a.window ? max(0, pos - a.window + 1) : 0;  // this row sees keys [near, pos] and those in front of sinks
-      float m = -INFINITY, base = 0.f, sum = 0.f;  // base: m scaled, what the exponents are taken from
+      float m = -INFINITY, base = 0.f, sum = 0.f;  // base: what the exponents are taken from, m or (before there is one) zero
       for (int b = 0; b < n; b++, blocks++) {
         const uint32_t s_tmem = tmem + lanes + (blocks & 1) * 128 + half * 64;
         if (!warp_used) {  // rows of nobody: P keeps what it holds, and so does O
           wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
-          mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
           continue;
         }
         const Meta& mt = take_meta(blocks);
@@ -473,23 +489,11 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
                              (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
         wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
         tc_fence_after();
-        // 32 scores, of columns 32 k on: scaled (int8), and those of keys this row does not see at -inf. The loops over them stay rolled up: a
+        // 32 scores, of columns 32 k on, those of keys this row does not see at -inf. The loops over them stay rolled up: a
         // processor's four quarters each run this beside other roles, and what does not fit their instruction buffers is waited for.
         auto scores = [&](int k, uint32_t (&s)[32]) {
           tmem_ld32_issue(s_tmem + 32 * k, s);
           tmem_ld_wait32(s);
-          if (I8) {
-            const float* scale = mt.k_scale + half * 64 + 32 * k;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(scale + i);
-              float f[4];
-              unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), pack_f32(x.x, x.y)), f[0], f[1]);
-              unpack_f32(mul_f32x2(pack_f32(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), pack_f32(x.z, x.w)), f[2], f[3]);
-#pragma unroll
-              for (int j = 0; j < 4; j++) s[i + j] = __float_as_uint(f[j]);
-            }
-          }
           if (partial) {
             // bits of the keys this row sees: not behind its position, inside the window or among the first, and held
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
@@ -498,6 +502,12 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
 #pragma unroll
             for (int i = 0; i < 32; i++) s[i] = see >> i & 1 ? s[i] : 0xff800000u;
           }
+        };
+        // four scores in units of log2
+        auto scale4 = [&](const uint32_t (&s)[32], int i, const float* scale, float (&x)[4]) {
+          const float4 by = I8 ? *reinterpret_cast<const float4*>(scale) : make_float4(cexp, cexp, cexp, cexp);
+          x[0] = __uint_as_float(s[i]) * by.x; x[1] = __uint_as_float(s[i + 1]) * by.y;
+          x[2] = __uint_as_float(s[i + 2]) * by.z; x[3] = __uint_as_float(s[i + 3]) * by.w;
         };
         float part;
         uint32_t p[32];  // two weights each; they take the place of the scores once these are not needed again
@@ -510,18 +520,22 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
               scores(k, s);
               float tops[2] = {top, -INFINITY};
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+              for (int i = 0; i < 32; i += 4) {
+                float x[4];
+                scale4(s, i, mt.k_scale + half * 64 + 32 * k + i, x);
+                tops[0] = max3(tops[0], x[0], x[1]);
+                tops[1] = max3(tops[1], x[2], x[3]);
+              }
               top = fmaxf(tops[0], tops[1]);
             }
             c.top[blocks & 1][half][row] = top;
             named_sync(1 + (warp & 3), 64);
             top = fmaxf(top, c.top[blocks & 1][half ^ 1][row]);
             float keep = 1.f;
-            if (top > m && (b == 0 || !((top - m) * cexp <= 8.f))) {
-              const float to = top * cexp;
-              keep = m == -INFINITY ? 0.f : exp2_fast(base - to);
+            if (top > m && (b == 0 || !(top - m <= 8.f))) {
+              keep = m == -INFINITY ? 0.f : exp2_fast(m - top);
               m = top;
-              base = to;
+              base = top;
             }
             if (b > 0) {
               sum *= keep;
@@ -549,18 +563,24 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
             uint32_t s[32];
             scores(k, s);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float x, y;
-              unpack_f32(fma_f32x2(pack_f32(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, base2), x, y);
-              most = max3(most, x, y);
-              unsigned long long e = pack_f32(exp2_fast(x), exp2_fast(y));
-              parts2[i >> 1 & 1] = add_f32x2(parts2[i >> 1 & 1], e);
+            for (int i = 0; i < 32; i += 4) {
+              unsigned long long ks[2] = {scale2, scale2}, vs[2];
               if (I8) {
-                const float2 vs = *reinterpret_cast<const float2*>(mt.v_scale + half * 64 + 32 * k + i);
-                e = mul_f32x2(e, pack_f32(vs.x, vs.y));
+                const float4 x = *reinterpret_cast<const float4*>(mt.k_scale + half * 64 + 32 * k + i), y = *reinterpret_cast<const float4*>(mt.v_scale + half * 64 + 32 * k + i);
+                ks[0] = pack_f32(x.x, x.y); ks[1] = pack_f32(x.z, x.w);
+                vs[0] = pack_f32(y.x, y.y); vs[1] = pack_f32(y.z, y.w);
               }
-              unpack_f32(e, x, y);
-              p[16 * k + (i >> 1)] = pack_bf16(x, y);
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                float x, y;
+                unpack_f32(fma_f32x2(pack_f32(__uint_as_float(s[i + 2 * j]), __uint_as_float(s[i + 2 * j + 1])), ks[j], base2), x, y);
+                most = max3(most, x, y);
+                unsigned long long e = pack_f32(exp2_fast(x), exp2_fast(y));
+                parts2[j] = add_f32x2(parts2[j], e);
+                if (I8) e = mul_f32x2(e, vs[j]);
+                unpack_f32(e, x, y);
+                p[16 * k + (i >> 1) + j] = pack_bf16(x, y);
+              }
             }
           }
           {
@@ -577,7 +597,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
         tmem_st32(s_tmem, p);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c.p_ready[blocks & 1]));
       }
       // ---- the item's rows: finished, or left for whoever finishes the tile
       wait(c.o_done, items & 1, 309);
