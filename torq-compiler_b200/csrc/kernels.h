@@ -288,6 +288,16 @@ bool gemv_w8_splits_fit(int B, int N, int K, int splits);
 // y bf16, or fp32 when y_f32
 void launch_gemv_w8(const uint16_t* x, const int8_t* W, const uint16_t* scale, void* y, int y_f32, float* scratch, int B,
                     int N, int K, int splits, cudaStream_t stream);
+// products of more than 32 rows on the tensor cores (linear_rows.cu): addresses 16-byte aligned, K a multiple of 16
+struct LinearRowsArgs {
+  const uint16_t* x;      // [rows][K]
+  const int8_t* w;        // [N][K]
+  const uint16_t* scale;  // [N]
+  void* y;                // [rows][N], bf16 or fp32
+  int y_f32, rows, N, K;
+  int* status;
+};
+cudaError_t launch_linear_rows(const LinearRowsArgs& a, int sms, cudaStream_t stream);
 void launch_rope_kv(const uint16_t* qkv, const int32_t* pos, const uint16_t* qw, const uint16_t* kw, uint16_t* q_out,
                     uint16_t* kcache, uint16_t* vcache, int B, int n_q, int n_kv, int D, int T, float theta, float eps,
                     cudaStream_t stream);

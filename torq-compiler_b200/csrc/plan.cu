@@ -2162,18 +2162,14 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
         size_t w_off, s_off;
         if (!b.add_raw_const(op.weights, (size_t)N * K, "weights", i, w_off)) return b.status;
         if (!b.add_raw_const(op.bias, (size_t)N * 2, "scales", i, s_off)) return b.status;
-        if (B > 32) {  // the rows of a chunk, 32 at a time
-          const int splits = op.i0 > 0 ? op.i0 : gemv_w8_splits(32, N, K);
-          if (!gemv_w8_splits_fit(32, N, K, splits))
-            return b.fail(TB200_OUT_OF_RANGE, "op %d: %d K slices leave a slice longer than the tensor-core gemv_w8 can stage", i, splits);
-          scratch_need = std::max(scratch_need, gemv_w8_scratch_bytes(32, N, splits));
-          Loc lx = loc(op.in0), lo = loc(op.out0);
-          step.kernel_name = "gemv_w8_rows";
-          step.launches = (B + 31) / 32 * (splits > 1 ? 2 : 1);
+        if (B > 32) {  // the rows of a chunk; K slices are asked for where rows are few
+          const Loc lx = loc(op.in0), lo = loc(op.out0);
+          const int sms = current_sm_count();
+          step.kernel_name = "linear_rows";
           step.launch = [=](const ExecContext& c) {
-            for (int r = 0; r < B; r += 32)
-              launch_gemv_w8((const uint16_t*)lx.resolve(c) + (size_t)r * K, (const int8_t*)(c.consts + w_off), (const uint16_t*)(c.consts + s_off),
-                             (char*)lo.resolve(c) + (size_t)r * N * (y_f32 ? 4 : 2), y_f32, (float*)c.scratch, std::min(32, B - r), N, K, splits, c.stream);
+            const LinearRowsArgs k{(const uint16_t*)lx.resolve(c), (const int8_t*)(c.consts + w_off), (const uint16_t*)(c.consts + s_off),
+                                   lo.resolve(c), y_f32, B, N, K, c.status};
+            report(launch_linear_rows(k, sms, c.stream), c);
           };
           break;
         }
