@@ -382,8 +382,9 @@ struct ReadPagedArgs {
   const float* scales;
   uint16_t* k_out;  // [rows][n_kv * D]
   uint16_t* v_out;
+  int per;          // rows a warp takes (filled by the launcher)
 };
-cudaError_t launch_kv_read_paged(const ReadPagedArgs& a, cudaStream_t stream);
+cudaError_t launch_kv_read_paged(ReadPagedArgs a, cudaStream_t stream);
 // A tile that several blocks of the grid share, as the first of them writes it down: rows row0 .. of the chunk, `used` of them times query heads
 struct AttnJoin {
   int parts;  // 0: this block begins no such tile
