@@ -4,6 +4,7 @@
 #include "dependent_launch.cuh"
 #include "kernels.h"
 #include "paged.cuh"
+#include "widen.cuh"
 
 namespace tb200 {
 
@@ -44,66 +45,79 @@ __device__ __forceinline__ int sequence_from(const PagedView& v, int s, int row)
 // with scale zero; one that holds an infinity or a NaN gets scale NaN and reads back as NaN.
 // The angle of a far position needs more than fp32: position * turns[i] with turns[i] = theta^(-2i / D) / 2 pi as a 64-bit fraction of a turn,
 // whose wrap-around is the reduction to one turn; its upper 32 bits go to sincospi.
-// L lanes hold a head (L the power of two from D / 16 on), eight neighbouring values of each half to a lane, so that every access has 16
-// bytes; a group of L lanes takes `per` heads of one row, one after another, so that a row's angles are worked out once for them, and asks
-// for the next head before it works on one.
+// What bounds it: memory, once its instructions are few enough (an int8 cache and norms take the most of them). L lanes hold a head (L the
+// power of two from D / 16 on), eight neighbouring values of each half to a lane, so that every access has 16 bytes. A warp takes the same
+// `per` heads of 32 / L rows one after another: its branches are then the same for all lanes, a row's angles and the norm's weights are
+// fetched once for several heads, and four heads are on their way while one is worked on.
+constexpr int kAhead = 4;
 template <int L>
-__global__ void __launch_bounds__(256) rope_kv_paged_kernel(const RopePagedArgs a) {
+__global__ void __launch_bounds__(128) rope_kv_paged_kernel(const RopePagedArgs a) {
   const PagedView& v = a.v;
   const int lane = threadIdx.x & 31, sub = lane % L, half = v.D >> 1;
   const bool active = sub * 8 < half;
   grid_dependency_wait();
   grid_dependency_release();
   const int heads = a.n_q + 2 * v.n_kv, groups = (heads + a.per - 1) / a.per;
-  const long long item = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
-  const int row = (int)min(item / groups, 0x7fffffffll), h0 = (int)(item % groups) * a.per, h1 = min(h0 + a.per, heads);
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), first = unit / groups * (32 / L);
+  if (first >= v.rows) return;
+  const int h0 = (int)(unit % groups) * a.per, h1 = min(h0 + a.per, heads);
+  const int row = (int)first + lane / L;
   const uint16_t* const src = a.qkv + (long long)row * heads * v.D + sub * 8;
-  uint4 next_a = make_uint4(0, 0, 0, 0), next_b = next_a;
+  // heads on their way: a lane's pieces land in places of its own, so only its own copies are waited for
+  __shared__ uint4 ring[kAhead][2][128];
+  const bool reads = active && row < v.rows;
   auto ask = [&](int h) {
-    if (active && row < v.rows && h < h1) {
-      next_a = __ldg(reinterpret_cast<const uint4*>(src + h * v.D));
-      next_b = __ldg(reinterpret_cast<const uint4*>(src + h * v.D + half));
+    if (h < h1) {
+      const uint16_t* const from = reads ? src + h * v.D : a.qkv;
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(&ring[(h - h0) % kAhead][0][threadIdx.x]);
+      copy16(to, from, reads);
+      copy16(to + sizeof(ring[0][0]), reads ? from + half : from, reads);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  ask(h0);
-  // the items of a warp may lie in several rows: the warp looks for the first one's sequence, and each goes on from there
-  const int first = (int)min((item - lane / L) / groups, (long long)v.rows - 1);
-  const int seq = sequence_from(v, sequence_of_row(v, first), min(row, v.rows - 1));
+#pragma unroll
+  for (int i = 0; i < kAhead; i++) ask(h0 + i);
+  const int seq = sequence_from(v, sequence_of_row(v, (int)first), min(row, v.rows - 1));
   const int pos = row < v.rows ? row_position(v, seq, row) : -1;
   const long long slot = pos >= 0 ? slot_of(v, seq, pos) : -1;
+  const bool on = active && pos >= 0;
   float cs[8], sn[8];
+  if (h0 < a.n_q + v.n_kv) {
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const int top = active ? (int)(((unsigned long long)(unsigned)max(pos, 0) * __ldg(a.turns + sub * 8 + j)) >> 32) : 0;
-    sincospif((float)top * 4.6566128730773926e-10f, &sn[j], &cs[j]);  // 2^-31: a turn is 2 in units of pi
+    for (int j = 0; j < 8; j++) {
+      const int top = active ? (int)(((unsigned long long)(unsigned)max(pos, 0) * __ldg(a.turns + sub * 8 + j)) >> 32) : 0;
+      sincospif((float)top * 4.6566128730773926e-10f, &sn[j], &cs[j]);  // 2^-31: a turn is 2 in units of pi
+    }
   }
-  for (int i = 0; i < a.per; i++) {  // every lane of the warp stays: the sums below are the warp's
-    const int h = h0 + i;
-    const bool on = active && pos >= 0 && h < h1;
+  uint4 w_a = make_uint4(0, 0, 0, 0), w_b = w_a;  // the norm's weights
+  for (int h = h0; h < h1; h++) {
     const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + v.n_kv;
     float xa[8], xb[8];
-    unpack(next_a, xa);
-    unpack(next_b, xb);
-    ask(h + 1);
-    if (a.norms) {
-      float ss = 0.f;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    unpack(ring[(h - h0) % kAhead][0][threadIdx.x], xa);
+    unpack(ring[(h - h0) % kAhead][1][threadIdx.x], xb);
+    ask(h + kAhead);
+    if (is_q || is_k) {
+      if (a.norms) {
+        if (active && (h == h0 || h == a.n_q)) {
+          const uint16_t* w = a.norms + (is_q ? 0 : v.D) + sub * 8;
+          w_a = __ldg(reinterpret_cast<const uint4*>(w));
+          w_b = __ldg(reinterpret_cast<const uint4*>(w + half));
+        }
+        float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; j++) ss += xa[j] * xa[j] + xb[j] * xb[j];
-      ss = group_sum<L>(ss);
-      if (on && (is_q || is_k)) {
+        for (int j = 0; j < 8; j++) ss += xa[j] * xa[j] + xb[j] * xb[j];
+        ss = group_sum<L>(ss);
         const float inv = rsqrtf(ss / (float)v.D + a.eps);
-        const uint16_t* w = a.norms + (is_q ? 0 : v.D) + sub * 8;
         float wa[8], wb[8];
-        unpack(__ldg(reinterpret_cast<const uint4*>(w)), wa);
-        unpack(__ldg(reinterpret_cast<const uint4*>(w + half)), wb);
+        unpack(w_a, wa);
+        unpack(w_b, wb);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           xa[j] = xa[j] * inv * (1.0f + wa[j]);
           xb[j] = xb[j] * inv * (1.0f + wb[j]);
         }
       }
-    }
-    if (is_q || is_k) {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const float p = xa[j], q = xb[j];
@@ -111,42 +125,40 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const RopePagedArgs 
         xb[j] = q * cs[j] + p * sn[j];
       }
     }
-    uint32_t top = 0;  // bits of the largest magnitude; those of a NaN are above an infinity's, and these above every number's
-    if (a.scales) {
-      if (on) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, max(__float_as_uint(fabsf(xa[j])), __float_as_uint(fabsf(xb[j]))));
-      }
-      top = group_max<L>(top);
-    }
-    if (!on) continue;
     if (is_q) {
+      if (!on) continue;
       uint16_t* dst = a.q_out + ((long long)row * a.n_q + h) * v.D + sub * 8;
       *reinterpret_cast<uint4*>(dst) = pack(xa);
       *reinterpret_cast<uint4*>(dst + half) = pack(xb);
       continue;
     }
-    if (slot < 0) continue;
     const int hk = is_k ? h - a.n_q : h - a.n_q - v.n_kv;
     const long long at = (slot * v.n_kv + hk) * v.D + sub * 8;
     void* pages = is_k ? a.k : a.vv;
     if (!a.scales) {
+      if (!on || slot < 0) continue;
       uint16_t* dst = (uint16_t*)pages + at;
       *reinterpret_cast<uint4*>(dst) = pack(xa);
       *reinterpret_cast<uint4*>(dst + half) = pack(xb);
       continue;
     }
+    uint32_t top = 0;  // bits of the largest magnitude; those of a NaN are above an infinity's, and these above every number's
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) top = max(top, max(__float_as_uint(fabsf(xa[j])), __float_as_uint(fabsf(xb[j]))));
+    }
+    top = group_max<L>(top);
+    if (!on || slot < 0) continue;
     const bool finite = top < 0x7f800000u;
     const float amax = __uint_as_float(top), scale = amax < 1e-34f ? 0.f : amax / 127.f;
     const float inv = finite && scale > 0.f ? 1.0f / scale : 0.f;
+    // Nearest integers by an addition: 1.5 * 2^23 + n has n in its low byte. |x| inv is at most 127 (1 + 2^-22), which rounds to 127.
     auto quant = [&](const float (&f)[8]) {
-      uint32_t w[2] = {0, 0};
+      uint32_t b[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int q = finite ? max(-127, min(127, __float2int_rn(f[j] * inv))) : 0;
-        w[j >> 2] |= (uint32_t)(uint8_t)q << (8 * (j & 3));
-      }
-      return make_uint2(w[0], w[1]);
+      for (int j = 0; j < 8; j++) b[j] = __float_as_uint(fmaf(finite ? f[j] : 0.f, inv, 12582912.0f));
+      return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                        __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
     };
     int8_t* dst = (int8_t*)pages + at;
     *reinterpret_cast<uint2*>(dst) = quant(xa);
@@ -220,16 +232,14 @@ cudaError_t launch_rope_kv_paged(RopePagedArgs a, cudaStream_t stream) {
   const int heads = a.n_q + 2 * a.v.n_kv;
   int lanes = 1;
   while (lanes < a.v.D / 16) lanes *= 2;
-  // One head to a group until the machine has 32 warps an SM: a single token's heads then run beside one another; more rows share the work on
+  // One head to a warp until the machine has 24 warps an SM: a single token's heads then run beside one another; more rows share the work on
   // their angles over up to eight heads.
-  const long long enough = 32ll * current_sm_count() * (32 / lanes);
+  const int rows = 32 / lanes;
+  const long long row_groups = (a.v.rows + rows - 1) / rows;
   a.per = 1;
-  while (a.per < 8 && a.per < heads && (long long)a.v.rows * heads / (2 * a.per) >= enough) a.per *= 2;
-  const long long items = (long long)a.v.rows * ((heads + a.per - 1) / a.per);
-  auto run = [&](auto kernel) {
-    const int per_block = 256 / lanes;
-    return launch_dependent(kernel, dim3((unsigned)((items + per_block - 1) / per_block)), dim3(256), 0, stream, a);
-  };
+  while (a.per < 8 && a.per < heads && row_groups * heads / (2 * a.per) >= 24ll * current_sm_count()) a.per *= 2;
+  const long long warps = row_groups * ((heads + a.per - 1) / a.per);
+  auto run = [&](auto kernel) { return launch_dependent(kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, a); };
   switch (lanes) {
     case 1: return run(rope_kv_paged_kernel<1>);
     case 2: return run(rope_kv_paged_kernel<2>);

@@ -24,5 +24,8 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {  // zeros when not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
 
 }  // namespace tb200
