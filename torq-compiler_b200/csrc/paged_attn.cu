@@ -452,13 +452,14 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
 
 // Adds up the parts of the tiles that several blocks shared, in their order: a block has 16 rows and 64 dims of a tile. What bounds it is how many
 // loads of parts are under way at once, so where rows are few the parts are spread over the threads that this leaves.
-constexpr int kJoinRows = 16, kJoinDims = 64, kJoinThreads = 256;
+constexpr int kJoinRows = 32, kJoinDims = 64, kJoinThreads = 256, kJoinAhead = 3;
 struct JoinSet {
   const float* partial;
   const AttnJoin* joins;
   int count, pitch;  // blocks that may have begun a shared tile; rows that partial sums have room for
+  int join_rows;     // rows a block of the join takes
 };
-__global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const AttnPagedArgs a, const JoinSet many, const JoinSet few) {
+__global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const AttnPagedArgs a, const JoinSet many, const JoinSet few) {
   extern __shared__ __align__(16) unsigned char join_sm[];
   __shared__ RowScratch<kJoinThreads> plain;
   __shared__ float4 meet[kJoinThreads];
@@ -469,82 +470,117 @@ __global__ void __launch_bounds__(kJoinThreads) attn_paged_join_kernel(const Att
   constexpr int kChunks = 128 / kJoinRows;
   const bool is_many = (int)blockIdx.x < many.count * kChunks;
   const JoinSet set = is_many ? many : few;
-  // tiles of many rows: 16 of them to a block, all dims one after another; tiles of few rows: 64 dims to a block
+  // tiles of many rows: 32 of them to a block, all dims one after another; tiles of few rows: 64 dims to a block
   const int rest = (int)blockIdx.x - many.count * kChunks, dim_blocks = (a.v.D + kJoinDims - 1) / kJoinDims;
   const int at = is_many ? blockIdx.x / kChunks : rest / dim_blocks, r0 = is_many ? blockIdx.x % kChunks * kJoinRows : 0;
   const int first_dim = is_many ? 0 : rest % dim_blocks * kJoinDims, end_dim = is_many ? a.v.D : min(a.v.D, first_dim + kJoinDims);
   const AttnJoin j = set.joins[at];
-  const int rows = min(kJoinRows, j.used - r0);
+  const int pitch = set.join_rows, rows = min(pitch, j.used - r0);
   if (!j.parts || rows <= 0) return;
   const int tid = threadIdx.x, D = a.v.D, group = a.n_q / a.v.n_kv;
-  float2* const ml = reinterpret_cast<float2*>(join_sm);  // [part][16 rows]: (base, sum), then (factor, -)
+  float2* const ml = reinterpret_cast<float2*>(join_sm);  // [part][rows]: (base, sum), then (factor, -)
   auto part = [&](int f) { return set.partial + (long long)attn_part(j.first + f, f == 0 && j.second_place) * attn_part_floats(D, set.pitch); };
   if (tid == 0) bad = 0;
+  // Tiles of many rows: a thread has four dims of every 64 of two rows (of a warp's lanes eight rows lie side by side, whose partial sums are
+  // 128 bytes, and 16 dims, which the result has in 32). The first 64 are asked for before the rows' factors are known.
+  const int many_r = (tid & 7) | (tid >> 2 & 8), many_q = (tid >> 3 & 3) | (tid >> 4 & 12);
+  float4 x[2][kJoinAhead];
+  auto ask = [&](int d) {
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+#pragma unroll
+      for (int f = 0; f < kJoinAhead; f++)
+        x[c][f] = many_r + 16 * c < rows && d < D && f < j.parts ? __ldcg(reinterpret_cast<const float4*>(part(f)) + d / 4 * set.pitch + r0 + many_r + 16 * c)
+                                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  if (is_many) ask(many_q * 4);
 #pragma unroll 4
-  for (int i = tid; i < j.parts * kJoinRows; i += kJoinThreads) {
-    const int f = i / kJoinRows, r = i % kJoinRows;
+  for (int i = tid; i < j.parts * pitch; i += kJoinThreads) {  // (a power of two)
+    const int f = i >> (31 - __clz(pitch)), r = i & (pitch - 1);
     ml[i] = r < rows ? __ldcg(reinterpret_cast<const float2*>(part(f) + D * set.pitch + (r0 + r) * 2)) : make_float2(-INFINITY, 0.f);
   }
   __syncthreads();
-  {  // 16 threads to a row: its maximum, and the sum against it
-    const int r = tid >> 4, sub = tid & 15;
+  {  // eight threads to a row: its maximum, and the sum against it
+    const int r = tid >> 3, sub = tid & 7, parts = r < pitch ? j.parts : 0;
     float top = -INFINITY, sum = 0.f;
-    for (int f = sub; f < j.parts; f += 16) top = fmaxf(top, ml[f * kJoinRows + r].x);
+    for (int f = sub; f < parts; f += 8) top = fmaxf(top, ml[f * pitch + r].x);
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float from = top == -INFINITY ? 0.f : top;
-    for (int f = sub; f < j.parts; f += 16) {
-      float2& x = ml[f * kJoinRows + r];
+    for (int f = sub; f < parts; f += 8) {
+      float2& x = ml[f * pitch + r];
       x.x = x.x == -INFINITY ? 0.f : exp2_fast(x.x - from);
       sum += x.x == 0.f ? 0.f : x.x * x.y;
     }
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sub == 0) {
       invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
       if (r < rows && sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
     }
   }
   __syncthreads();
-  int span = 1;  // a power of two that holds the rows
-  while (span < rows) span *= 2;
-  const int groups = kJoinRows / span, r = tid & (span - 1), q = tid / span & 15, mine = tid / (span * 16);
-  for (int d0 = first_dim; d0 < end_dim; d0 += kJoinDims) {
-  const bool on = r < rows && d0 + q * 4 < D;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (on) {
-    for (int f0 = mine; f0 < j.parts; f0 += 4 * groups) {
-      float4 x[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int f = f0 + k * groups;
-        x[k] = f < j.parts ? __ldcg(reinterpret_cast<const float4*>(part(f)) + (d0 / 4 + q) * set.pitch + r0 + r) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int f = f0 + k * groups;
-        const float y = f < j.parts ? ml[f * kJoinRows + r].x : 0.f;
-        if (y == 0.f) continue;  // that part saw no key of this row
-        o.x += y * x[k].x; o.y += y * x[k].y; o.z += y * x[k].z; o.w += y * x[k].w;
-      }
-    }
-  }
-  meet[tid] = o;
-  __syncthreads();
-  if (mine == 0 && on) {
-    for (int k = 1; k < groups; k++) {
-      const float4 x = meet[tid + k * span * 16];
-      o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
-    }
+  auto add = [](float4& o, float y, const float4& x) {
+    if (y == 0.f) return;  // that part saw no key of this row
+    o.x += y * x.x; o.y += y * x.y; o.z += y * x.z; o.w += y * x.w;
+  };
+  auto store = [&](int r, int d, float4 o) {
     const float inv = invs[r];
     o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
     if (!(fabsf(o.x) <= 3.0e38f && fabsf(o.y) <= 3.0e38f && fabsf(o.z) <= 3.0e38f && fabsf(o.w) <= 3.0e38f)) atomicOr(&bad, 1u << r);
     const int tok = page_of(r0 + r, a.group_div);
-    *reinterpret_cast<uint2*>(a.out + ((long long)(j.row0 + tok) * a.n_q + j.head * group + r0 + r - tok * group) * D + d0 + q * 4) =
+    *reinterpret_cast<uint2*>(a.out + ((long long)(j.row0 + tok) * a.n_q + j.head * group + r0 + r - tok * group) * D + d) =
         make_uint2(pack_bf16(o.x, o.y), pack_bf16(o.z, o.w));
+  };
+  if (is_many) {
+    for (int d = many_q * 4; d < D; d += kJoinDims) {
+      if (d >= kJoinDims) ask(d);
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const int r = many_r + 16 * c;
+        if (r >= rows) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int f = 0; f < kJoinAhead; f++)
+          if (f < j.parts) add(o, ml[f * pitch + r].x, x[c][f]);
+#pragma unroll 4
+        for (int f = kJoinAhead; f < j.parts; f++) add(o, ml[f * pitch + r].x, __ldcg(reinterpret_cast<const float4*>(part(f)) + d / 4 * set.pitch + r0 + r));
+        store(r, d, o);
+      }
+    }
+  } else {
+    int span = 1;  // a power of two that holds the rows
+    while (span < rows) span *= 2;
+    const int groups = 16 / span, r = tid & (span - 1), q = tid / span & 15, mine = tid / (span * 16);
+    const bool on = r < rows && first_dim + q * 4 < end_dim;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) {
+      for (int f0 = mine; f0 < j.parts; f0 += 4 * groups) {
+        float4 y[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int f = f0 + k * groups;
+          y[k] = f < j.parts ? __ldcg(reinterpret_cast<const float4*>(part(f)) + (first_dim / 4 + q) * set.pitch + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int f = f0 + k * groups;
+          if (f < j.parts) add(o, ml[f * pitch + r].x, y[k]);
+        }
+      }
+    }
+    meet[tid] = o;
+    __syncthreads();
+    if (mine == 0 && on) {
+      for (int k = 1; k < groups; k++) {
+        const float4 y = meet[tid + k * span * 16];
+        o.x += y.x; o.y += y.y; o.z += y.z; o.w += y.w;
+      }
+      store(r, first_dim + q * 4, o);
+    }
   }
   __syncthreads();
-  }
   const uint32_t again = bad;
   for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
     if (!(again >> i & 1)) continue;
@@ -615,7 +651,7 @@ cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStrea
   a.few_rows = c.few ? 8 * c.rt : 0;
   a.wait_ns = wait_limit_ns();
   char* at = (char*)scratch;
-  JoinSet sets[2] = {{(float*)at, nullptr, c.many ? sms : 0, 128}, {(float*)(at + (c.many ? part_bytes(a, sms, 128) : 0)), nullptr, c.few_blocks, kFewRows}};
+  JoinSet sets[2] = {{(float*)at, nullptr, c.many ? sms : 0, 128, kJoinRows}, {(float*)(at + (c.many ? part_bytes(a, sms, 128) : 0)), nullptr, c.few_blocks, kFewRows, 8 * c.rt}};
   AttnJoin* const joins = (AttnJoin*)((char*)sets[1].partial + part_bytes(a, c.few_blocks, kFewRows));
   sets[0].joins = joins;
   sets[1].joins = joins + sms;
@@ -640,7 +676,7 @@ cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStrea
     const cudaError_t e = launch_attn_paged_tile(shaped(128 / group, sms, sets[0], 0, 2), stream);
     if (e != cudaSuccess) return e;
   }
-  const int join_smem = std::max(sets[0].count, sets[1].count) * kJoinRows * (int)sizeof(float2);
+  const int join_smem = std::max(sets[0].count * sets[0].join_rows, sets[1].count * sets[1].join_rows) * (int)sizeof(float2);
   static std::atomic<unsigned long long> attr_done;
   if (first_use_on_device(attr_done)) {
     const cudaError_t e = cudaFuncSetAttribute(attn_paged_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
