@@ -489,16 +489,15 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
                              (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= a.sinks);
         wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
         tc_fence_after();
-        // 32 scores, of columns 32 k on, those of keys this row does not see at -inf. The loops over them stay rolled up: a
+        // Of 32 scores, of columns 32 k on, those of keys this row does not see become -inf. The loops over them stay rolled up: a
         // processor's four quarters each run this beside other roles, and what does not fit their instruction buffers is waited for.
-        auto scores = [&](int k, uint32_t (&s)[32]) {
-          tmem_ld32_issue(s_tmem + 32 * k, s);
-          tmem_ld_wait32(s);
+        auto hide = [&](int k, uint32_t (&s)[32]) {
           if (partial) {
             // bits of the keys this row sees: not behind its position, inside the window or among the first, and held
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
             const int k0 = key0 + 32 * k;
             const uint32_t see = below(pos - k0 + 1) & (~below(near - k0) | below(a.sinks - k0)) & mt.holds[half * 2 + k];
+            if (__all_sync(0xffffffffu, see == 0xffffffffu)) return;  // most of a partial block is seen by all
 #pragma unroll
             for (int i = 0; i < 32; i++) s[i] = see >> i & 1 ? s[i] : 0xff800000u;
           }
@@ -517,7 +516,9 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
 #pragma unroll 1
             for (int k = 0; k < 2; k++) {
               uint32_t s[32];
-              scores(k, s);
+              tmem_ld32_issue(s_tmem + 32 * k, s);
+              tmem_ld_wait32(s);
+              hide(k, s);
               float tops[2] = {top, -INFINITY};
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
@@ -558,10 +559,17 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
           const unsigned long long scale2 = pack_f32(cexp, cexp), base2 = pack_f32(-base, -base);
           unsigned long long parts2[2] = {0ull, 0ull};  // two pairs of running sums
           float most = -INFINITY;
+          uint32_t both[I8 ? 1 : 2][32];  // (beside the widening warps there are no registers for 64 scores)
+          if (!I8) {
+            tmem_ld32_issue(s_tmem, both[0]);
+            tmem_ld32_issue(s_tmem + 32, both[I8 ? 0 : 1]);
+          }
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            uint32_t s[32];
-            scores(k, s);
+            uint32_t (&s)[32] = both[I8 ? 0 : k];
+            if (I8) tmem_ld32_issue(s_tmem + 32 * k, s);
+            tmem_ld_wait32(s);
+            hide(k, s);
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               unsigned long long ks[2] = {scale2, scale2}, vs[2];
