@@ -63,7 +63,9 @@ TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int
   s.near_block = (int)(near / kKeyBlock);
   const int sink_blocks = (int)span_min((sinks + (long long)kKeyBlock - 1) / kKeyBlock, s.near_block);
   s.sink_blocks = sink_blocks;
-  const int last = (int)((end + kKeyBlock - 1) / kKeyBlock);
+  // (tokens a window behind the table's end see first tokens only: those of near_block, if any)
+  const bool any = near < end || sinks > (long long)s.near_block * kKeyBlock;
+  const int last = any ? (int)((end + kKeyBlock - 1) / kKeyBlock) : s.near_block;
   s.blocks = sink_blocks + (last > s.near_block ? last - s.near_block : 0);
   if (s.blocks < 1) s.blocks = 1;
   return s;
