@@ -75,7 +75,8 @@ enum tb200_op_kind {
   /* decoder (bf16 activations, int8 per-output-channel weights) */
   TB200_OP_EMBED = 32,        /* gather rows of an int8 table, dequant, * f0 */
   TB200_OP_RMSNORM = 33,      /* y = x * rsqrt(mean(x^2) + f0) * (1 + w)  (bf16) */
-  TB200_OP_GEMV_W8 = 34,      /* y[b,n] = (sum_k x[b,k] * W[n,k]) * scale[n]  (fp32 acc) */
+  TB200_OP_GEMV_W8 = 34,      /* y[b,n] = (sum_k x[b,k] * W[n,k]) * scale[n]  (fp32 acc); any number of rows b. i0 > 0 asks for
+                               * that many slices of K, up to 32 rows (more rows are cut by their own rule) */
   TB200_OP_ROPE_KV = 35,      /* q/k per-head RMSNorm + rotary, append k,v to cache */
   TB200_OP_ATTN_DECODE = 36,  /* single-query GQA attention over the cache */
   TB200_OP_GEGLU = 37,        /* y = gelu_tanh(gate) * up */
@@ -95,7 +96,8 @@ enum tb200_op_kind {
    * sequence s, at positions context[s], context[s] + 1, ... (in2, i32 [S]); rows in no sequence are padding, and what an op would write for
    * them is left as it was. Position p of a sequence lies in page table[s][p / page_size] (multiplier slot, i32 [S, max_pages], bound or
    * state); a page id outside [0, pages), or a position behind max_pages * page_size, holds nothing: writes to it are dropped, its keys are
-   * not seen, reads of it give zeros. Caches: shift slot = keys, table slot = values, [layers, pages, page_size, kv * D], bf16, or
+   * not seen, reads of it give zeros. Sequences may share pages that are read; where two rows of a chunk are written to one place, either (or
+   * a mixture, 16 bytes at a time) may last. Caches: shift slot = keys, table slot = values, [layers, pages, page_size, kv * D], bf16, or
    * int8 with fp32 scales [layers, pages, page_size, 2 * kv] (bias slot; of the keys, then of the values): bound or state tensors that the
    * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. */
   TB200_OP_ROPE_KV_PAGED = 43,/* in0 = qkv [rows, (i0 + 2 kv) * D] -> out0 = rotated queries [rows, i0 * D]; keys and values go to their pages.

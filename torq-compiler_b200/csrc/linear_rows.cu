@@ -9,11 +9,16 @@
 // clocks over it. A result's row of TMEM is then a weight row, so its scale is one number a thread, and 32 lanes store 32 neighbouring
 // outputs of one row: no alignment of N is needed.
 //
-// Roles: 8 warps widen (a warp has 32 weight rows, as TMEM's lanes want it), 8 warps scale, round and store what is finished (a tile's sums
-// go to registers first, so that the next tile begins while they are stored), one or two multiply (one for each half),
-// two copy (steps by turns).
+// Roles: 16 warps widen, as teams of four that take 128 weight rows of a step by turns (a warp has 32 of them, as TMEM's lanes want it): eight
+// warps took 1050 clocks over a step of 256 rows, most of it the latency of their own chain, where the instructions take 768; with 16 a step
+// takes 770. Eight warps finish: they scale, round and turn patches of 32 x 32 in shared memory, so that they store 16 bytes a lane (stored 2
+// bytes a lane straight from TMEM, a tile took longer than its products: 127 us against 102 for 4000 x 13824 x 1152). One or two multiply (one
+// for each half, whose sums are its own), two copy (steps by turns).
 // Blocks are persistent and take every grid-th tile. Tiles of the same weights lie one behind another, so weights and activations both
-// come from L2 but for their first use.
+// come from L2 but for their first use. Where tiles are few, a cluster of up to eight blocks shares one, a part of K each, and adds the parts
+// up over distributed shared memory in their order: 128 x 1152 x 6912 in 12.7 us (32 with a block to a tile).
+// Measured from memory: 4000 x 13824 x 1152 104 us (1.22 PFLOP/s) in a loop of its own; 125 us where the plain form in fp32 runs in between
+// and has used up the power budget.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -368,7 +373,10 @@ cudaError_t run_rows(const LinearRowsArgs& l, int splits, int sms, cudaStream_t 
 
 }  // namespace
 
-// Shapes, with what a step of K and everything else of a tile took (microseconds; all processors at work, K = 1152 and 6912).
+// Shapes, with what a step of K and everything else of a tile took (microseconds). With 5 us for the launch these give 40 times (four shapes at ten
+// sizes: 33 to 4000 rows, N of 1152 to 13824, K of 1152 to 6912) within 22 %, most of them too low by a tenth, and the shape they pick was the
+// fastest at each of the ten. In the order of the list: 4000 x 13824 x 1152 105 / 122 / 143 / 230 us, 1000 x 13824 x 1152 (an earlier form, whole
+// K) 41 / 35 / 41 / 64, 1000 x 1152 x 6912 29 / 35 / 25 / 33, 300 x 1536 x 1152 16.8 / 14.6 / 12.6 / 10.6.
 struct RowsShape {
   int halves, xn;
   float step, tile;

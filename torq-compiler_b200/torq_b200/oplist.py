@@ -437,7 +437,7 @@ class Graph:
 
     def gemv_w8(self, x, weights_i8, scales_bf16, splits: int = 0, out_dtype: str = "bf16", in_offset: int = 0):
         """y[b, n] = scale[n] * sum_k x[b, in_offset + k] * W[n, k], rounded to bf16 or kept in fp32 (out_dtype
-        "f32"); W is [N, K] int8. A W narrower than x (with in_offset) takes a column slice of x; that form
+        "f32"); W is [N, K] int8, x has any number of rows (`splits` slices of K are a matter of up to 32). A W narrower than x (with in_offset) takes a column slice of x; that form
         exists only inside the fused decode step (tensor-parallel shards)."""
         w = weights_i8 if isinstance(weights_i8, TensorRef) else self.const(np.asarray(weights_i8, np.int8))
         sc = scales_bf16 if isinstance(scales_bf16, TensorRef) else self.const(np.asarray(scales_bf16, np.uint16), "bf16")
