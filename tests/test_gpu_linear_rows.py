@@ -5,6 +5,7 @@ import pytest
 from gpu_exec import run_graph_gpu
 from torq_b200.bf16 import from_bf16, to_bf16
 from torq_b200.oplist import Graph
+from torq_b200.runtime import Executable
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +83,28 @@ def test_products_behind_one_another(device):
     got_gu, got_act, got_y = run_graph_gpu(device, g, [x])
     check(from_bf16(got_gu), x, w1, s1, False)
     check(from_bf16(got_y), got_act, w2, s2, False)
+
+
+def test_one_executable_on_several_buffers(device):
+    """Dispatched by turns on two inputs and two results, and once more on the first: what a call prepares for its addresses is the call's own."""
+    x, w, s = inputs(70, 260, 320)
+    x2 = inputs(70, 260, 320, 9)[0]
+    g = Graph()
+    g.output(g.gemv_w8(g.input(x.shape, "bf16"), w, s, out_dtype="f32"))
+    ex = Executable(device, g.serialize())
+    ins, outs = [device.alloc(x.nbytes) for _ in range(2)], [device.alloc(70 * 260 * 4) for _ in range(2)]
+    try:
+        for b, a in zip(ins, (x, x2)):
+            b.upload(a)
+        for i, o in ((0, 0), (1, 1), (1, 0), (0, 1), (0, 0)):
+            ex.dispatch([ins[i]], [outs[o]])
+        device.wait()
+        check(outs[0].download((70, 260), np.float32), x, w, s, True)
+        check(outs[1].download((70, 260), np.float32), x, w, s, True)
+        ex.dispatch([ins[1]], [outs[1]])
+        device.wait()
+        check(outs[1].download((70, 260), np.float32), x2, w, s, True)
+    finally:
+        for b in ins + outs:
+            b.free()
+        ex.destroy()

@@ -186,6 +186,48 @@ def test_attention_repeats_bit_by_bit(device, i8):
         assert np.array_equal(first, attend(device, b, q, times=3)[0])
 
 
+def test_attention_two_executables_and_changing_batches(device):
+    """Two loaded chunks take turns, and the batch of one changes between its calls (more sequences of few rows, then one of many, then none): nothing
+    is kept from a call that another would see."""
+    first = Batch([100, 1, 3], [300, 2000, 40], n_q=8, n_kv=2, d=64, page=16, pad=40, seed=3)
+    other = Batch([1] * 5, [700, 3, 90, 1500, 128], n_q=4, n_kv=1, d=256, page=32, i8=True, seed=4)
+    loaded = []
+    try:
+        for b in (first, other):
+            g = Graph()
+            refs, arrays, kw = b.inputs(g)
+            q = bf16(b.rng, b.rows, b.n_q * b.d)
+            g.output(g.attn_paged(g.input(q.shape, "bf16"), *refs, n_q=b.n_q, scale=b.d ** -0.5, **kw))
+            bufs = []
+            for a in arrays + [q, bf16(b.rng, *q.shape)]:
+                bufs.append(device.alloc(a.nbytes))
+                bufs[-1].upload(np.ascontiguousarray(a))
+            loaded.append((Executable(device, g.serialize()), bufs, b, q))
+
+        def turn(which):
+            ex, bufs, b, q = loaded[which]
+            bufs[0].upload(b.row_start)
+            bufs[1].upload(b.context)
+            before = bf16(b.rng, *q.shape)
+            bufs[-1].upload(before)
+            ex.dispatch(bufs[:-1], bufs[-1:])
+            device.wait()
+            check_attention(bufs[-1].download(q.shape, np.uint16), before, *attention(b, q, b.d ** -0.5))
+
+        for new in ([100, 1, 3], [2, 140, 2], [1, 1, 1], [0, 0, 0], [144, 0, 0], [0, 2, 90]):
+            first.new = new
+            first.row_start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+            first.ctx = [300 - min(300, new[0]), 2000 - new[1], 40 if new[2] < 4 else 0]
+            first.context = np.array(first.ctx, np.int32)
+            turn(0)
+            turn(1)
+    finally:
+        for ex, bufs, _, _ in loaded:
+            for x in bufs:
+                x.free()
+            ex.destroy()
+
+
 # ---- cache -------------------------------------------------------------------------------------------------------
 
 def write(device, b, qkv, norms=None, theta=10000.0, eps=1e-6):
