@@ -99,7 +99,8 @@ enum tb200_op_kind {
    * not seen, reads of it give zeros. Sequences may share pages that are read; where two rows of a chunk are written to one place, either (or
    * a mixture, 16 bytes at a time) may last. Caches: shift slot = keys, table slot = values, [layers, pages, page_size, kv * D], bf16, or
    * int8 with fp32 scales [layers, pages, page_size, 2 * kv] (bias slot; of the keys, then of the values): bound or state tensors that the
-   * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. */
+   * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. A dispatch whose results are bound over
+   * what such an op reads (or keys over values, when they are written) ends with an error before anything of the op runs. */
   TB200_OP_ROPE_KV_PAGED = 43,/* in0 = qkv [rows, (i0 + 2 kv) * D] -> out0 = rotated queries [rows, i0 * D]; keys and values go to their pages.
                                * weights = bf16 norms [2, D] of queries and keys (x * rsqrt(mean(x^2) + f1) * (1 + w)) or -1; f0 = RoPE base >= 1.
                                * fp32 inside, rounded once. int8: scale = amax / 127 of a token's head, nearest integer; a head with

@@ -6,7 +6,7 @@ import pytest
 from paged_ref import Batch, attention, bf16, check_attention, rope_write
 from torq_b200.bf16 import from_bf16, to_bf16
 from torq_b200.oplist import Graph
-from torq_b200.runtime import Executable
+from torq_b200.runtime import Executable, TorqB200Error
 
 pytestmark = pytest.mark.gpu
 
@@ -375,3 +375,63 @@ def test_a_chunk_as_it_is_used(device, i8):
     for buf in bufs + outs:
         buf.free()
     ex.destroy()
+
+
+def test_results_bound_over_what_is_read_are_refused(device):
+    """One buffer as queries and result, as product's input and result, as keys and values that are written, or as cache and what is read from it."""
+    b = Batch([3, 40], [20, 5], n_q=4, n_kv=4, d=64, page=16)
+    room = device.alloc(max(b.k.nbytes, b.rows * 16 * 64 * 2) + 4096)
+    rest = [device.alloc(1 << 20) for _ in range(8)]
+
+    def run(graph, inputs, outputs):
+        ex = Executable(device, graph.serialize())
+        try:
+            ex.dispatch(inputs, outputs)
+            device.wait()
+        finally:
+            ex.destroy()
+
+    def refused(make):
+        g = Graph()
+        refs, arrays, kw = b.inputs(g)
+        own = [device.alloc(a.nbytes) for a in arrays]
+        try:
+            for x, a in zip(own, arrays):
+                x.upload(a)
+            with pytest.raises(TorqB200Error):
+                run(*make(g, refs, kw, own))
+        finally:
+            for x in own:
+                x.free()
+
+    def attend_over(which):
+        def make(g, refs, kw, own):
+            g.output(g.attn_paged(g.input((b.rows, 256), "bf16"), *refs, n_q=4, scale=0.125, **kw))
+            return g, own + [room], [room if which == "q" else own[3]]
+        return make
+
+    def write_over(which):
+        def make(g, refs, kw, own):
+            g.output(g.rope_kv_paged(g.input((b.rows, 12 * 64), "bf16"), *refs, n_q=4, theta=1e4, **kw))
+            if which == "kv":
+                own = own[:4] + [own[3]]
+            return g, own + [room], [rest[0] if which == "kv" else room]
+        return make
+
+    def read_over(g, refs, kw, own):
+        for t in g.kv_read_paged(*refs, rows=b.rows, **kw):
+            g.output(t)
+        return g, own, [rest[0], rest[0]]
+
+    def product_over(g, refs, kw, own):
+        g = Graph()
+        g.output(g.gemv_w8(g.input((40, 64), "bf16"), np.ones((64, 64), np.int8), to_bf16(np.ones(64, np.float32))))
+        return g, [room], [room]
+
+    try:
+        for make in (attend_over("q"), attend_over("k"), write_over("qkv"), write_over("kv"), read_over, product_over):
+            refused(make)
+        check(device, b)  # and the device goes on
+    finally:
+        for x in [room] + rest:
+            x.free()

@@ -387,6 +387,7 @@ struct PagedPlan {
   PagedView v{};  // pointers are filled at dispatch
   bool i8 = false;
   size_t layer_bytes = 0, layer_scales = 0;  // byte offset of the layer in the pages, element offset in the scales
+  size_t layer_size() const { return (size_t)v.pages * v.page_size * v.n_kv * v.D * (i8 ? 1 : 2); }
 };
 bool paged_plan(Builder& b, const tb200_op_t& op, int row_start, int context, int i, const char* name, PagedPlan& c) {
   const auto& T = b.tensors;
@@ -1138,6 +1139,10 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
   };
   auto report = [](cudaError_t e, const ExecContext& c) {
     if (e != cudaSuccess && c.launch_error) *c.launch_error = e;
+  };
+  // A chunk's kernels read what they are given while they write: bindings that lie over one another are refused when they are dispatched.
+  auto apart = [](const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    return (const char*)a + a_bytes <= (const char*)b || (const char*)b + b_bytes <= (const char*)a;
   };
   struct PlannedPool { PoolArgs args; Loc x; size_t lut_off, rec_off; bool has_lut; std::function<void(const ExecContext&)> launch; };
   std::map<int, PlannedPool> pools;  // held pool ops
@@ -2169,6 +2174,7 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           step.launch = [=](const ExecContext& c) {
             const LinearRowsArgs k{(const uint16_t*)lx.resolve(c), (const int8_t*)(c.consts + w_off), (const uint16_t*)(c.consts + s_off),
                                    lo.resolve(c), y_f32, B, N, K, c.status};
+            if (!apart(k.x, (size_t)B * K * 2, k.y, (size_t)B * N * (y_f32 ? 4 : 2))) return report(cudaErrorInvalidValue, c);
             report(launch_linear_rows(k, sms, c.stream), c);
           };
           break;
@@ -2320,6 +2326,10 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.scales = c.i8 ? (float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.n_q = n_q;
           k.eps = eps;
+          const size_t cache = c.layer_size(), q_bytes = (size_t)k.v.rows * n_q * k.v.D * 2;
+          if (!apart(k.k, cache, k.vv, cache) || !apart(k.q_out, q_bytes, k.qkv, q_bytes + (size_t)k.v.rows * 2 * k.v.n_kv * k.v.D * 2) ||
+              !apart(k.q_out, q_bytes, k.k, cache) || !apart(k.q_out, q_bytes, k.vv, cache))
+            return report(cudaErrorInvalidValue, x);
           report(launch_rope_kv_paged(k, x.stream), x);
         };
         break;
@@ -2342,6 +2352,10 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.k_out = (uint16_t*)lk.resolve(x);
           k.v_out = (uint16_t*)lv.resolve(x);
+          const size_t cache = c.layer_size(), bytes = (size_t)k.v.rows * k.v.n_kv * k.v.D * 2;
+          for (const void* out : {(const void*)k.k_out, (const void*)k.v_out})
+            if (!apart(out, bytes, k.k, cache) || !apart(out, bytes, k.vv, cache)) return report(cudaErrorInvalidValue, x);
+          if (!apart(k.k_out, bytes, k.v_out, bytes)) return report(cudaErrorInvalidValue, x);
           report(launch_kv_read_paged(k, x.stream), x);
         };
         break;
@@ -2382,6 +2396,9 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.vv = (const char*)at.v.resolve(x) + c.layer_bytes;
           k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.out = (uint16_t*)lo.resolve(x);
+          const size_t cache = c.layer_size(), bytes = (size_t)k.v.rows * n_q * k.v.D * 2;
+          if (!apart(k.out, bytes, k.q, bytes) || !apart(k.out, bytes, k.k, cache) || !apart(k.out, bytes, k.vv, cache))
+            return report(cudaErrorInvalidValue, x);
           report(launch_attn_paged(k, sms, x.scratch, x.stream), x);
         };
         break;
