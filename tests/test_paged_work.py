@@ -31,19 +31,26 @@ static int spans() {
     const int tpt = 1 + rand() % 64, n = 1 + rand() % 200, ctx = rand() % 3 ? rand() % 1500 : 0, tile = rand() % ((n + tpt - 1) / tpt);
     const int window = rand() % 3 ? rand() % 600 : 0, sinks = window && rand() % 2 ? rand() % 400 : 0, capacity = rand() % 4 ? 4000 : 1 + rand() % 1700;
     const TileSpan t = tile_span(ctx, n, tile, tpt, window, sinks, capacity);
-    std::set<int> blocks;
+    std::set<int> keys;
     if (t.blocks < 1) return printf("no block\n"), 1;
-    for (int b = 0; b < t.blocks; b++)
-      if (!blocks.insert(tile_block(t, b)).second) return printf("a block twice: %d\n", tile_block(t, b)), 1;
-    std::set<int> needed;
+    for (int p = 0; p < t.blocks * kKeyBlock; p++) {
+      const int key = tile_key(t.front, t.shift, p);
+      if (key < 0 || !keys.insert(key).second) return printf("a key twice: %d\n", key), 1;
+      if (p % kSpanAlign && key != tile_key(t.front, t.shift, p - 1) + 1) return printf("keys do not follow one another: %d\n", key), 1;
+      if (p % kSpanAlign == 0 && key % kSpanAlign) return printf("key %d begins a run\n", key), 1;
+      if (!sinks && p % kKeyBlock == 0 && key % kKeyBlock) return printf("key %d begins a block\n", key), 1;
+    }
+    std::set<int> needed, blocks;
     for (int k = tile * tpt; k < n && k < (tile + 1) * tpt; k++)
       for (int j = 0; j <= ctx + k && j < capacity; j++) {
         if (window && j <= ctx + k - window && j >= sinks) continue;
-        if (!blocks.count(j / kKeyBlock)) return printf("key %d of token %d is in no block\n", j, k), 1;
+        if (!keys.count(j)) return printf("key %d of token %d has no place\n", j, k), 1;
         if (!(j < t.end_key && (j >= t.near_key || j < sinks))) return printf("key %d of token %d counts as unseen\n", j, k), 1;
-        needed.insert(j / kKeyBlock);
+        needed.insert(j);
+        blocks.insert(j / kKeyBlock);
       }
-    if ((int)needed.size() != t.blocks && !(needed.empty() && t.blocks == 1)) return printf("%d blocks for %zu\n", t.blocks, needed.size()), 1;
+    const int most = sinks ? ((int)needed.size() + 2 * (kSpanAlign - 1) + kKeyBlock - 1) / kKeyBlock : (int)blocks.size();
+    if (t.blocks > (most > 1 ? most : 1)) return printf("%d blocks for %d\n", t.blocks, most), 1;
   }
   return 0;
 }

@@ -41,15 +41,17 @@ struct PagedView {
 };
 
 // ---- how attention cuts a chunk into tiles, and shares the tiles' work out ----
-// A tile is up to tokens_per_tile new tokens of a sequence with the query heads of one key/value head; its work is the blocks of kKeyBlock
-// keys that one of its tokens may see: those of the first tokens that stay visible, then those from the window's start on.
+// A tile is up to tokens_per_tile new tokens of a sequence with the query heads of one key/value head; its work is the keys that one of its
+// tokens may see, in blocks of kKeyBlock: those of the first tokens that stay visible, and right behind them those from the window's start on.
+// (As blocks of their own 4 first tokens cost a window of 512 one block in six.)
 constexpr int kKeyBlock = 128;
+constexpr int kSpanAlign = 16;  // where both parts begin and the first one ends: keys that lie one behind another from such a place on still do
 struct TileSpan {
-  int sink_blocks;  // key blocks 0 .. sink_blocks - 1 come first
-  int near_block;   // then near_block, near_block + 1, ...
-  int blocks;       // in all; at least one, so that a tile that sees nothing is visited as well
-  int near_key;     // keys in front of it are seen as first tokens only
-  int end_key;      // one past the last key a token of the tile sees
+  int front;     // places 0 .. front - 1 of the tile's keys are those keys
+  int shift;     // place i from there on is key i + shift
+  int blocks;    // in all; at least one, so that a tile that sees nothing is visited as well
+  int near_key;  // keys in front of it are seen as first tokens only
+  int end_key;   // one past the last key a token of the tile sees
 };
 TB200_BOTH long long span_min(long long a, long long b) { return a < b ? a : b; }
 TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int window, int sinks, int capacity) {
@@ -60,19 +62,23 @@ TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int
   TileSpan s;
   s.near_key = (int)near;
   s.end_key = (int)end;
-  s.near_block = (int)(near / kKeyBlock);
-  const int sink_blocks = (int)span_min((sinks + (long long)kKeyBlock - 1) / kKeyBlock, s.near_block);
-  s.sink_blocks = sink_blocks;
-  // (tokens a window behind the table's end see first tokens only: those of near_block, if any)
-  const bool any = near < end || sinks > (long long)s.near_block * kKeyBlock;
-  const int last = any ? (int)((end + kKeyBlock - 1) / kKeyBlock) : s.near_block;
-  s.blocks = sink_blocks + (last > s.near_block ? last - s.near_block : 0);
+  const long long front = ((long long)sinks + kSpanAlign - 1) / kSpanAlign * kSpanAlign, align = sinks > 0 ? kSpanAlign : kKeyBlock;
+  long long base = near / align * align;  // the window's part
+  s.front = 0;
+  if (sinks > 0) {
+    if (front <= base) s.front = (int)front;
+    else base = 0;  // no gap between the two
+  }
+  s.shift = (int)(base - s.front);
+  // (a window that lies behind the table's end leaves the first tokens)
+  const long long places = near < end ? end - s.shift : s.front ? s.front : span_min(sinks, end);
+  s.blocks = (int)((places + kKeyBlock - 1) / kKeyBlock);
   if (s.blocks < 1) s.blocks = 1;
   return s;
 }
 // A tile counts as its blocks and, in front of them, kTileCost more: what it takes to begin it and to store its rows.
 constexpr int kTileCost = 1;
-TB200_BOTH int tile_block(const TileSpan& s, int i) { return i < s.sink_blocks ? i : s.near_block + (i - s.sink_blocks); }
+TB200_BOTH int tile_key(int front, int shift, int place) { return place < front ? place : place + shift; }
 // `total` pieces of work in one row, shared out to `parts`: part i begins here
 TB200_BOTH long long work_begin(long long total, int i, int parts) { return total * i / parts; }
 TB200_BOTH int work_owner(long long w, long long total, int parts) {

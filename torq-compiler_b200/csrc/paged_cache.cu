@@ -48,7 +48,8 @@ __device__ __forceinline__ int sequence_from(const PagedView& v, int s, int row)
 // What bounds it: memory, once its instructions are few enough (an int8 cache and norms take the most of them). L lanes hold a head (L the
 // power of two from D / 16 on), eight neighbouring values of each half to a lane, so that every access has 16 bytes. A warp takes the same
 // `per` heads of 32 / L rows one after another: its branches are then the same for all lanes, a row's angles and the norm's weights are
-// fetched once for several heads, and four heads are on their way while one is worked on.
+// fetched once for several heads, and four heads are on their way while one is worked on (one ahead: 28.7 us against 22.7 for 16384 rows of 4/1 heads
+// of 256 into bf16, 101 MB; 4001 rows of 32/8 heads of 128 with norms into int8, 90 MB, take 29 us, at 64 % of the issue slots).
 constexpr int kAhead = 4;
 template <int L>
 __global__ void __launch_bounds__(128) rope_kv_paged_kernel(const RopePagedArgs a) {
@@ -169,7 +170,8 @@ __global__ void __launch_bounds__(128) rope_kv_paged_kernel(const RopePagedArgs 
 
 // k_out / v_out [rows][n_kv * D] bf16: the tokens' keys and values, int8 ones as bf16(integer * scale); zeros where a position holds
 // nothing. A warp takes `per` rows, whose slots its lanes look up side by side; a lane then takes 16 values of a head at a time, and asks for
-// four such pieces before it stores one.
+// four such pieces before it stores one. 20011 rows of a head of 256 from int8 (31 MB) take 12.3 us, of which 4.6 are any call's: the reads of
+// a row's sequence, context and page stand in front of its values.
 template <bool I8>
 __global__ void __launch_bounds__(256) kv_read_paged_kernel(const ReadPagedArgs a) {
   grid_dependency_wait();

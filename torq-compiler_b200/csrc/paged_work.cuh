@@ -11,7 +11,7 @@ struct Item {
   int seq, head;
   int row0, tokens;         // the tile's rows of the chunk; tokens 0: there is no more work
   int first_pos;            // position of the first token
-  int near_key, end_key, sink_blocks, near_block, blocks;  // tile_span
+  int near_key, end_key, front, shift, blocks;  // tile_span
   int b0, b1;
   long long w0;             // where the tile's work begins
 };
@@ -37,12 +37,12 @@ __device__ __forceinline__ int tiles_of(const AttnPagedArgs& a, const Span& s) {
 // for each); slots have 32 bits (the planner refuses more), -1 where no token of the tile sees the key or nothing is held.
 struct Keys {
   const int32_t* pages_of;
-  int near_key, end_key, sinks, sink_blocks, near_block, last, pages, page_size;
+  int near_key, end_key, sinks, front, shift, last, pages, page_size;
   PageDivisor div;
   __device__ __forceinline__ Keys(const AttnPagedArgs& a, const Item& w)
-      : pages_of(a.v.table + (long long)w.seq * a.v.max_pages), near_key(w.near_key), end_key(w.end_key), sinks(a.sinks), sink_blocks(w.sink_blocks),
-        near_block(w.near_block), last(a.v.capacity - 1), pages(a.v.pages), page_size(a.v.page_size), div(a.v.div) {}
-  __device__ __forceinline__ int first(int b) const { return (b < sink_blocks ? b : near_block + (b - sink_blocks)) * kKeyBlock; }
+      : pages_of(a.v.table + (long long)w.seq * a.v.max_pages), near_key(w.near_key), end_key(w.end_key), sinks(a.sinks), front(w.front),
+        shift(w.shift), last(a.v.capacity - 1), pages(a.v.pages), page_size(a.v.page_size), div(a.v.div) {}
+  __device__ __forceinline__ int at(int place) const { return tile_key(front, shift, place); }
   __device__ __forceinline__ int ask(int key) const {
     int page;  // volatile: it is to be on its way now, not when it is used
     asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(page) : "l"(pages_of + page_of(min(key, last), div)));
@@ -158,7 +158,7 @@ struct ItemCursor {
         w.row0 = span.row0 + tile * tpt;
         w.tokens = min(tpt, span.n - tile * tpt);
         w.first_pos = (int)min((long long)span.ctx + tile * tpt, 0x7fffffffll);
-        w.near_key = ts.near_key; w.end_key = ts.end_key; w.sink_blocks = ts.sink_blocks; w.near_block = ts.near_block; w.blocks = ts.blocks;
+        w.near_key = ts.near_key; w.end_key = ts.end_key; w.front = ts.front; w.shift = ts.shift; w.blocks = ts.blocks;
         w.b0 = max(off - kTileCost, 0); w.b1 = upto - kTileCost;
         w.w0 = cur - off + kTileCost;
       }
