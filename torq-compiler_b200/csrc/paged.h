@@ -62,17 +62,18 @@ TB200_BOTH TileSpan tile_span(int ctx, int n, int tile, int tokens_per_tile, int
   TileSpan s;
   s.near_key = (int)near;
   s.end_key = (int)end;
-  const long long front = ((long long)sinks + kSpanAlign - 1) / kSpanAlign * kSpanAlign, align = sinks > 0 ? kSpanAlign : kKeyBlock;
-  long long base = near / align * align;  // the window's part
+  // from here on in 32 bits and without divisions: the capacity is at most 2^30
+  const uint32_t front = ((uint32_t)sinks + kSpanAlign - 1) & ~(uint32_t)(kSpanAlign - 1);
+  int base = s.near_key & (sinks > 0 ? -kSpanAlign : -kKeyBlock);  // the window's part
   s.front = 0;
   if (sinks > 0) {
-    if (front <= base) s.front = (int)front;
+    if (front <= (uint32_t)base) s.front = (int)front;
     else base = 0;  // no gap between the two
   }
-  s.shift = (int)(base - s.front);
+  s.shift = base - s.front;
   // (a window that lies behind the table's end leaves the first tokens)
-  const long long places = near < end ? end - s.shift : s.front ? s.front : span_min(sinks, end);
-  s.blocks = (int)((places + kKeyBlock - 1) / kKeyBlock);
+  const int places = s.near_key < s.end_key ? s.end_key - s.shift : s.front ? s.front : sinks < s.end_key ? sinks : s.end_key;
+  s.blocks = (places + kKeyBlock - 1) / kKeyBlock;
   if (s.blocks < 1) s.blocks = 1;
   return s;
 }

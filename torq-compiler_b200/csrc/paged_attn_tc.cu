@@ -49,7 +49,9 @@ struct alignas(16) Meta {
   float k_scale[kKeyBlock], v_scale[kKeyBlock];
   int slot[kKeyBlock];  // where the cache holds the key, -1 where no row of the tile sees it or nothing is held
   uint32_t holds[4];    // the keys with a slot, a bit each
-  int key0;             // column c holds key key0 + c; where that lies in front of a window's part of the keys, one of the first tokens
+  // column c holds key key0 + c; where that lies in front of a window's part of the keys, one of the first tokens. Rows see what lies in front of
+  // `firsts` whatever their window (here, beside the slots, and not with the item: the softmax has no register left for it)
+  int key0, firsts;
 };
 static_assert(sizeof(Meta) % 16 == 0 && sizeof(TileRowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
 struct Control {
@@ -440,7 +442,10 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
             *reinterpret_cast<float4*>(&m.v_scale[4 * lane]) = make_float4(vs[0], vs[1], vs[2], vs[3]);
           }
           if ((lane & 7) == 0) m.holds[lane >> 3] = held;
-          if (lane == 0) m.key0 = b * kKeyBlock + keys_of.shift;
+          if (lane == 0) {
+            m.key0 = b * kKeyBlock + keys_of.shift;
+            m.firsts = keys_of.front ? keys_of.front + keys_of.shift : keys_of.sinks;
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&c.meta_full[at]));
         }
@@ -478,8 +483,6 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
       const int pos = (int)min((long long)first_pos + min(tok, tokens - 1), 0x7fffffffll);
       const int last_pos = (int)min((long long)first_pos + tokens - 1, 0x7fffffffll);
       const int near = a.window ? max(0, pos - a.window + 1) : 0;  // this row sees keys [near, pos] and those in front of `firsts`
-      // (the first tokens: every place in front of the window's part holds one, or nothing; read where it is needed, there is no register for it)
-      auto firsts = [&]() { return w.front ? w.front + w.shift : a.sinks; };
       float m = -INFINITY, base = 0.f, sum = 0.f;  // base: what the exponents are taken from, m or (before there is one) zero
       for (int b = 0; b < n; b++, blocks++) {
         const uint32_t s_tmem = tmem + lanes + (blocks & 1) * 128 + half * 64;
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
         const int key0 = mt.key0 + half * 64;
         // whether some row of the tile does not see some key of this half
         const bool partial = (mt.holds[half * 2] & mt.holds[half * 2 + 1]) != 0xffffffffu || key0 + 63 > first_pos ||
-                             (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= firsts());
+                             (a.window && key0 < max(0, last_pos - a.window + 1) && key0 + 63 >= mt.firsts);
         wait(c.s_full[blocks & 1], (blocks >> 1) & 1, 307);
         tc_fence_after();
         // Of 32 scores, of columns 32 k on, those of keys this row does not see become -inf. The loops over them stay rolled up: a
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
             auto upto = [](int n) { return n < 0 ? 0u : n >= 31 ? 0xffffffffu : (2u << n) - 1u; };
             const int k0 = key0 + 32 * k;
-            const uint32_t see = upto(pos - k0) & (~below(near - k0) | below(firsts() - k0)) & mt.holds[half * 2 + k];
+            const uint32_t see = upto(pos - k0) & (~below(near - k0) | below(mt.firsts - k0)) & mt.holds[half * 2 + k];
             if (__all_sync(0xffffffffu, see == 0xffffffffu)) return;  // most of a partial block is seen by all
 #pragma unroll
             for (int i = 0; i < 32; i++) s[i] = see >> i & 1 ? s[i] : 0xff800000u;
