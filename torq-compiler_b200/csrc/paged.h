@@ -43,7 +43,8 @@ struct PagedView {
 // ---- how attention cuts a chunk into tiles, and shares the tiles' work out ----
 // A tile is up to tokens_per_tile new tokens of a sequence with the query heads of one key/value head; its work is the keys that one of its
 // tokens may see, in blocks of kKeyBlock: those of the first tokens that stay visible, and right behind them those from the window's start on.
-// (As blocks of their own 4 first tokens cost a window of 512 one block in six.)
+// (As a block of their own 4 first tokens cost a window of 512 over
+// 8192 tokens, 16/2 heads of 64, 142.7 us instead of 94.0.)
 constexpr int kKeyBlock = 128;
 constexpr int kSpanAlign = 16;  // where both parts begin and the first one ends: keys that lie one behind another from such a place on still do
 struct TileSpan {

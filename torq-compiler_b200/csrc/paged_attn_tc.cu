@@ -13,7 +13,7 @@
 // Work is shared out evenly: all tiles' key blocks in one row, every block of the grid takes an equal piece. A tile that falls to several
 // leaves partial sums in memory, which the launch behind adds up in their order.
 // What bounds it is the chain of the softmax, and the issue of copies and matrix instructions beside it; not the tensor cores. In a loop, the
-// launch for the joins included: a prompt of 4096 tokens, 4 query heads of 256, 73 us (0.47 PFLOP/s of pairs that are seen; half of the blocks
+// launch for the joins included: a prompt of 4096 tokens, 4 query heads of 256, 74 us (0.46 PFLOP/s of pairs that are seen; half of the blocks
 // on the diagonal are not); 2000 tokens behind 7000, 32/8 heads of 128, 327 us on bf16 (0.80 PFLOP/s), 637 us on int8 (0.41), whose
 // widening warps share the issue slots with the softmax.
 #include <algorithm>
