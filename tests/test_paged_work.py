@@ -27,7 +27,7 @@ static int pages() {
 }
 
 static int spans() {
-  for (int i = 0; i < 40000; i++) {
+  for (int i = 0; i < 8000; i++) {
     const int tpt = 1 + rand() % 64, n = 1 + rand() % 200, ctx = rand() % 3 ? rand() % 1500 : 0, tile = rand() % ((n + tpt - 1) / tpt);
     const int window = rand() % 3 ? rand() % 600 : 0, sinks = window && rand() % 2 ? rand() % 400 : 0, capacity = rand() % 4 ? 4000 : 1 + rand() % 1700;
     const TileSpan t = tile_span(ctx, n, tile, tpt, window, sinks, capacity);
