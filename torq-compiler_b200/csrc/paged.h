@@ -4,11 +4,28 @@
 // The caches are [pages][page_size][n_kv * D] of one layer, bf16, or int8 with fp32 scales [pages][page_size][2 * n_kv] (of the
 // keys, then of the values): a value is its integer times its scale.
 #pragma once
+#include <stddef.h>
 #include <stdint.h>
+
+#include <initializer_list>
 
 #include "chunk_divide.h"
 
 namespace tb200 {
+
+// What an op reads while it writes must not lie under what it writes. The first `written` ranges are written, the others only read (those may
+// lie over one another); a range of no bytes is nowhere.
+struct ByteRange {
+  const void* at;
+  size_t bytes;
+};
+inline bool writes_lie_apart(std::initializer_list<ByteRange> ranges, int written) {
+  const ByteRange* r = ranges.begin();
+  for (int i = 0; i < written; i++)
+    for (int j = i + 1; j < (int)ranges.size(); j++)
+      if (r[i].bytes && r[j].bytes && (uintptr_t)r[i].at < (uintptr_t)r[j].at + r[j].bytes && (uintptr_t)r[j].at < (uintptr_t)r[i].at + r[i].bytes) return false;
+  return true;
+}
 
 // n / d for 0 <= n < 2^31: with l = ceil(log2 d) and m = floor(2^32 * (2^l - d) / d) + 1, the quotient is (mulhi(n, m) + n) >> l (the
 // round-up multiplier m + 2^32 exceeds 2^(32 + l) / d by less than 2^l / d, which no n below 2^32 turns into a step; n < 2^31 keeps

@@ -387,7 +387,13 @@ struct PagedPlan {
   PagedView v{};  // pointers are filled at dispatch
   bool i8 = false;
   size_t layer_bytes = 0, layer_scales = 0;  // byte offset of the layer in the pages, element offset in the scales
-  size_t layer_size() const { return (size_t)v.pages * v.page_size * v.n_kv * v.D * (i8 ? 1 : 2); }
+  // what lies where: a layer's pages and scales, and what says which rows and pages are whose
+  size_t slots() const { return (size_t)v.pages * v.page_size; }
+  ByteRange pages(const void* at) const { return {at, slots() * v.n_kv * v.D * (i8 ? 1 : 2)}; }
+  ByteRange scales(const void* at) const { return {at, i8 ? slots() * 2 * v.n_kv * sizeof(float) : 0}; }
+  static ByteRange row_start(const PagedView& w) { return {w.row_start, (size_t)(w.S + 1) * 4}; }
+  static ByteRange context(const PagedView& w) { return {w.context, (size_t)w.S * 4}; }
+  static ByteRange table(const PagedView& w) { return {w.table, (size_t)w.S * w.max_pages * 4}; }
 };
 bool paged_plan(Builder& b, const tb200_op_t& op, int row_start, int context, int i, const char* name, PagedPlan& c) {
   const auto& T = b.tensors;
@@ -1139,10 +1145,6 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
   };
   auto report = [](cudaError_t e, const ExecContext& c) {
     if (e != cudaSuccess && c.launch_error) *c.launch_error = e;
-  };
-  // A chunk's kernels read what they are given while they write: bindings that lie over one another are refused when they are dispatched.
-  auto apart = [](const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    return (const char*)a + a_bytes <= (const char*)b || (const char*)b + b_bytes <= (const char*)a;
   };
   struct PlannedPool { PoolArgs args; Loc x; size_t lut_off, rec_off; bool has_lut; std::function<void(const ExecContext&)> launch; };
   std::map<int, PlannedPool> pools;  // held pool ops
@@ -2174,7 +2176,7 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           step.launch = [=](const ExecContext& c) {
             const LinearRowsArgs k{(const uint16_t*)lx.resolve(c), (const int8_t*)(c.consts + w_off), (const uint16_t*)(c.consts + s_off),
                                    lo.resolve(c), y_f32, B, N, K, c.status};
-            if (!apart(k.x, (size_t)B * K * 2, k.y, (size_t)B * N * (y_f32 ? 4 : 2))) return report(cudaErrorInvalidValue, c);
+            if (!writes_lie_apart({{k.y, (size_t)B * N * (y_f32 ? 4 : 2)}, {k.x, (size_t)B * K * 2}}, 1)) return report(cudaErrorInvalidValue, c);
             report(launch_linear_rows(k, sms, c.stream), c);
           };
           break;
@@ -2326,9 +2328,9 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.scales = c.i8 ? (float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.n_q = n_q;
           k.eps = eps;
-          const size_t cache = c.layer_size(), q_bytes = (size_t)k.v.rows * n_q * k.v.D * 2;
-          if (!apart(k.k, cache, k.vv, cache) || !apart(k.q_out, q_bytes, k.qkv, q_bytes + (size_t)k.v.rows * 2 * k.v.n_kv * k.v.D * 2) ||
-              !apart(k.q_out, q_bytes, k.k, cache) || !apart(k.q_out, q_bytes, k.vv, cache))
+          const size_t rows = k.v.rows;
+          if (!writes_lie_apart({{k.q_out, rows * n_q * k.v.D * 2}, c.pages(k.k), c.pages(k.vv), c.scales(k.scales), {k.qkv, rows * (n_q + 2 * (size_t)k.v.n_kv) * k.v.D * 2},
+                                 c.row_start(k.v), c.context(k.v), c.table(k.v)}, 4))
             return report(cudaErrorInvalidValue, x);
           report(launch_rope_kv_paged(k, x.stream), x);
         };
@@ -2352,10 +2354,9 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.k_out = (uint16_t*)lk.resolve(x);
           k.v_out = (uint16_t*)lv.resolve(x);
-          const size_t cache = c.layer_size(), bytes = (size_t)k.v.rows * k.v.n_kv * k.v.D * 2;
-          for (const void* out : {(const void*)k.k_out, (const void*)k.v_out})
-            if (!apart(out, bytes, k.k, cache) || !apart(out, bytes, k.vv, cache)) return report(cudaErrorInvalidValue, x);
-          if (!apart(k.k_out, bytes, k.v_out, bytes)) return report(cudaErrorInvalidValue, x);
+          const size_t bytes = (size_t)k.v.rows * k.v.n_kv * k.v.D * 2;
+          if (!writes_lie_apart({{k.k_out, bytes}, {k.v_out, bytes}, c.pages(k.k), c.pages(k.vv), c.scales(k.scales), c.row_start(k.v), c.context(k.v), c.table(k.v)}, 2))
+            return report(cudaErrorInvalidValue, x);
           report(launch_kv_read_paged(k, x.stream), x);
         };
         break;
@@ -2396,8 +2397,8 @@ int build_plan(const std::vector<tb200_tensor_t>& tensors, const std::vector<tb2
           k.vv = (const char*)at.v.resolve(x) + c.layer_bytes;
           k.scales = c.i8 ? (const float*)at.scales.resolve(x) + c.layer_scales : nullptr;
           k.out = (uint16_t*)lo.resolve(x);
-          const size_t cache = c.layer_size(), bytes = (size_t)k.v.rows * n_q * k.v.D * 2;
-          if (!apart(k.out, bytes, k.q, bytes) || !apart(k.out, bytes, k.k, cache) || !apart(k.out, bytes, k.vv, cache))
+          const size_t bytes = (size_t)k.v.rows * n_q * k.v.D * 2;
+          if (!writes_lie_apart({{k.out, bytes}, {k.q, bytes}, c.pages(k.k), c.pages(k.vv), c.scales(k.scales), c.row_start(k.v), c.context(k.v), c.table(k.v)}, 1))
             return report(cudaErrorInvalidValue, x);
           report(launch_attn_paged(k, sms, x.scratch, x.stream), x);
         };
