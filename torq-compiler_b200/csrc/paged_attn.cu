@@ -58,7 +58,7 @@ TB200_BOTH FewShape few_shape(int D, bool i8, int stages) {
   }
   s.q_pitch = ((D + 63) / 64 * 64) * 2 + 16;
   s.stages = stages;
-  s.ring = kFewWarps * stages * kChunk * (s.k_pitch + s.v_pitch);
+  s.ring = kFewWarps * stages * kChunk * (s.k_pitch + s.v_pitch);  // 39936 at least, more than RowsScratch
   const int meet = kFewWarps * kFewRows * D * 4;  // the warps' sums take the rings' place
   s.ring = s.ring > meet ? s.ring : meet;
   s.ring = (s.ring + 15) / 16 * 16;
@@ -68,10 +68,9 @@ TB200_BOTH FewShape few_shape(int D, bool i8, int stages) {
 
 // NT: steps of 16 dims a head has at most. RT: groups of 8 rows of a tile.
 template <int NT, int RT, int STAGES, bool I8>
-__global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnPagedArgs a) {
+__global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const __grid_constant__ AttnPagedArgs a) {
   extern __shared__ __align__(16) unsigned char sm[];
   __shared__ WorkShared shared;
-  __shared__ RowScratch<kFewThreads> plain;
   __shared__ uint32_t held_bits[kFewWarps][STAGES], bad;
   const PagedView& v = a.v;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
@@ -440,13 +439,8 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const AttnP
     if (!whole && tid == 0 && here == first) write_join(a, work, w, first, used);
     __syncthreads();  // the rings are free again
     const uint32_t again = bad;
-    if (again) {  // rare: an infinity or a NaN among the values
-      for (int r = 0; r < used; r++) {
-        if (!(again >> r & 1)) continue;
-        const int tok = page_of(r, a.group_div);
-        attend_row<kFewThreads>(a, plain, tid, w.row0 + tok, w.head * group + r - tok * group, w.seq, (int)min((long long)w.first_pos + tok, 0x7fffffffll), 0, D,
-                                [] { __syncthreads(); });
-      }
+    if (again) {  // rare: an infinity or a NaN among the values (the rings have room for the scratch at every head size)
+      attend_rows<kFewThreads>(a, *reinterpret_cast<RowsScratch<kFewThreads>*>(sm), tid, {w.row0, w.head, w.seq, w.first_pos}, 0, again, 0, D, [] { __syncthreads(); });
       if (tid == 0) bad = 0;
     }
   }
@@ -463,9 +457,8 @@ struct JoinSet {
   int count, pitch;  // blocks that may have begun a shared tile; rows that partial sums have room for
   int join_rows;     // rows a block of the join takes
 };
-__global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const AttnPagedArgs a, const JoinSet many, const JoinSet few) {
+__global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const __grid_constant__ AttnPagedArgs a, const JoinSet many, const JoinSet few) {
   extern __shared__ __align__(16) unsigned char join_sm[];
-  __shared__ RowScratch<kJoinThreads> plain;
   __shared__ float4 meet[kJoinThreads];
   __shared__ float invs[kJoinRows];
   __shared__ uint32_t bad;
@@ -586,12 +579,9 @@ __global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const 
   }
   __syncthreads();
   const uint32_t again = bad;
-  for (int i = 0; i < rows; i++) {  // rare: an infinity or a NaN among the values
-    if (!(again >> i & 1)) continue;
-    const int tok = page_of(r0 + i, a.group_div);
-    attend_row<kJoinThreads>(a, plain, tid, j.row0 + tok, j.head * group + r0 + i - tok * group, j.seq, (int)min((long long)j.first_pos + tok, 0x7fffffffll),
-                             first_dim, end_dim, [] { __syncthreads(); });
-  }
+  if (again)  // rare: an infinity or a NaN among the values
+    attend_rows<kJoinThreads>(a, *reinterpret_cast<RowsScratch<kJoinThreads>*>(join_sm), tid, {j.row0, j.head, j.seq, j.first_pos}, r0, again, first_dim, end_dim,
+                              [] { __syncthreads(); });
 }
 
 // Which kernels run, and how they are cut. Sequences of up to 8 * rt rows (new tokens times query heads of a key/value head) are the kernel
@@ -680,7 +670,7 @@ cudaError_t launch_attn_paged(AttnPagedArgs a, int sms, void* scratch, cudaStrea
     const cudaError_t e = launch_attn_paged_tile(shaped(128 / group, sms, sets[0], 0, 2), stream);
     if (e != cudaSuccess) return e;
   }
-  const int join_smem = std::max(sets[0].count * sets[0].join_rows, sets[1].count * sets[1].join_rows) * (int)sizeof(float2);
+  const int join_smem = std::max(std::max(sets[0].count * sets[0].join_rows, sets[1].count * sets[1].join_rows) * (int)sizeof(float2), (int)sizeof(RowsScratch<kJoinThreads>));
   static std::atomic<unsigned long long> attr_done;
   if (first_use_on_device(attr_done)) {
     const cudaError_t e = cudaFuncSetAttribute(attn_paged_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);

@@ -43,7 +43,7 @@ static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreadsOf<false> * 128, 
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kUnit = 128 * 128;  // bytes of 128 rows of 64 bf16 values
 constexpr int kMetaBlocks = 6, kItems = 4;
-using TileRowScratch = RowScratch<kSoftmaxThreads>;  // the plain row is computed by the softmax warps
+using TileScratch = RowsScratch<kSoftmaxThreads>;  // rows are computed once more by the softmax warps
 
 struct alignas(16) Meta {
   float k_scale[kKeyBlock], v_scale[kKeyBlock];
@@ -53,14 +53,17 @@ struct alignas(16) Meta {
   // `firsts` whatever their window (here, beside the slots, and not with the item: the softmax has no register left for it)
   int key0, firsts;
 };
-static_assert(sizeof(Meta) % 16 == 0 && sizeof(TileRowScratch) % 16 == 0, "what lies behind them in shared memory is read 16 and 8 bytes at a time");
+static_assert(sizeof(Meta) % 16 == 0, "what lies behind it in shared memory is read 8 bytes at a time");
 struct Control {
   uint64_t full[16], empty[16], s_full[2], p_ready[2], pv_done, o_done, q_full, q_empty, item_full[kItems], item_empty[kItems], meta_full[kMetaBlocks], meta_empty[kMetaBlocks];
   Item items[kItems];
-  uint32_t tmem, bad_rows[4];
-  int abort, stop;
+  uint32_t tmem;
+  int abort;
+  int stop;   // of the softmax warps: 1 when there is no more work, 2 when a wait ran out
+  int again;  // a tile of this block alone has rows that came out non-finite
   float top[2][2][128];  // row maxima of the two halves, by parity of the block
   WorkShared work;
+  Work share;  // for mend_tiles
 };
 
 // two fp32 operations in one instruction
@@ -107,6 +110,38 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// Rows of the tiles that a block has done alone, and whose result is not finite, once more (rare: an infinity or a NaN among the values). By the
+// softmax warps, which have written these results.
+__device__ __noinline__ void mend_tiles(const AttnPagedArgs& a, const Control& control, TileScratch& sm, int t) {
+  auto sync = [] { named_sync(5, kSoftmaxThreads); };
+  const int group = a.n_q / a.v.n_kv, D = a.v.D;
+  const Work& work = control.share;
+  ItemCursor cursor(a, work, control.work);
+  Item w;
+  while (cursor.take(a, work, w)) {
+    if (w.b1 - w.b0 != w.blocks) continue;  // the join's
+    const int used = w.tokens * group;
+    for (int r0 = 0; r0 < used; r0 += 32) {
+      const int r = r0 + (t >> 3), tok = page_of(r, a.group_div);  // eight threads look at a row
+      bool bad = false;
+      if (r < used) {
+        const uint16_t* const row = a.out + ((long long)(w.row0 + tok) * a.n_q + w.head * group + r - tok * group) * D;
+        for (int d = (t & 7) * 8; d < D; d += 64) {
+          const uint4 x = *reinterpret_cast<const uint4*>(row + d);
+          for (uint32_t y : {x.x, x.y, x.z, x.w}) bad = bad || (y & 0x7f80u) == 0x7f80u || (y & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+      const uint32_t by8 = __ballot_sync(0xffffffffu, bad);
+      sync();
+      if ((t & 31) == 0) sm.any[t >> 5] = (by8 & 0xff ? 1u : 0u) | (by8 & 0xff00 ? 2u : 0u) | (by8 & 0xff0000 ? 4u : 0u) | (by8 >> 24 ? 8u : 0u);
+      sync();
+      uint32_t bits = 0;
+      for (int i = 0; i < kSoftmaxWarps; i++) bits |= sm.any[i] << (4 * i);
+      if (bits) attend_rows<kSoftmaxThreads>(a, sm, t, {w.row0, w.head, w.seq, w.first_pos}, r0, bits, 0, D, sync);
+    }
+  }
+}
+
 // How the copy engine sees the queries and a bf16 cache: boxes of 64 dims by the rows of a tile / by box_rows keys, and single keys.
 struct TileMaps {
   CUtensorMap q, k, v, k_rows, v_rows;
@@ -114,7 +149,7 @@ struct TileMaps {
 
 // DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
 template <int DC, int UNITS, int AHEAD, bool I8>
-__global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+__device__ __forceinline__ void attend_tiles(const AttnPagedArgs& a, const TileMaps& maps) {
   constexpr int GROUPS = UNITS / DC;  // a block's keys, or its values, lie one behind another: a group
   constexpr int kCopyWarps = kCopyWarpsOf<I8>, kCopyThreads = kCopyWarps * 32, kThreads = kThreadsOf<I8>;
   extern __shared__ unsigned char smem_raw[];
@@ -123,8 +158,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
   const uint32_t q_smem = smem_u32(base), ring = q_smem + DC * kUnit;
   unsigned char* const raw = base + (DC + UNITS) * kUnit;  // int8 pieces on their way
   Meta* const meta = reinterpret_cast<Meta*>(raw + (I8 ? AHEAD * kUnit / 2 : 0));
-  TileRowScratch& plain = *reinterpret_cast<TileRowScratch*>(meta + kMetaBlocks);
-  Control& c = *reinterpret_cast<Control*>(reinterpret_cast<unsigned char*>(&plain) + sizeof(TileRowScratch));
+  Control& c = *reinterpret_cast<Control*>(meta + kMetaBlocks);
   int* const first_tile = reinterpret_cast<int*>(base);  // while the work is shared out: tiles in front of each sequence
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -157,7 +191,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
     mbar_init(smem_u32(&c.q_empty), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     c.abort = 0;
-    c.bad_rows[0] = c.bad_rows[1] = c.bad_rows[2] = c.bad_rows[3] = 0;
+    c.again = 0;
   }
   grid_dependency_wait();
   grid_dependency_release();
@@ -165,6 +199,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
   if (tid == 0) a.joins[blockIdx.x].parts = 0;
   const Work work = share_out<kThreads>(a, c.work, first_tile);
   const bool works = work.works;
+  if (tid == 0) c.share = work;  // (kept in a register it would cost the softmax one)
   tc_fence_before();
   __syncthreads();  // the first item is known, and first_tile's room is free
   tc_fence_after();
@@ -473,7 +508,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
     for (;; items++) {
       if (tid == 0) {  // one decides for all, who meet at barriers from here on
         const Item& w = take_item(items);
-        c.stop = gave_up || *(volatile int*)&c.abort || !w.tokens;
+        c.stop = gave_up || *(volatile int*)&c.abort ? 2 : !w.tokens;
       }
       named_sync(5, kSoftmaxThreads);
       if (c.stop) break;
@@ -629,7 +664,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
       const bool mine = row < used;
       const int my_row = w.row0 + tok, my_head = w.head * group + row - tok * group;
       uint16_t* const dst = a.out + ((long long)my_row * a.n_q + my_head) * D;
-      bool finite = l != 0.f || m == -INFINITY;  // sums of a row are fit to be used
+      bool finite = true;
       const bool whole = n == w.blocks;
       float* to = nullptr;  // partial sums: [four columns][row][4] and (base, l) of every row, in one of this block's two places
       if (!whole) {
@@ -638,7 +673,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
         if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
         if (tid == 0 && here == first) write_join(a, work, w, first, used);
       }
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const bool none = l == 0.f && m == -INFINITY;  // the row saw no key
+      const float inv = l > 0.f ? 1.f / l : __int_as_float(0x7fc00000);
       if (warp_used) {
 #pragma unroll 1
         for (int i = 32 * half; i < D; i += 64) {
@@ -658,7 +694,7 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
             uint32_t p[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const float x = l == 0.f ? 0.f : __uint_as_float(o[j + 2 * k]) * inv, y = l == 0.f ? 0.f : __uint_as_float(o[j + 2 * k + 1]) * inv;
+              const float x = none ? 0.f : __uint_as_float(o[j + 2 * k]) * inv, y = none ? 0.f : __uint_as_float(o[j + 2 * k + 1]) * inv;
               finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
               p[k] = pack_bf16(x, y);
             }
@@ -666,24 +702,14 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
           }
         }
       }
-      if (whole) {
-        if (mine && !finite) atomicOr(&c.bad_rows[row >> 5], 1u << (row & 31));
-        named_sync(5, kSoftmaxThreads);
-        const uint32_t bad[4] = {c.bad_rows[0], c.bad_rows[1], c.bad_rows[2], c.bad_rows[3]};
-        if (bad[0] | bad[1] | bad[2] | bad[3]) {  // rare: an infinity or a NaN among the values
-          auto sync = [] { named_sync(5, kSoftmaxThreads); };
-          for (int r = 0; r < used; r++) {
-            if (!(bad[r >> 5] >> (r & 31) & 1)) continue;
-            const int tk = page_of(r, a.group_div);
-            attend_row<kSoftmaxThreads>(a, plain, tid, w.row0 + tk, w.head * group + r - tk * group, w.seq, (int)min((long long)first_pos + tk, 0x7fffffffll), 0, D, sync);
-          }
-          if (tid < 4) c.bad_rows[tid] = 0;
-        }
-      }
+      if (whole && mine && !finite) c.again = 1;
       tc_fence_before();
-      named_sync(5, kSoftmaxThreads);  // everybody has read O, the exchange and the flags
+      named_sync(5, kSoftmaxThreads);  // everybody has read O and the exchange
       release_item(items);
     }
+    // All other roles are through, so no wait's limit runs while this goes on; and what was asked for has been copied and multiplied, so the
+    // room of queries and units is free.
+    if (c.again && c.stop == 1) mend_tiles(a, c, *reinterpret_cast<TileScratch*>(base), tid);
     }
   }
   tc_fence_before();
@@ -697,6 +723,18 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
+}
+
+// mend_tiles takes the arguments by address. bf16: from where the launch has put them (by way of a copy on the stack the prompt of 4096 takes 70 us instead
+// of 66). int8, whose softmax has no register to spare: from such a copy, which the compiler then spills around (252 us for 1999 rows of five chunks, 32/8
+// heads of 128, instead of 266).
+template <int DC, int UNITS, int AHEAD>
+__global__ void __launch_bounds__(kThreadsOf<false>, 1) attn_paged_tile_kernel(const __grid_constant__ AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+  attend_tiles<DC, UNITS, AHEAD, false>(a, maps);
+}
+template <int DC, int UNITS, int AHEAD>
+__global__ void __launch_bounds__(kThreadsOf<true>, 1) attn_paged_tile_i8_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
+  attend_tiles<DC, UNITS, AHEAD, true>(a, maps);
 }
 
 // A bf16 tensor [outer][heads][D], fetched in boxes of 64 dims by box_heads by box_outer.
@@ -724,11 +762,12 @@ bool encode_rows(CUtensorMap* map, const void* base, uint64_t rows, int D) {
 
 template <int DC, int UNITS, int AHEAD, bool I8>
 cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
-  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? AHEAD * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(TileRowScratch) + (int)sizeof(Control);
+  constexpr int smem = 1024 + (DC + UNITS) * kUnit + (I8 ? AHEAD * kUnit / 2 : 0) + kMetaBlocks * (int)sizeof(Meta) + (int)sizeof(Control);
+  static_assert((DC + UNITS) * kUnit >= (int)sizeof(TileScratch), "room for rows that are computed once more");
   static_assert(smem <= 227 * 1024, "shared memory");
   static_assert(UNITS % DC == 0, "a block's units lie one behind another");
   static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
-  auto kernel = attn_paged_tile_kernel<DC, UNITS, AHEAD, I8>;
+  auto kernel = I8 ? attn_paged_tile_i8_kernel<DC, UNITS, AHEAD> : attn_paged_tile_kernel<DC, UNITS, AHEAD>;
   static std::atomic<unsigned long long> attr_done;
   if (first_use_on_device(attr_done)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
