@@ -428,9 +428,9 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const __gri
         if (q == 0) *reinterpret_cast<float2*>(to + D * kFewRows + row * 2) = make_float2(top, all);
         continue;
       }
-      const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);
+      const float inv = all > 0.f ? 1.f / all : (all == 0.f ? 0.f : all);  // no weights: no key seen, or none with a score above -inf
       x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
-      if (!(fabsf(x.x) <= 3.0e38f && fabsf(x.y) <= 3.0e38f && fabsf(x.z) <= 3.0e38f && fabsf(x.w) <= 3.0e38f) || (all == 0.f && top != -INFINITY))
+      if (!(fabsf(x.x) <= 3.0e38f && fabsf(x.y) <= 3.0e38f && fabsf(x.z) <= 3.0e38f && fabsf(x.w) <= 3.0e38f) || all == 0.f)
         atomicOr(&bad, 1u << row);
       const int tok = page_of(row, a.group_div);
       *reinterpret_cast<uint2*>(a.out + ((long long)(w.row0 + tok) * a.n_q + w.head * group + row - tok * group) * D + q * 4) =
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kFewThreads) attn_paged_few_kernel(const __gri
     if (!whole && tid == 0 && here == first) write_join(a, work, w, first, used);
     __syncthreads();  // the rings are free again
     const uint32_t again = bad;
-    if (again) {  // rare: an infinity or a NaN among the values (the rings have room for the scratch at every head size)
+    if (again) {  // rare: an infinity or a NaN among the values, a row without a key (the rings have room for the scratch at every head size)
       attend_rows<kFewThreads>(a, *reinterpret_cast<RowsScratch<kFewThreads>*>(sm), tid, {w.row0, w.head, w.seq, w.first_pos}, 0, again, 0, D, [] { __syncthreads(); });
       if (tid == 0) bad = 0;
     }
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const 
     for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sub == 0) {
       invs[r] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-      if (r < rows && sum == 0.f && top != -INFINITY) atomicOr(&bad, 1u << r);
+      if (r < rows && sum == 0.f) atomicOr(&bad, 1u << r);
     }
   }
   __syncthreads();
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kJoinThreads, 4) attn_paged_join_kernel(const 
   }
   __syncthreads();
   const uint32_t again = bad;
-  if (again)  // rare: an infinity or a NaN among the values
+  if (again)  // rare: an infinity or a NaN among the values, a row without a key
     attend_rows<kJoinThreads>(a, *reinterpret_cast<RowsScratch<kJoinThreads>*>(join_sm), tid, {j.row0, j.head, j.seq, j.first_pos}, r0, again, first_dim, end_dim,
                               [] { __syncthreads(); });
 }

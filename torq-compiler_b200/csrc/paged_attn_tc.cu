@@ -36,8 +36,8 @@ template <bool I8>
 constexpr int kCopyWarpsOf = I8 ? 8 : 4;  // four widening warps took twice as long over a block as all else
 template <bool I8>
 constexpr int kThreadsOf = (kSoftmaxWarps + kCopyWarpsOf<I8> + 4) * 32;
-// a block starts with 128 (bf16) or 96 (int8) registers a thread
-constexpr int kSoftmaxRegs = 200, kSoftmaxRegsI8 = 144, kCopyRegsI8 = 64, kIssueRegs = 56;
+// a block starts with 128 (bf16) or 96 (int8) registers a thread (int8, 1999 rows of five chunks, 32/8 heads of 128: 248 us so, 258 with 144 and 64)
+constexpr int kSoftmaxRegs = 200, kSoftmaxRegsI8 = 152, kCopyRegsI8 = 56, kIssueRegs = 56;
 static_assert(256 * kSoftmaxRegsI8 + 256 * kCopyRegsI8 + 128 * kIssueRegs <= kThreadsOf<true> * 96, "register split, int8");
 static_assert(256 * kSoftmaxRegs + 256 * kIssueRegs <= kThreadsOf<false> * 128, "register split, bf16");
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
@@ -110,8 +110,8 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Rows of the tiles that a block has done alone, and whose result is not finite, once more (rare: an infinity or a NaN among the values). By the
-// softmax warps, which have written these results.
+// Rows of the tiles that a block has done alone, and whose result is not finite, once more (rare: an infinity or a NaN among the values, a row without
+// a key). By the softmax warps, which have written these results.
 __device__ __noinline__ void mend_tiles(const AttnPagedArgs& a, const Control& control, TileScratch& sm, int t) {
   auto sync = [] { named_sync(5, kSoftmaxThreads); };
   const int group = a.n_q / a.v.n_kv, D = a.v.D;
@@ -147,9 +147,10 @@ struct TileMaps {
   CUtensorMap q, k, v, k_rows, v_rows;
 };
 
-// DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory.
+// DC: units (64 dims) of a head. UNITS: ring of keys' and values' units in shared memory. (mend_tiles takes the arguments by address: from where the
+// launch has put them the prompt of 4096 takes 67 us, by way of a copy on the stack 70.)
 template <int DC, int UNITS, int AHEAD, bool I8>
-__device__ __forceinline__ void attend_tiles(const AttnPagedArgs& a, const TileMaps& maps) {
+__global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(const __grid_constant__ AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
   constexpr int GROUPS = UNITS / DC;  // a block's keys, or its values, lie one behind another: a group
   constexpr int kCopyWarps = kCopyWarpsOf<I8>, kCopyThreads = kCopyWarps * 32, kThreads = kThreadsOf<I8>;
   extern __shared__ unsigned char smem_raw[];
@@ -673,7 +674,7 @@ __device__ __forceinline__ void attend_tiles(const AttnPagedArgs& a, const TileM
         if (mine && half == 0) *reinterpret_cast<float2*>(to + D * 128 + row * 2) = make_float2(m == -INFINITY ? m : base, l);
         if (tid == 0 && here == first) write_join(a, work, w, first, used);
       }
-      const bool none = l == 0.f && m == -INFINITY;  // the row saw no key
+      // no weights (no key seen, or none with a score above -inf): not finite, and seen to behind
       const float inv = l > 0.f ? 1.f / l : __int_as_float(0x7fc00000);
       if (warp_used) {
 #pragma unroll 1
@@ -694,7 +695,7 @@ __device__ __forceinline__ void attend_tiles(const AttnPagedArgs& a, const TileM
             uint32_t p[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const float x = none ? 0.f : __uint_as_float(o[j + 2 * k]) * inv, y = none ? 0.f : __uint_as_float(o[j + 2 * k + 1]) * inv;
+              const float x = __uint_as_float(o[j + 2 * k]) * inv, y = __uint_as_float(o[j + 2 * k + 1]) * inv;
               finite = finite && fabsf(x) <= 3.0e38f && fabsf(y) <= 3.0e38f;
               p[k] = pack_bf16(x, y);
             }
@@ -723,18 +724,6 @@ __device__ __forceinline__ void attend_tiles(const AttnPagedArgs& a, const TileM
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
-}
-
-// mend_tiles takes the arguments by address. bf16: from where the launch has put them (by way of a copy on the stack the prompt of 4096 takes 70 us instead
-// of 66). int8, whose softmax has no register to spare: from such a copy, which the compiler then spills around (252 us for 1999 rows of five chunks, 32/8
-// heads of 128, instead of 266).
-template <int DC, int UNITS, int AHEAD>
-__global__ void __launch_bounds__(kThreadsOf<false>, 1) attn_paged_tile_kernel(const __grid_constant__ AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
-  attend_tiles<DC, UNITS, AHEAD, false>(a, maps);
-}
-template <int DC, int UNITS, int AHEAD>
-__global__ void __launch_bounds__(kThreadsOf<true>, 1) attn_paged_tile_i8_kernel(const AttnPagedArgs a, const __grid_constant__ TileMaps maps) {
-  attend_tiles<DC, UNITS, AHEAD, true>(a, maps);
 }
 
 // A bf16 tensor [outer][heads][D], fetched in boxes of 64 dims by box_heads by box_outer.
@@ -767,7 +756,7 @@ cudaError_t run_tile(const AttnPagedArgs& a, cudaStream_t stream) {
   static_assert(smem <= 227 * 1024, "shared memory");
   static_assert(UNITS % DC == 0, "a block's units lie one behind another");
   static_assert((DC + UNITS) * kUnit >= (4096 + 1) * 4, "room for the sequences' first tiles");
-  auto kernel = I8 ? attn_paged_tile_i8_kernel<DC, UNITS, AHEAD> : attn_paged_tile_kernel<DC, UNITS, AHEAD>;
+  auto kernel = attn_paged_tile_kernel<DC, UNITS, AHEAD, I8>;
   static std::atomic<unsigned long long> attr_done;
   if (first_use_on_device(attr_done)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -37,6 +37,7 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
     sync();
     if ((t & 31) == 0) sm.any[warp] = x;
     sync();
+#pragma unroll 1
     for (int i = 0; i < THREADS / 32; i++) x |= sm.any[i];
     return x;
   };
@@ -45,10 +46,27 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
   while (lanes * 4 < D) lanes *= 2;
   const int d = (t & (lanes - 1)) * 4, key_step = THREADS / lanes, first_key = t / lanes;
   const bool on = d < D && d >= d0 && d < d1;
+  {  // a sequence without pages (an idle one of a batch, say): zeros at once
+    const int newest = (int)min((long long)w.first_pos + page_of(r0 + 31 - __clz(bits), a.group_div), v.capacity - 1ll);
+    uint32_t held = 0;
+#pragma unroll 1
+    for (int i = t; i <= page_of(newest, v.div); i += THREADS) held |= (unsigned)pages_of[i] < (unsigned)v.pages;
+    if (!all_or(held)) {
+#pragma unroll 1
+      for (int i = warp; i < 32; i += THREADS / 32) {
+        const int tok = page_of(r0 + i, a.group_div);
+        uint16_t* const to = a.out + ((long long)(w.row0 + tok) * a.n_q + w.head * group + r0 + i - tok * group) * D;
+        for (int k = d0 + (t & 31) * 4; (bits >> i & 1) && k < d1; k += 128) *reinterpret_cast<uint2*>(to + k) = make_uint2(0, 0);
+      }
+      sync();
+      return;
+    }
+  }
   while (bits) {
     sync();
     if (t < kPlainRows) {
       uint32_t left = bits;
+#pragma unroll 1
       for (int i = 0; i < t; i++) left &= left - 1;
       const int r = left ? r0 + __ffs(left) - 1 : -1, tok = r < 0 ? 0 : page_of(r, a.group_div);
       const int pos = r < 0 ? -1 : (int)min((long long)w.first_pos + tok, 0x7fffffffll);
@@ -57,19 +75,20 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
       sm.near_key[t] = a.window ? max(0, pos - a.window + 1) : 0;
     }
     sync();
+#pragma unroll 1
     for (int i = 0; i < kPlainRows; i++) bits &= bits - 1;
     int last = -1, near_first = 0x7fffffff;
+#pragma unroll 1
     for (int i = 0; i < kPlainRows; i++) {
       if (sm.at[i] < 0) continue;
       last = max(last, sm.pos[i]);
       near_first = min(near_first, sm.near_key[i]);
     }
     last = min(last, v.capacity - 1);
+#pragma unroll 1
     for (int i = 0; i < kPlainRows; i++)
       for (int k = t; k < D; k += THREADS) sm.q[i][k] = sm.at[i] < 0 ? 0.f : paged_bf2f(a.q[(long long)sm.at[i] * D + k]) * a.scale;
-    uint32_t held = 0;
-    for (int i = t; i <= page_of(last, v.div); i += THREADS) held |= (unsigned)pages_of[i] < (unsigned)v.pages;
-    if (!all_or(held)) last = -1;  // a sequence without pages
+    sync();
 
     float m[kPlainRows], sum[kPlainRows], o[kPlainRows][4] = {};
     uint32_t saw = 0;
@@ -80,8 +99,8 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
       if (j0 >= a.sinks) j0 = max(j0, near_first & -THREADS);
       const int j = j0 + t;
       uint32_t seen = 0;
-      if (j <= last)
-        for (int i = 0; i < kPlainRows; i++) seen |= (j <= sm.pos[i] && (j >= sm.near_key[i] || j < a.sinks) ? 1u : 0u) << i;
+#pragma unroll 1
+      for (int i = 0; i < kPlainRows && j <= last; i++) seen |= (j <= sm.pos[i] && (j >= sm.near_key[i] || j < a.sinks) ? 1u : 0u) << i;
       const int slot = seen ? (int)slot_of(v, w.seq, j) : -1;
       if (slot < 0) seen = 0;
       saw |= seen;
@@ -170,6 +189,7 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
       for (int off = 16; off > 0; off >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
       if ((t & 31) == 0) sm.red[warp][i] = sum[i];
     }
+#pragma unroll 1
     for (int g = 0; g < key_step; g++) {
       if (on && first_key == g) {
 #pragma unroll
@@ -180,9 +200,11 @@ __device__ __noinline__ void attend_rows(const AttnPagedArgs& a, RowsScratch<THR
       sync();
     }
     if (on && first_key == 0) {
+#pragma unroll 1
       for (int i = 0; i < kPlainRows; i++) {
         if (sm.at[i] < 0) continue;
         float all = 0.f;
+#pragma unroll 1
         for (int k = 0; k < THREADS / 32; k++) all += sm.red[k][i];
         // a row that sees no key is all zeros; one whose scores are all -inf has no weights
         auto value = [&](int e) { return saw >> i & 1 ? sm.q[i][d + e] / all : 0.f; };
