@@ -201,6 +201,8 @@ __global__ void __launch_bounds__(kThreadsOf<I8>, 1) attn_paged_tile_kernel(cons
   const Work work = share_out<kThreads>(a, c.work, first_tile);
   const bool works = work.works;
   if (tid == 0) c.share = work;  // (kept in a register it would cost the softmax one)
+  // first_tile lies where queries and units will be: the copy engine's writes come behind every thread's accesses to it
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();  // the first item is known, and first_tile's room is free
   tc_fence_after();
