@@ -61,6 +61,10 @@ struct Shape {
   static constexpr int a_stages = std::min(8, (512 - HALVES * XN) / a_columns);
   static constexpr int smem = 1024 + stages * stage_bytes + kFinishWarps * kPatch;
   static_assert(stage_bytes % 1024 == 0 && a_stages >= 2 && XN % 64 == 0 && XN <= 256, "tile");
+  // A team sees every team_step-th step. It tells a stage's copies from the ones before by one bit, which takes that it sees all of that stage's, or
+  // that the ones before have been multiplied when it comes to wait (it has waited for room of its last step, a_stages behind).
+  static constexpr int team_step = kWidenTeams / HALVES;
+  static_assert(stages % team_step == 0 || team_step + a_stages <= stages, "phases told apart");
 };
 
 template <int HALVES, int XN>
