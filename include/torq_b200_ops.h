@@ -99,8 +99,9 @@ enum tb200_op_kind {
    * not seen, reads of it give zeros. Sequences may share pages that are read; where two rows of a chunk are written to one place, either (or
    * a mixture, 16 bytes at a time) may last. Caches: shift slot = keys, table slot = values, [layers, pages, page_size, kv * D], bf16, or
    * int8 with fp32 scales [layers, pages, page_size, 2 * kv] (bias slot; of the keys, then of the values): bound or state tensors that the
-   * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. A dispatch whose results are bound over
-   * what such an op reads (or keys over values, when they are written) ends with an error before anything of the op runs. */
+   * ops read and write in place. i1 = kv heads, i2 = D (a multiple of 16 up to 256), pad_t = layer. A dispatch that binds what such an op writes
+   * (its results, and the layer's keys, values and scales where they are written) over anything else that the op reads or writes
+   * ends with an error before anything of the op runs. */
   TB200_OP_ROPE_KV_PAGED = 43,/* in0 = qkv [rows, (i0 + 2 kv) * D] -> out0 = rotated queries [rows, i0 * D]; keys and values go to their pages.
                                * weights = bf16 norms [2, D] of queries and keys (x * rsqrt(mean(x^2) + f1) * (1 + w)) or -1; f0 = RoPE base >= 1.
                                * fp32 inside, rounded once. int8: scale = amax / 127 of a token's head, nearest integer; a head with
@@ -108,8 +109,10 @@ enum tb200_op_kind {
   TB200_OP_KV_READ_PAGED = 44,/* out0 / out1 = keys / values [rows, kv * D] bf16 of the tokens at those positions (in0 = row_start, in1 = context) */
   TB200_OP_ATTN_PAGED = 45,   /* in0 = queries [rows, i0 * D] -> out0 of the same shape: softmax(f0 * q k^T) v over the keys j <= p, and with
                                * i3 = window > 0 only j > p - window or j < pad_b (first tokens that stay visible). Keys of masked
-                               * places count for nothing whatever they hold; a row that sees no key gets zeros. pad_l > 0: a promise
-                               * that no sequence has more new rows (those behind are left as they were). */
+                               * places count for nothing whatever they hold; a row that sees no key gets zeros, one whose visible scores are
+                               * all -inf NaN. pad_l > 0: a promise that no sequence has more new rows (those behind are left as they were).
+                               * fp32 inside, rounded once, but for the weights: of sequences of few rows (with pad_l * i0 / i1 <= 16 all are) they
+                               * meet the values as two bf16 terms (2^-16 of a weight is lost), of others as one (2^-8). */
   /* tensor ops outside the layer set: what the reference's fixtures exercise around the layers
    * (tests/testdata/tosa_ops: cast-*, Elementwise_*, rescale-*, transpose-*, pad_*, identity-stride-offset-*,
    * reduce-*, argmax-*). Dense row-major tensors of rank <= 4, element types i8 / i16 / i32 / f32 / bf16;

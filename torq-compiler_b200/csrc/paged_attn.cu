@@ -8,7 +8,7 @@
 // bf16 terms (2^-17 of it is lost). int8 caches are widened in registers: keys 16 bytes to a thread, the order of the dims inside a step being
 // free as long as the queries follow it; values 2 bytes a tile of 16 dims, dims 8 apart in steps of D / 8. Warps meet in shared memory, in their
 // order. Tiles that several blocks share are joined by the launch behind. With it, from memory: one token behind 1024 (4/1 heads of 256) 17 us, 32
-// sequences of up to 8000 tokens (32/8 heads of 128, int8) 96 us, at 54 % of the issue slots.
+// sequences of up to 8000 tokens (32/8 heads of 128, int8) 86 us, at 52 % of the issue slots.
 #include <algorithm>
 
 #include "dependent_launch.cuh"

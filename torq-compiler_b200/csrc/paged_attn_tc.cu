@@ -3,6 +3,9 @@
 // A tile is 128 rows: up to 128 / group tokens with the query heads of one key/value head. Per block of 128 keys: S = Q K^T into TMEM
 // (fp32), softmax in registers against a running maximum, P as bf16 back into TMEM, O += P V with P as the TMEM operand. S is double
 // buffered, so the product of the next block runs while this block's softmax does; O (up to 256 columns) and both S fill TMEM.
+// P is one bf16 a weight (half a step off, each by itself, while the row's sum is of the unrounded ones): results are off by 0.0021 to 0.0024, relative,
+// where rounding the result alone gives 0.0017. A second term, as the kernel for few rows has it, would double the products with V and what the
+// softmax, which bounds this kernel, has to convert and store.
 //   p = 2^((s - m) scale log2 e), sums in fp32; m is the row's maximum, but follows it only when it has grown by more than 2^8 in
 //   p (O and the sum are scaled then): a bound serves as well as the maximum itself, and most blocks leave O alone.
 // Warps: eight for softmax (two to a row quarter, half a row's keys each); four that ask the copy engine for bf16 keys and values, or eight that
@@ -13,8 +16,8 @@
 // Work is shared out evenly: all tiles' key blocks in one row, every block of the grid takes an equal piece. A tile that falls to several
 // leaves partial sums in memory, which the launch behind adds up in their order.
 // What bounds it is the chain of the softmax, and the issue of copies and matrix instructions beside it; not the tensor cores. In a loop, the
-// launch for the joins included: a prompt of 4096 tokens, 4 query heads of 256, 74 us (0.46 PFLOP/s of pairs that are seen; half of the blocks
-// on the diagonal are not); 2000 tokens behind 7000, 32/8 heads of 128, 327 us on bf16 (0.80 PFLOP/s), 637 us on int8 (0.41), whose
+// launch for the joins included: a prompt of 4096 tokens, 4 query heads of 256, 67 us (0.51 PFLOP/s of pairs that are seen; half of the blocks
+// on the diagonal are not); 2000 tokens behind 7000, 32/8 heads of 128, 331 us on bf16 (0.79 PFLOP/s), 655 us on int8 (0.40), whose
 // widening warps share the issue slots with the softmax.
 #include <algorithm>
 

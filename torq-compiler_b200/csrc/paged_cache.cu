@@ -49,7 +49,7 @@ __device__ __forceinline__ int sequence_from(const PagedView& v, int s, int row)
 // power of two from D / 16 on), eight neighbouring values of each half to a lane, so that every access has 16 bytes. A warp takes the same
 // `per` heads of 32 / L rows one after another: its branches are then the same for all lanes, a row's angles and the norm's weights are
 // fetched once for several heads, and four heads are on their way while one is worked on (one ahead: 28.7 us against 22.7 for 16384 rows of 4/1 heads
-// of 256 into bf16, 101 MB; 4001 rows of 32/8 heads of 128 with norms into int8, 90 MB, take 29 us, at 64 % of the issue slots).
+// of 256 into bf16, 101 MB; 4001 rows of 32/8 heads of 128 with norms into int8, 90 MB, take 29 us, at 66 % of the issue slots).
 constexpr int kAhead = 4;
 template <int L>
 __global__ void __launch_bounds__(128) rope_kv_paged_kernel(const RopePagedArgs a) {
